@@ -8,7 +8,7 @@ CPU fallback: loading fails loudly when the library is missing.
 """
 from . import native  # noqa: F401
 from .native import (  # noqa: F401
-    LIBRARY_PATH, DeviceBuffer, MLK_F32, MLK_Q4, MLK_Q8, NativeError, load)
+    LIBRARY_PATH, DeviceBuffer, MLK_BF16, MLK_F32, MLK_Q4, MLK_Q8, NativeError, load)
 
 __all__ = ["native", "load", "DeviceBuffer", "NativeError", "LIBRARY_PATH",
-           "MLK_F32", "MLK_Q8", "MLK_Q4"]
+           "MLK_F32", "MLK_Q8", "MLK_Q4", "MLK_BF16"]

@@ -1,0 +1,358 @@
+// fp8_rows.hip -- rows and matrices quantised to e4m3 with block scales
+// (gfx950, wave64).
+//
+// A block's scale is s = max(amax / 448, 2^-126), amax the largest magnitude in
+// it; a code is the e4m3 value nearest to x * (1 / s), ties to even.  The two
+// quotients and the product are rounded in f32, so that the codes are a function
+// of the inputs' bits: x * (1 / s) lies within 3 half steps of f32 of x / s, and
+// an x at the border of two codes may take either.  The largest product is at
+// most 448 (1 + 2^-22), which rounds to 448.  A NaN keeps to its own code (it
+// takes no part in amax); an infinity gives its block an infinite scale, with
+// which every value of the block reads as NaN.
+//
+// All three are bound by memory: 16 lanes hold a block of 128 columns, 8 values
+// a lane, so a wave reads 2 KB (f32) or 1 KB (bf16) of a row in one piece and
+// stores its codes 8 bytes a lane.
+#include "fp8.h"
+#include "mlh_device.h"
+#include "mlh_host.h"
+
+#include <math.h>
+
+namespace mlh {
+
+namespace {
+
+constexpr int kThreads = 256;
+constexpr int kVec = 8;                       // values of a lane
+constexpr int kLanes = kFp8Block / kVec;      // lanes of a block
+constexpr int kGroups = kThreads / kLanes;    // blocks a workgroup holds at once
+constexpr int kSpan = kThreads * kVec;        // columns a workgroup holds at once
+
+template <bool BF16> struct Elem { using type = float; };
+template <> struct Elem<true> { using type = uint16_t; };
+
+__device__ __forceinline__ float bf16_value(unsigned bits) { return __uint_as_float(bits << 16); }
+
+// to the nearest bf16, ties to even; a NaN stays one
+__device__ __forceinline__ unsigned bf16_bits(float v) {
+    const unsigned u = __float_as_uint(v);
+    if (v != v) return (u >> 16) | 0x40u;
+    return (u + 0x7FFFu + ((u >> 16) & 1u)) >> 16;
+}
+
+// Columns c .. c + 7 of a row, zeros from `cols` on.  WIDE: cols % 8 == 0 and
+// 16-byte aligned rows.
+template <bool BF16, bool WIDE>
+__device__ __forceinline__ void load_cols(float (&v)[kVec], const typename Elem<BF16>::type *row,
+                                          int c, int cols) {
+    if constexpr (WIDE) {
+        if (c < cols) {
+            if constexpr (BF16) {
+                const u32x4 u = *reinterpret_cast<const u32x4 *>(row + c);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    v[2 * i] = __uint_as_float(u[i] << 16);
+                    v[2 * i + 1] = __uint_as_float(u[i] & 0xFFFF0000u);
+                }
+            } else {
+                const f32x4 a = load_f4(row + c), b = load_f4(row + c + 4);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    v[i] = a[i];
+                    v[4 + i] = b[i];
+                }
+            }
+            return;
+        }
+#pragma unroll
+        for (int i = 0; i < kVec; ++i) v[i] = 0.0f;
+    } else {
+#pragma unroll
+        for (int i = 0; i < kVec; ++i) {
+            v[i] = 0.0f;
+            if (c + i < cols) {
+                if constexpr (BF16) v[i] = bf16_value(row[c + i]);
+                else v[i] = row[c + i];
+            }
+        }
+    }
+}
+
+template <bool BF16, bool WIDE>
+__device__ __forceinline__ void store_cols(const float (&v)[kVec], typename Elem<BF16>::type *row,
+                                           int c, int cols) {
+    if constexpr (WIDE) {
+        if (c >= cols) return;
+        if constexpr (BF16) {
+            u32x4 u;
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                u[i] = bf16_bits(v[2 * i]) | (bf16_bits(v[2 * i + 1]) << 16);
+            *reinterpret_cast<u32x4 *>(row + c) = u;
+        } else {
+            *reinterpret_cast<f32x4 *>(row + c) = f32x4{v[0], v[1], v[2], v[3]};
+            *reinterpret_cast<f32x4 *>(row + c + 4) = f32x4{v[4], v[5], v[6], v[7]};
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < kVec; ++i) {
+            if (c + i < cols) {
+                if constexpr (BF16) row[c + i] = (uint16_t)bf16_bits(v[i]);
+                else row[c + i] = v[i];
+            }
+        }
+    }
+}
+
+__device__ __forceinline__ float amax8(const float (&v)[kVec]) {
+    float m = 0.0f;
+#pragma unroll
+    for (int i = 0; i < kVec; ++i) m = fmaxf(m, fabsf(v[i]));  // fmaxf passes NaN by
+    return m;
+}
+
+__device__ __forceinline__ float group_max(float m) {
+#pragma unroll
+    for (int o = kLanes / 2; o >= 1; o >>= 1) m = fmaxf(m, __shfl_xor(m, o, kWave));
+    return m;
+}
+
+__device__ __forceinline__ float scale_of(float amax) {
+    return fmaxf(amax / kFp8Top, kFp8TinyScale);
+}
+
+template <bool WIDE>
+__device__ __forceinline__ void store_codes(const float (&v)[kVec], float inv, uint8_t *row, int c,
+                                            int cols) {
+    unsigned w[2];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        int u = __builtin_amdgcn_cvt_pk_fp8_f32(v[4 * h] * inv, v[4 * h + 1] * inv, 0, false);
+        u = __builtin_amdgcn_cvt_pk_fp8_f32(v[4 * h + 2] * inv, v[4 * h + 3] * inv, u, true);
+        w[h] = (unsigned)u;
+    }
+    if constexpr (WIDE) {
+        if (c < cols) *reinterpret_cast<uint2 *>(row + c) = make_uint2(w[0], w[1]);
+    } else {
+#pragma unroll
+        for (int i = 0; i < kVec; ++i)
+            if (c + i < cols) row[c + i] = (uint8_t)(w[i / 4] >> (8 * (i % 4)));
+    }
+}
+
+// silu(g) * u in this order: g u may leave f32's range where silu(g) u does not
+__device__ __forceinline__ void swiglu8(float (&g)[kVec], const float (&u)[kVec]) {
+#pragma unroll
+    for (int i = 0; i < kVec; ++i) g[i] = silu(g[i]) * u[i];
+}
+
+// Blocks of 1 x 128, each on its own: plain rows, or gate and up halves.
+template <bool BF16, bool WIDE, bool SWIGLU>
+__global__ __launch_bounds__(kThreads) void fp8_rows_kernel(const typename Elem<BF16>::type *x,
+                                                            int rows, int cols, uint8_t *q,
+                                                            float *scale) {
+    const unsigned per_row = (unsigned)((cols + kFp8Block - 1) / kFp8Block);
+    const unsigned total = per_row * (unsigned)rows;
+    const int lane = threadIdx.x % kLanes;
+    for (unsigned b = blockIdx.x * kGroups + threadIdx.x / kLanes; b < total;
+         b += gridDim.x * kGroups) {
+        const unsigned row = b / per_row, cb = b - row * per_row;
+        const int c = (int)cb * kFp8Block + lane * kVec;
+        float v[kVec];
+        const auto *src = x + (long)row * cols * (SWIGLU ? 2 : 1);
+        load_cols<BF16, WIDE>(v, src, c, cols);
+        if constexpr (SWIGLU) {
+            float u[kVec];
+            load_cols<BF16, WIDE>(u, src + cols, c, cols);
+            swiglu8(v, u);
+        }
+        const float s = scale_of(group_max(amax8(v)));
+        if (lane == 0) scale[b] = s;
+        store_codes<WIDE>(v, 1.0f / s, q + (long)row * cols, c, cols);
+    }
+}
+
+// One 128 x 128 block per workgroup: 8 passes of 16 rows, held in registers.
+template <bool BF16, bool WIDE>
+__global__ __launch_bounds__(kThreads) void fp8_matrix_kernel(const typename Elem<BF16>::type *x,
+                                                              int rows, int cols, uint8_t *q,
+                                                              float *scale) {
+    constexpr int kPasses = kFp8Block / kGroups;
+    __shared__ float red[kThreads / kWave];
+    const unsigned per_row = (unsigned)((cols + kFp8Block - 1) / kFp8Block);
+    const unsigned rb = blockIdx.x / per_row, cb = blockIdx.x - rb * per_row;
+    const int c = (int)cb * kFp8Block + (int)(threadIdx.x % kLanes) * kVec;
+    const long r0 = (long)rb * kFp8Block + threadIdx.x / kLanes;
+    float v[kPasses][kVec], m = 0.0f;
+#pragma unroll
+    for (int p = 0; p < kPasses; ++p) {
+        const long r = r0 + p * kGroups;
+        load_cols<BF16, WIDE>(v[p], x + (r < rows ? r : 0) * cols, c, r < rows ? cols : 0);
+        m = fmaxf(m, amax8(v[p]));
+    }
+    m = wave_max(m);
+    if (threadIdx.x % kWave == 0) red[threadIdx.x / kWave] = m;
+    __syncthreads();
+    m = red[0];
+#pragma unroll
+    for (int w = 1; w < kThreads / kWave; ++w) m = fmaxf(m, red[w]);
+    const float s = scale_of(m), inv = 1.0f / s;
+    if (threadIdx.x == 0) scale[blockIdx.x] = s;
+#pragma unroll
+    for (int p = 0; p < kPasses; ++p) {
+        const long r = r0 + p * kGroups;
+        if (r < rows) store_codes<WIDE>(v[p], inv, q + r * cols, c, cols);
+    }
+}
+
+// One row per workgroup.  HELD passes of 2048 columns stay in registers between
+// the sum of squares and the norm; HELD = 0 reads a longer row twice, the
+// second time from `sum` where that is stored (x and resid may be its memory).
+template <bool BF16, bool WIDE, int HELD>
+__global__ __launch_bounds__(kThreads) void fp8_rmsnorm_kernel(
+    const typename Elem<BF16>::type *x, const typename Elem<BF16>::type *resid, const float *norm_w,
+    float eps, int cols, typename Elem<BF16>::type *sum, uint8_t *q, float *scale) {
+    __shared__ float red[kThreads / kWave];
+    const long at = (long)blockIdx.x * cols;
+    const int c0 = threadIdx.x * kVec;
+    const int lane = threadIdx.x % kLanes;
+    auto load_h = [&](float(&h)[kVec], int c) {
+        load_cols<BF16, WIDE>(h, x + at, c, cols);
+        if (resid) {
+            float r[kVec];
+            load_cols<BF16, WIDE>(r, resid + at, c, cols);
+#pragma unroll
+            for (int i = 0; i < kVec; ++i) {
+                h[i] += r[i];
+                // the stream is kept in its own type, and the norm is that of what is kept
+                if constexpr (BF16) h[i] = bf16_value(bf16_bits(h[i]));
+            }
+        }
+    };
+    auto add_squares = [](const float(&h)[kVec], float s) {
+#pragma unroll
+        for (int i = 0; i < kVec; ++i) s = fmaf(h[i], h[i], s);
+        return s;
+    };
+    auto emit = [&](float(&h)[kVec], float inv_rms, int c) {
+        float w[kVec];
+        load_cols<false, WIDE>(w, norm_w, c, cols);
+#pragma unroll
+        for (int i = 0; i < kVec; ++i) h[i] = h[i] * inv_rms * w[i];
+        const float s = scale_of(group_max(amax8(h)));
+        if (lane == 0 && c < cols)
+            scale[(long)blockIdx.x * ((cols + kFp8Block - 1) / kFp8Block) + c / kFp8Block] = s;
+        store_codes<WIDE>(h, 1.0f / s, q + at, c, cols);
+    };
+    float ss = 0.0f;
+    float held[HELD > 0 ? HELD : 1][kVec];
+    if constexpr (HELD > 0) {
+#pragma unroll
+        for (int p = 0; p < HELD; ++p) load_h(held[p], c0 + p * kSpan);
+#pragma unroll
+        for (int p = 0; p < HELD; ++p) ss = add_squares(held[p], ss);
+    } else {
+        for (int base = 0; base < cols; base += kSpan) {
+            float h[kVec];
+            load_h(h, base + c0);
+            ss = add_squares(h, ss);
+            if (sum) store_cols<BF16, WIDE>(h, sum + at, base + c0, cols);
+        }
+    }
+    ss = wave_sum(ss);
+    if (threadIdx.x % kWave == 0) red[threadIdx.x / kWave] = ss;
+    __syncthreads();
+    ss = (red[0] + red[1]) + (red[2] + red[3]);
+    const float inv_rms = 1.0f / sqrtf(ss / (float)cols + eps);
+    if constexpr (HELD > 0) {
+#pragma unroll
+        for (int p = 0; p < HELD; ++p) {
+            if (sum) store_cols<BF16, WIDE>(held[p], sum + at, c0 + p * kSpan, cols);
+            emit(held[p], inv_rms, c0 + p * kSpan);
+        }
+    } else {
+        for (int base = 0; base < cols; base += kSpan) {
+            float h[kVec];
+            if (sum) load_cols<BF16, WIDE>(h, sum + at, base + c0, cols);
+            else load_h(h, base + c0);
+            emit(h, inv_rms, base + c0);
+        }
+    }
+}
+
+bool aligned16(const void *p) { return ((uintptr_t)p & 15) == 0; }
+
+template <typename F> int with_types(const Fp8Rows &p, bool wide, F launch) {
+    if (p.bf16) {
+        if (wide) launch(std::true_type{}, std::true_type{});
+        else launch(std::true_type{}, std::false_type{});
+    } else {
+        if (wide) launch(std::false_type{}, std::true_type{});
+        else launch(std::false_type{}, std::false_type{});
+    }
+    return hipGetLastError() == hipSuccess ? kOk : kErrLaunch;
+}
+
+// whole 8-value pieces at 16-byte (codes: 8-byte) addresses in every row
+bool wide_rows(const Fp8Rows &p) {
+    return p.cols % kVec == 0 && aligned16(p.x) && ((uintptr_t)p.q & 7) == 0;
+}
+
+constexpr unsigned kMaxGrid = 1u << 20;  // workgroups of a launch that loops
+
+template <bool SWIGLU> int launch_rows(const Fp8Rows &p, hipStream_t stream) {
+    const long blocks = (long)p.rows * fp8_blocks(p.cols);
+    if (blocks > 0x7FFFFFFFL) return kErrSize;
+    const long wgs = (blocks + kGroups - 1) / kGroups;
+    const unsigned grid = wgs < (long)kMaxGrid ? (unsigned)wgs : kMaxGrid;
+    return with_types(p, wide_rows(p), [&](auto bf16, auto wide) {
+        using T = typename Elem<decltype(bf16)::value>::type;
+        hipLaunchKernelGGL((fp8_rows_kernel<decltype(bf16)::value, decltype(wide)::value, SWIGLU>),
+                           dim3(grid), dim3(kThreads), 0, stream, static_cast<const T *>(p.x),
+                           p.rows, p.cols, p.q, p.scale);
+    });
+}
+
+}  // namespace
+
+int fp8_quantize(const Fp8Rows &p, int block_rows, hipStream_t stream) {
+    if (p.rows == 0) return kOk;
+    if (block_rows == 1) return launch_rows<false>(p, stream);
+    const long tiles = (long)fp8_blocks(p.rows) * fp8_blocks(p.cols);
+    if (tiles > 0xFFFFFFL) return kErrSize;  // (2^32 threads a launch)
+    return with_types(p, wide_rows(p), [&](auto bf16, auto wide) {
+        using T = typename Elem<decltype(bf16)::value>::type;
+        hipLaunchKernelGGL((fp8_matrix_kernel<decltype(bf16)::value, decltype(wide)::value>),
+                           dim3((unsigned)tiles), dim3(kThreads), 0, stream,
+                           static_cast<const T *>(p.x), p.rows, p.cols, p.q, p.scale);
+    });
+}
+
+int fp8_swiglu(const Fp8Rows &p, hipStream_t stream) {
+    return p.rows == 0 ? kOk : launch_rows<true>(p, stream);
+}
+
+int fp8_rmsnorm(const Fp8Rows &p, const void *resid, const float *norm_w, float eps, void *sum,
+                hipStream_t stream) {
+    if (p.rows == 0) return kOk;
+    if (p.rows > 0xFFFFFF) return kErrSize;  // (2^32 threads a launch)
+    const bool wide = wide_rows(p) && aligned16(resid) && aligned16(sum) && aligned16(norm_w);
+    const int held = p.cols <= kSpan ? 1 : p.cols <= 2 * kSpan ? 2 : p.cols <= 4 * kSpan ? 4 : 0;
+    return with_types(p, wide, [&](auto bf16, auto w) {
+        using T = typename Elem<decltype(bf16)::value>::type;
+        auto go = [&](auto n) {
+            hipLaunchKernelGGL((fp8_rmsnorm_kernel<decltype(bf16)::value, decltype(w)::value,
+                                                   decltype(n)::value>),
+                               dim3((unsigned)p.rows), dim3(kThreads), 0, stream,
+                               static_cast<const T *>(p.x), static_cast<const T *>(resid), norm_w,
+                               eps, p.cols, static_cast<T *>(sum), p.q, p.scale);
+        };
+        if (held == 1) go(std::integral_constant<int, 1>{});
+        else if (held == 2) go(std::integral_constant<int, 2>{});
+        else if (held == 4) go(std::integral_constant<int, 4>{});
+        else go(std::integral_constant<int, 0>{});
+    });
+}
+
+}  // namespace mlh

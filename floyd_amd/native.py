@@ -11,7 +11,7 @@ import numpy as np
 HERE = os.path.dirname(os.path.abspath(__file__))
 LIBRARY_PATH = os.path.join(HERE, "lib", "libfloyd_amd.so")
 
-MLK_F32, MLK_Q8, MLK_Q4 = 0, 1, 2
+MLK_F32, MLK_Q8, MLK_Q4, MLK_BF16 = 0, 1, 2, 3
 
 _c = ctypes
 _vp = _c.c_void_p
@@ -55,6 +55,14 @@ SIGNATURES = {
     "mlk_quantize": (_c.c_int, [_c.c_int, _vp, _c.c_int, _c.c_int, _vp, _vp]),
     "mlk_fill_normal": (_c.c_int, [_vp, _c.c_int64, _c.c_uint64, _c.c_float, _c.c_float,
                                    _c.c_int]),
+    "mlk_quantize_fp8": (_c.c_int, [_c.c_int, _vp, _c.c_int, _c.c_int, _c.c_int, _vp, _vp]),
+    "mlk_rmsnorm_fp8": (_c.c_int, [_c.c_int, _vp, _vp, _vp, _c.c_float, _c.c_int, _c.c_int,
+                                   _vp, _vp, _vp]),
+    "mlk_swiglu_fp8": (_c.c_int, [_c.c_int, _vp, _c.c_int, _c.c_int, _vp, _vp]),
+    "mlk_matmul_fp8": (_c.c_int, [_c.c_int, _vp, _vp, _vp, _vp, _vp, _c.c_int, _c.c_int,
+                                  _c.c_int, _vp]),
+    "mlk_matmul_fp8_grouped": (_c.c_int, [_c.c_int, _vp, _vp, _vp, _vp, _c.c_int, _vp, _c.c_int,
+                                          _c.c_int, _c.c_int, _vp, _vp, _c.c_int]),
     # include/fm_backend.h
     "fm_init": (_c.c_int, []),
     "fm_device_name": (_c.c_char_p, []),
@@ -233,3 +241,38 @@ def quantize(bits, w, rows, cols, q, s):
 def fill_normal(out, n, seed, mean=0.0, std=1.0, bf16=False):
     check(load().mlk_fill_normal(_ptr(out), n, seed, mean, std, int(bf16)),
           "mlk_fill_normal")
+
+
+def quantize_fp8(dtype, x, rows, cols, block_rows, q, s):
+    """Codes and block scales of x (mlk_quantize_fp8); dtype MLK_F32 or MLK_BF16."""
+    check(load().mlk_quantize_fp8(dtype, _ptr(x), rows, cols, block_rows, _ptr(q), _ptr(s)),
+          "mlk_quantize_fp8")
+
+
+def rmsnorm_fp8(dtype, x, norm_w, rows, cols, q, s, resid=None, total=None, eps=1e-5):
+    """Codes and scales of RMSNorm(x + resid) * norm_w, the sum kept in `total`
+    (mlk_rmsnorm_fp8)."""
+    check(load().mlk_rmsnorm_fp8(dtype, _ptr(x), _ptr(resid), _ptr(norm_w), eps, rows, cols,
+                                 _ptr(total), _ptr(q), _ptr(s)), "mlk_rmsnorm_fp8")
+
+
+def swiglu_fp8(dtype, gate_up, rows, width, q, s):
+    """Codes and scales of silu(gate) * up (mlk_swiglu_fp8)."""
+    check(load().mlk_swiglu_fp8(dtype, _ptr(gate_up), rows, width, _ptr(q), _ptr(s)),
+          "mlk_swiglu_fp8")
+
+
+def matmul_fp8(out_dtype, w, ws, x, xs, y, out_width, in_width, rows, resid=None):
+    """fp8 rows times an fp8 matrix (mlk_matmul_fp8)."""
+    check(load().mlk_matmul_fp8(out_dtype, _ptr(w), _ptr(ws), _ptr(x), _ptr(xs), _ptr(y),
+                                out_width, in_width, rows, _ptr(resid)), "mlk_matmul_fp8")
+
+
+def matmul_fp8_grouped(out_dtype, w, ws, x, xs, y, out_width, in_width, groups, offsets,
+                       entries, row_ids=None, x_rows=None):
+    """fp8 rows times the matrix of their group (mlk_matmul_fp8_grouped); x_rows
+    defaults to `entries`."""
+    check(load().mlk_matmul_fp8_grouped(out_dtype, _ptr(w), _ptr(ws), _ptr(x), _ptr(xs),
+                                        entries if x_rows is None else x_rows, _ptr(y),
+                                        out_width, in_width, groups, _ptr(offsets),
+                                        _ptr(row_ids), entries), "mlk_matmul_fp8_grouped")

@@ -30,7 +30,9 @@
 extern "C" {
 #endif
 
-enum { MLK_F32 = 0, MLK_Q8 = 1, MLK_Q4 = 2 };
+/* Weight formats of mlk_gemv; MLK_F32 and MLK_BF16 are also the types of the
+ * values that the fp8 entry points take and return beside their codes. */
+enum { MLK_F32 = 0, MLK_Q8 = 1, MLK_Q4 = 2, MLK_BF16 = 3 };
 
 /* ---- device plumbing (no counterpart in the reference: Metal used shared
  *      memory buffers, moonlight_metal.m:733-755) ---------------------------- */
@@ -109,6 +111,66 @@ int mlk_quantize(int bits, const float *w, int rows, int cols, uint8_t *q,
                  float *s);
 int mlk_fill_normal(float *out, int64_t n, uint64_t seed, float mean,
                     float std, int bf16);
+
+/* ---- fp8 rows and products ------------------------------------------------
+ * No counterpart in the reference, whose matrices are int8 or int4 with f32
+ * activations.  Values are e4m3 codes (one byte; largest value 448) times an
+ * f32 scale per block: 128 columns of one row for activations, 128 x 128 for
+ * matrices, the form that fp8 checkpoints of this architecture come in.  A
+ * [rows, cols] tensor of codes is dense, its scales are
+ * [rows or ceil(rows / 128), ceil(cols / 128)] f32; the last block of a row
+ * and of a column may be narrower.  Any width and any alignment of codes is
+ * taken; widths that are multiples of 16 at 16-byte addresses are faster.
+ *
+ * Quantising: scale = max(amax / 448, 2^-126) with amax the block's largest
+ * magnitude, code = the e4m3 value nearest to x * (1 / scale), ties to even;
+ * quotients and product in f32.  A NaN keeps to its own code; a block that
+ * holds an infinity gets an infinite scale, and all of it reads as NaN.
+ *
+ * Like mlk_gemv these queue their work on the library stream of the current
+ * device and return (work of other streams on the same memory has to be
+ * waited for by the caller, before and after); they allocate nothing and
+ * keep nothing.  Pointers have to be memory of the current device (-1
+ * otherwise), f32, bf16 and int values at addresses of their own size.
+ * rows = 0 (entries = 0) writes nothing.  Outputs must not overlap inputs
+ * unless stated. */
+
+/* Codes and scales of x, f32 or bf16 [rows, cols] (type MLK_F32 or MLK_BF16):
+ * block_rows = 1 for activations, 128 for matrices. */
+int mlk_quantize_fp8(int type, const void *x, int rows, int cols,
+                     int block_rows, uint8_t *q, float *s);
+/* h = x + resid (resid == NULL: h = x), rounded to `type` and stored to sum
+ * unless that is NULL; q, s = the codes and scales (block_rows = 1) of
+ * RMSNorm(h) * norm_w, the norm as in mlk_gemv.  x, resid and sum are of one
+ * type; sum may be x or resid itself. */
+int mlk_rmsnorm_fp8(int type, const void *x, const void *resid,
+                    const float *norm_w, float eps, int rows, int cols,
+                    void *sum, uint8_t *q, float *s);
+/* Codes and scales (block_rows = 1) of silu(gate) * up, gate_up [rows,
+ * 2 * width] holding each row's gate values and then its up values. */
+int mlk_swiglu_fp8(int type, const void *gate_up, int rows, int width,
+                   uint8_t *q, float *s);
+/* y[r, o] = sum_i x[r, i] W[o, i] (+ resid[r, o]) for codes x [rows, in_width]
+ * with scales xs and codes w [out_width, in_width] with scales ws; y and
+ * resid of out_type, MLK_F32 or MLK_BF16 (rounded once, resid added before;
+ * y may be resid itself). */
+int mlk_matmul_fp8(int out_type, const uint8_t *w, const float *ws,
+                   const uint8_t *x, const float *xs, void *y, int out_width,
+                   int in_width, int rows, const void *resid);
+/* The same with one matrix per group of rows (w [groups, out_width, in_width],
+ * ws likewise): y [entries, out_width] holds the groups' rows one after the
+ * other, group g's from offsets[g] to offsets[g + 1] (device memory,
+ * groups + 1 numbers that do not decrease; a group may be empty).  Row j of
+ * y is the product of x row row_ids[j], or of x row j where row_ids == NULL.
+ * Rows of y before offsets[0] and from offsets[groups] on are left as they
+ * were.  A row whose row_ids[j] is outside [0, x_rows) becomes NaN; offsets
+ * outside [0, entries] or that decrease leave rows out, and nothing is read
+ * or written out of range. */
+int mlk_matmul_fp8_grouped(int out_type, const uint8_t *w, const float *ws,
+                           const uint8_t *x, const float *xs, int x_rows,
+                           void *y, int out_width, int in_width, int groups,
+                           const int *offsets, const int *row_ids,
+                           int entries);
 
 #ifdef __cplusplus
 }
