@@ -102,17 +102,30 @@ def check_codes(code, scale, v, delta):
 
 
 def product(x, xs, w, ws):
-    """(y, bound): the product in 64 bits, and the sum of the magnitudes added."""
+    """(y, mass, top): the product in 64 bits, the sum of the magnitudes added, and the
+    sum of the largest magnitude of each 8 neighbouring columns."""
     a, b = dequantize(x, xs, 1), dequantize(w, ws, BLOCK)
-    return a @ b.T, np.abs(a) @ np.abs(b).T
+    top = np.zeros((a.shape[0], b.shape[0]))
+    for c in range(0, a.shape[1], 8):
+        part = np.zeros_like(top)
+        for i in range(c, min(c + 8, a.shape[1])):
+            np.maximum(part, np.abs(a[:, i, None] * b[None, :, i]), out=part)
+        top += part
+    return a @ b.T, np.abs(a) @ np.abs(b).T, top
 
 
-def product_tolerance(y, mass, inp, out_bf16, resid=None):
+def product_tolerance(y, mass, top, inp, out_bf16, resid=None):
     """A sum of n f32 additions in any order, each off by at most a whole last
     place (2 * 2^-24: to nearest or cut off), is within n * 2^-23 of the magnitudes
     added; per output 128 in a block, then a rounded factor and an addition per
-    block, and up to 8 more where waves join their shares or a residual is added."""
+    block, and up to 8 more where waves join their shares or a residual is added.
+    Products for bf16 outputs may come from fp8 matrix instructions, which add 8
+    neighbouring products after cutting each below 2^-13 of the largest's power of
+    two."""
     n = min(inp, BLOCK) + 2 * blocks(inp) + 8
     room = n * 2 * HALF_F32 * (mass if resid is None else mass + np.abs(resid))
     total = y if resid is None else y + resid
-    return room + (HALF_BF16 * (np.abs(total) + room) if out_bf16 else 0.0)
+    if not out_bf16:
+        return room
+    room = room + 8 * 2.0 ** -13 * top
+    return room + HALF_BF16 * (np.abs(total) + room)

@@ -243,8 +243,8 @@ def check_matmul(dtype, rows, out, inp, with_resid, lead_w=0, lead_x=0, lead_y=0
         np.testing.assert_array_equal(
             rb.download(np.uint8)[lead_y:].view(got.dtype).reshape(got.shape), got)
     got = (U.from_bf16(got) if dtype == MLK_BF16 else got).astype(np.float64)
-    want, mass = U.product(x, xs, w, ws)
-    room = U.product_tolerance(want, mass, inp, dtype == MLK_BF16, resid)
+    want, *parts = U.product(x, xs, w, ws)
+    room = U.product_tolerance(want, *parts, inp, dtype == MLK_BF16, resid)
     off = np.abs(got - (want if resid is None else want + resid))
     assert np.all(off <= room), (np.max(off / room), np.argmax(off / room))
 
@@ -299,8 +299,8 @@ def run_grouped(rng, dtype, counts, out, inp, gather, first=0, spare=0, ids=None
         ok = (src >= 0) & (src < x_rows)
         assert np.isnan(got[at[~ok]]).all()
         at, src = at[ok], src[ok]
-        want, mass = U.product(x[src], xs[src], w[g], ws[g])
-        room = U.product_tolerance(want, mass, inp, dtype == MLK_BF16)
+        want, *parts = U.product(x[src], xs[src], w[g], ws[g])
+        room = U.product_tolerance(want, *parts, inp, dtype == MLK_BF16)
         off = np.abs(got[at] - want)
         assert np.all(off <= room), (g, np.max(off / room))
     return got
@@ -365,8 +365,8 @@ def test_calls_of_two_threads(device):
         t.start()
     for t in threads:
         t.join()
-    for rows, _, outs, (want, mass) in jobs:
-        room = U.product_tolerance(want, mass, 512, False)
+    for rows, _, outs, (want, *parts) in jobs:
+        room = U.product_tolerance(want, *parts, 512, False)
         for y in outs:
             assert np.all(np.abs(y.get(F32, (rows, 320)) - want) <= room)
 
@@ -440,16 +440,16 @@ def test_expert_layer(device, dtype, tokens):
     for e in range(experts):
         at = slice(ends[e], ends[e + 1])
         src = (order // top_k)[at]
-        want, mass = U.product(xc[src], xsc[src], packed[0][0][e], packed[0][1][e])
+        want, *parts = U.product(xc[src], xsc[src], packed[0][0][e], packed[0][1][e])
         assert np.all(np.abs(gate_up_out[at] - want) <=
-                      U.product_tolerance(want, mass, hidden, bf16))
-        want, mass = U.product(hc[at], hsc[at], packed[1][0][e], packed[1][1][e])
-        assert np.all(np.abs(down_out[at] - want) <= U.product_tolerance(want, mass, inter, bf16))
+                      U.product_tolerance(want, *parts, hidden, bf16))
+        want, *parts = U.product(hc[at], hsc[at], packed[1][0][e], packed[1][1][e])
+        assert np.all(np.abs(down_out[at] - want) <= U.product_tolerance(want, *parts, inter, bf16))
     g, u = gate_up_out[:, :inter], gate_up_out[:, inter:]
     U.check_codes(hc, hsc, g / (1.0 + np.exp(-g)) * u, 7 * U.HALF_F32)
-    want, mass = U.product(xc, xsc, packed[2][0][0], packed[2][1][0])
+    want, *parts = U.product(xc, xsc, packed[2][0][0], packed[2][1][0])
     got = value(y.get(kind, (tokens, hidden)))
-    assert np.all(np.abs(got - want - h) <= U.product_tolerance(want, mass, hidden, bf16, h))
+    assert np.all(np.abs(got - want - h) <= U.product_tolerance(want, *parts, hidden, bf16, h))
     # the layer without fp8: a code is off by at most 2^-4 of its value, in the rows and
     # matrices of three products in a row; sums of many such errors of either sign are
     # far below 4 x 2^-4 of the whole
