@@ -5,18 +5,24 @@
 //
 // Codes are widened to bf16, which holds every e4m3 value, and multiplied on
 // v_mfma_f32_16x16x32_bf16: the products are exact in f32 and a block's 128 are
-// added in f32.  Each block's sum is then scaled and added in f32.
+// added in f32.  Tiles of many rows with bf16 outputs multiply the codes as they are
+// (multiply_fp8).  Each block's sum is then scaled and added in f32.
 //
 // Weights are the A operand and rows the B operand: lane l supplies matrix row
 // and token l % 16, and of a block of 128 columns the 16-byte chunks l / 16 and
 // 4 + l / 16 (which of the lane's values meet in one instruction does not
 // matter, as long as both operands agree).  Register r of lane l of a result
 // is output column 4 (l / 16) + r of token l % 16, so that a lane scales with
-// one factor and stores 4 neighbouring outputs.
+// one factor and holds 4 neighbouring outputs.
+//
+// Operands pass through LDS: the lanes of an operand read hold 16 different rows,
+// whose 16-byte pieces the memory pipe takes one a clock (a 1 KB load in 64 clocks),
+// while 8 neighbouring lanes on a row's 128 bytes are taken 64 bytes a clock.
 #include "fp8.h"
 #include "mlh_device.h"
 #include "mlh_host.h"
-#include <stdlib.h>
+
+#include <math.h>
 
 namespace mlh {
 
@@ -32,6 +38,18 @@ __device__ __forceinline__ bf16x8 widen8(unsigned lo, unsigned hi) {
     const bf16x2 c = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, 1.0f, false);
     const bf16x2 d = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, 1.0f, true);
     return bf16x8{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
+}
+
+// The 128 products of a block for 16 x 16 outputs, added, on codes as they are.
+// The instruction adds 8 neighbouring columns' products after cutting each below
+// 2^-13 of the largest's power of two, and these sums in f32: 1.5e-5 to 5e-5 off in
+// norm, where the bf16 output it serves is rounded by up to 4e-3.
+__device__ __forceinline__ f32x4 multiply_fp8(const u32x4 (&w)[2], const u32x4 (&x)[2]) {
+    const i32x8 a = {(int)w[0][0], (int)w[0][1], (int)w[0][2], (int)w[0][3],
+                     (int)w[1][0], (int)w[1][1], (int)w[1][2], (int)w[1][3]};
+    const i32x8 b = {(int)x[0][0], (int)x[0][1], (int)x[0][2], (int)x[0][3],
+                     (int)x[1][0], (int)x[1][1], (int)x[1][2], (int)x[1][3]};
+    return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, f32x4{0, 0, 0, 0}, 0, 0, 0, 0, 0, 0);
 }
 
 __device__ __forceinline__ float bf16_float(uint16_t b) {
@@ -51,12 +69,36 @@ __device__ __forceinline__ u32x4 load16_any(const uint8_t *p) {
     return v;
 }
 
-// columns c .. c + 15 of a row of `width` codes, zeros past its end
+// columns c .. c + 15 of a row of `width` codes, zeros past its end; nothing
+// outside the row is read
 __device__ __forceinline__ u32x4 load16_tail(const uint8_t *row, int c, int width) {
     u32x4 v = {0, 0, 0, 0};
-#pragma unroll
-    for (int i = 0; i < 16; ++i)
-        if (c + i < width) v[i / 4] |= (unsigned)row[c + i] << (8 * (i % 4));
+    if (c + 16 <= width) return load16_any(row + c);
+    if (c >= width) return v;
+    if (width >= 16) {  // the row's last 16, moved down
+        const u32x4 u = load16_any(row + width - 16);
+        const unsigned long long lo = u[0] | (unsigned long long)u[1] << 32;
+        const unsigned long long hi = u[2] | (unsigned long long)u[3] << 32;
+        const int bits = 8 * (c + 16 - width);  // 8 .. 120
+        const unsigned long long l =
+            bits >= 64 ? hi >> (bits - 64) : lo >> bits | hi << (64 - bits);
+        const unsigned long long h = bits >= 64 ? 0 : hi >> bits;
+        v[0] = (unsigned)l;
+        v[1] = (unsigned)(l >> 32);
+        v[2] = (unsigned)h;
+        v[3] = (unsigned)(h >> 32);
+        return v;
+    }
+    unsigned long long l = 0, h = 0;
+#pragma unroll 1
+    for (int i = 0; c + i < width; ++i) {
+        if (i < 8) l |= (unsigned long long)row[c + i] << (8 * i);
+        else h |= (unsigned long long)row[c + i] << (8 * (i - 8));
+    }
+    v[0] = (unsigned)l;
+    v[1] = (unsigned)(l >> 32);
+    v[2] = (unsigned)h;
+    v[3] = (unsigned)(h >> 32);
     return v;
 }
 
@@ -115,7 +157,7 @@ template <int BM> long row_tiles(const Fp8Matmul &p) {
 template <bool BF16>
 __device__ __forceinline__ void store4(const Fp8Matmul &p, long row, int o, f32x4 v) {
     const long at = row * p.O + o;
-    if (o + 4 <= p.O && p.O % 4 == 0) {
+    if (o + 4 <= p.O) {  // (at any address)
         if constexpr (BF16) {
             uint16_t *y = static_cast<uint16_t *>(p.y) + at;
             if (p.resid) {
@@ -164,7 +206,7 @@ __device__ __forceinline__ void store_row(const Fp8Matmul &p, long row, int o, c
         for (int k = 0; k < 4; ++k) f[i + k] = x[k];
     }
     constexpr int kSize = BF16 ? 2 : 4;
-    if (o + EACH <= p.O && (long)p.O * kSize % 16 == 0) {
+    if (o + EACH <= p.O) {  // (at any address)
         const long byte = at * kSize;
         if (p.resid) {
             const u32x4 r = load16_any(static_cast<const uint8_t *>(p.resid) + byte);
@@ -196,158 +238,6 @@ __device__ __forceinline__ void store_row(const Fp8Matmul &p, long row, int o, c
     }
 }
 
-// Both operands straight from memory into registers, any width and alignment.
-// A wave holds NT x MT results of 16 x 16; WO waves share the tile's tokens, WM
-// its matrix rows, and WK waves take every WK-th block of columns, added
-// through LDS.
-template <int NT_, int MT_, int WO_, int WM_, int WK_> struct DirectShape {
-    static constexpr int NT = NT_, MT = MT_, WO = WO_, WM = WM_, WK = WK_;
-    static constexpr int kWaves = WO * WM * WK;
-    static constexpr int kThreads = kWaves * kWave;
-    static constexpr int BO = 16 * NT * WO, BM = 16 * MT * WM;
-};
-
-template <class Sh, bool BF16>
-__global__ __launch_bounds__(Sh::kThreads) void fp8_direct_kernel(Fp8Matmul p, int o_tiles) {
-    constexpr int NT = Sh::NT, MT = Sh::MT, WO = Sh::WO, WM = Sh::WM, WK = Sh::WK;
-    __shared__ f32x4 red[WK > 1 ? (WK - 1) * WO * WM * NT * MT * kWave : 1];
-    const int slot = blockIdx.x / o_tiles;
-    const RowTile rt = row_tile<Sh::BM>(p, slot);
-    if (rt.count <= 0) return;  // the same for the whole workgroup
-    const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
-    const int l16 = lane & 15, quad = lane >> 4;
-    const int wk = wave % WK, wo = wave / WK % WO, wm = wave / (WK * WO);
-    const int o0 = (blockIdx.x - slot * o_tiles) * Sh::BO + wo * 16 * NT;
-    const int m0 = wm * 16 * MT;
-    const int blocks = (p.I - 1) / kFp8Block + 1, whole = p.I / kFp8Block;
-    const int o_blocks = (p.O - 1) / kFp8Block + 1;
-    const uint8_t *wbase = p.w + (long)rt.group * p.O * p.I;
-    const float *wsbase = p.ws + (long)rt.group * o_blocks * blocks;
-
-    // rows past the tile's end are those of its last one, columns past O those
-    // of the last: neither is stored
-    const uint8_t *wrow[NT], *xrow[MT];
-    const float *wsrow[NT], *xsrow[MT];
-    bool bad[MT];
-#pragma unroll
-    for (int n = 0; n < NT; ++n) {
-        const int o = min(o0 + 16 * n, p.O - 1);
-        wrow[n] = wbase + (long)min(o0 + 16 * n + l16, p.O - 1) * p.I;
-        wsrow[n] = wsbase + (long)(o / kFp8Block) * blocks;
-    }
-#pragma unroll
-    for (int m = 0; m < MT; ++m) {
-        int r = rt.first + min(m0 + 16 * m + l16, rt.count - 1);
-        bad[m] = false;
-        if (p.row_ids) {
-            r = p.row_ids[r];
-            bad[m] = r < 0 || r >= p.x_rows;
-            if (bad[m]) r = 0;
-        }
-        xrow[m] = p.x + (long)r * p.I;
-        xsrow[m] = p.xs + (long)r * blocks;
-    }
-
-    struct Step {
-        u32x4 w[NT][2], x[MT][2];
-        float ws[NT], xs[MT];
-    };
-    auto load = [&](Step &s, int b) {
-        const int c = b * kFp8Block + 16 * quad;
-        if (b < whole) {
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-#pragma unroll
-                for (int n = 0; n < NT; ++n) s.w[n][h] = load16_any(wrow[n] + c + 64 * h);
-#pragma unroll
-                for (int m = 0; m < MT; ++m) s.x[m][h] = load16_any(xrow[m] + c + 64 * h);
-            }
-        } else {
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-#pragma unroll
-                for (int n = 0; n < NT; ++n) s.w[n][h] = load16_tail(wrow[n], c + 64 * h, p.I);
-#pragma unroll
-                for (int m = 0; m < MT; ++m) s.x[m][h] = load16_tail(xrow[m], c + 64 * h, p.I);
-            }
-        }
-#pragma unroll
-        for (int n = 0; n < NT; ++n) s.ws[n] = wsrow[n][b];
-#pragma unroll
-        for (int m = 0; m < MT; ++m) s.xs[m] = xsrow[m][b];
-    };
-    f32x4 acc[NT][MT];
-#pragma unroll
-    for (int n = 0; n < NT; ++n)
-#pragma unroll
-        for (int m = 0; m < MT; ++m) acc[n][m] = f32x4{0, 0, 0, 0};
-    auto multiply = [&](const Step &s) {
-        f32x4 d[NT][MT];
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {
-            const int h = q / 2, e = 2 * (q % 2);
-            bf16x8 x[MT];
-#pragma unroll
-            for (int m = 0; m < MT; ++m) x[m] = widen8(s.x[m][h][e], s.x[m][h][e + 1]);
-#pragma unroll
-            for (int n = 0; n < NT; ++n) {
-                const bf16x8 w = widen8(s.w[n][h][e], s.w[n][h][e + 1]);
-#pragma unroll
-                for (int m = 0; m < MT; ++m)
-                    d[n][m] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
-                        w, x[m], q == 0 ? f32x4{0, 0, 0, 0} : d[n][m], 0, 0, 0);
-            }
-        }
-#pragma unroll
-        for (int n = 0; n < NT; ++n)
-#pragma unroll
-            for (int m = 0; m < MT; ++m) {
-                const float f = s.ws[n] * s.xs[m];
-#pragma unroll
-                for (int i = 0; i < 4; ++i) acc[n][m][i] = fmaf(d[n][m][i], f, acc[n][m][i]);
-            }
-    };
-    Step s0, s1;
-    if (wk < blocks) load(s0, wk);
-    for (int b = wk; b < blocks; b += 2 * WK) {
-        if (b + WK < blocks) load(s1, b + WK);
-        multiply(s0);
-        if (b + WK >= blocks) break;
-        if (b + 2 * WK < blocks) load(s0, b + 2 * WK);
-        multiply(s1);
-    }
-
-    if constexpr (WK > 1) {
-        f32x4 *mine = red + ((long)(wk - 1) * WO * WM + wm * WO + wo) * NT * MT * kWave + lane;
-        if (wk > 0) {
-#pragma unroll
-            for (int n = 0; n < NT; ++n)
-#pragma unroll
-                for (int m = 0; m < MT; ++m) mine[(n * MT + m) * kWave] = acc[n][m];
-        }
-        __syncthreads();
-        if (wk > 0) return;
-#pragma unroll
-        for (int k = 1; k < WK; ++k) {
-            const f32x4 *other = red + ((long)(k - 1) * WO * WM + wm * WO + wo) * NT * MT * kWave + lane;
-#pragma unroll
-            for (int n = 0; n < NT; ++n)
-#pragma unroll
-                for (int m = 0; m < MT; ++m) acc[n][m] += other[(n * MT + m) * kWave];
-        }
-    }
-#pragma unroll
-    for (int m = 0; m < MT; ++m) {
-        const int r = m0 + 16 * m + l16;
-        if (r >= rt.count) continue;
-        const float nan = __int_as_float(0x7fc00000);
-#pragma unroll
-        for (int n = 0; n < NT; ++n)
-            store4<BF16>(p, rt.first + r, o0 + 16 * n + 4 * quad,
-                         bad[m] ? f32x4{nan, nan, nan, nan} : acc[n][m]);
-    }
-}
-
 // ---------------------------------------------------------------------------
 // Tiles through LDS, for many rows
 // ---------------------------------------------------------------------------
@@ -368,7 +258,7 @@ template <int BO_, int BM_, int WO_, int WM_, int STAGES_> struct TileShape {
     static constexpr int kStage = (BO + BM) * kFp8Block;
     // scales: two groups of kSpan steps, each BM / 8 pieces of 8 tokens by kSpan steps and
     // one of matrix blocks; behind them the place of copies that stand for none
-    static constexpr int kPieces = BM / 8 + 1;
+    static constexpr int kPieces = BM / 8 + 1, kMatrixBlocks = (BO + kFp8Block - 1) / kFp8Block;
     static constexpr int kScales = kStages * kStage, kScaleGroup = kPieces * 256;
     static constexpr int kIdle = kScales + 2 * kScaleGroup;
     // offsets of the rows' scales: BM tokens, 8 matrix blocks, 8 that stand for none
@@ -377,7 +267,8 @@ template <int BO_, int BM_, int WO_, int WM_, int STAGES_> struct TileShape {
     static constexpr int kWPer = BO / 8 / kWaves, kXPer = BM / 8 / kWaves;  // DMA blocks of a wave
     static constexpr int kDma = kWPer + kXPer;
     static_assert(BO % (8 * kWaves) == 0 && BM % (8 * kWaves) == 0, "whole DMA blocks");
-    static_assert((kPieces + kWaves - 1) / kWaves <= kSpan - (kStages - 2) && BO / kFp8Block <= 8,
+    static_assert((kPieces + kWaves - 1) / kWaves <= kSpan - (kStages - 2) && kMatrixBlocks <= 8 &&
+                      (BO % kFp8Block == 0 || kFp8Block % BO == 0),
                   "a group's scales land before its first step");
     static_assert(BO / 16 % WO == 0 && BM / 16 % WM == 0 && kFp8Block % (16 * NT) == 0,
                   "a wave's matrix rows lie in one block");
@@ -423,7 +314,7 @@ template <int BM> __device__ __forceinline__ int used_tiles(const Fp8Matmul &p) 
 
 constexpr int kTileGroup = 4;  // row tiles that share matrix rows, one after the other
 
-template <class Sh, bool FAST, bool BF16>
+template <class Sh, bool FAST, bool BF16, bool DMA>
 __global__ __launch_bounds__(Sh::kThreads, 2) void fp8_tile_kernel(Fp8Matmul p, int o_tiles, int slots) {
     constexpr int NT = Sh::NT, MT = Sh::MT, BO = Sh::BO, BM = Sh::BM, S = Sh::kStages;
     constexpr int kWaves = Sh::kWaves;
@@ -469,11 +360,12 @@ __global__ __launch_bounds__(Sh::kThreads, 2) void fp8_tile_kernel(Fp8Matmul p, 
         const int r = p.row_ids[rt.first + m];
         return r >= 0 && r < p.x_rows ? r : -1;
     };
-    unsigned x_off[Sh::kXPer];
+    unsigned x_off[Sh::kXPer];  // byte offsets; without DMA the rows (0 where there is none)
 #pragma unroll
     for (int q = 0; q < Sh::kXPer; ++q) {
         const int r = x_row((wave + kWaves * q) * 8 + dma_row);
-        x_off[q] = r < 0 ? (unsigned)kOutside : (unsigned)r * (unsigned)p.I;
+        if constexpr (DMA) x_off[q] = r < 0 ? (unsigned)kOutside : (unsigned)r * (unsigned)p.I;
+        else x_off[q] = max(r, 0);
     }
     const unsigned w_off = (unsigned)(wave * 8 + dma_row) * (unsigned)p.I;
     // A piece of scales: lane l takes step l / 8 of the group and token (or matrix
@@ -482,7 +374,7 @@ __global__ __launch_bounds__(Sh::kThreads, 2) void fp8_tile_kernel(Fp8Matmul p, 
     const int sc_lane = lane & 7, sc_step = lane >> 3;
     unsigned *const row_off = reinterpret_cast<unsigned *>(lds + Sh::kRowOffsets);
     for (int i = threadIdx.x; i < BM + 16; i += Sh::kThreads) {
-        const int r = i < BM ? x_row(i) : i - BM < BO / kFp8Block ? i - BM : -1;
+        const int r = i < BM ? x_row(i) : i - BM < Sh::kMatrixBlocks ? i - BM : -1;
         row_off[i] = r < 0 ? (unsigned)kOutside : (unsigned)r * (unsigned)blocks * 4u;
     }
     __syncthreads();
@@ -519,6 +411,30 @@ __global__ __launch_bounds__(Sh::kThreads, 2) void fp8_tile_kernel(Fp8Matmul p, 
                       past || x_off[q] == (unsigned)kOutside ? (unsigned)kOutside
                                                              : x_off[q] + (unsigned)(chunk * 16),
                       k0, stage + BO * kFp8Block + blk * 1024);
+        }
+    };
+    // The same through registers, for rows at any address: loaded before a step's
+    // products, stored after them.
+    u32x4 held[DMA ? 1 : Sh::kDma];
+    auto load_tiles = [&](int b) {
+        const int k0 = b * kFp8Block;
+#pragma unroll
+        for (int i = 0; i < Sh::kDma; ++i) {
+            const int q = i < Sh::kWPer ? i : i - Sh::kWPer;
+            const int blk = wave + kWaves * q;
+            const int c = k0 + ((lane & 7) ^ ((blk & 1) * 4 + dma_row / 2)) * 16;
+            const uint8_t *row = i < Sh::kWPer ? w_base + (long)min(blk * 8 + dma_row, p.O - 1 - o0) * p.I
+                                               : x_base + (long)x_off[q] * p.I;
+            if (k0 + kFp8Block <= p.I) held[i] = load16_any(row + c);
+            else held[i] = load16_tail(row, c, p.I);
+        }
+    };
+    auto store_tiles = [&](int st) {
+#pragma unroll
+        for (int i = 0; i < Sh::kDma; ++i) {
+            const int q = i < Sh::kWPer ? i : i - Sh::kWPer;
+            *reinterpret_cast<u32x4 *>(lds + st * Sh::kStage + (i < Sh::kWPer ? 0 : BO * kFp8Block) +
+                                       (wave + kWaves * q) * 1024 + lane * 16) = held[i];
         }
     };
 
@@ -560,13 +476,7 @@ __global__ __launch_bounds__(Sh::kThreads, 2) void fp8_tile_kernel(Fp8Matmul p, 
 #pragma unroll
                 for (int m = 0; m < MT; ++m) {
                     if (n < NT) {
-                        const u32x4 *a = wf[n & 1], *x = xf[m];
-                        const i32x8 wa = {(int)a[0][0], (int)a[0][1], (int)a[0][2], (int)a[0][3],
-                                          (int)a[1][0], (int)a[1][1], (int)a[1][2], (int)a[1][3]};
-                        const i32x8 xa = {(int)x[0][0], (int)x[0][1], (int)x[0][2], (int)x[0][3],
-                                          (int)x[1][0], (int)x[1][1], (int)x[1][2], (int)x[1][3]};
-                        d[n & 1][m] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(
-                            wa, xa, f32x4{0, 0, 0, 0}, 0, 0, 0, 0, 0, 0);
+                        d[n & 1][m] = multiply_fp8(wf[n & 1], xf[m]);
                     }
                     if (n > 0) {
 #pragma unroll
@@ -611,20 +521,30 @@ __global__ __launch_bounds__(Sh::kThreads, 2) void fp8_tile_kernel(Fp8Matmul p, 
     // __syncthreads() would wait for the DMA in flight as well.)
 #pragma unroll
     for (int q = 0; q < (Sh::kPieces + kWaves - 1) / kWaves; ++q) copy_scales(0, q, scale_row(q));
+    static_assert(DMA || S == 2, "one stage ahead");
+    if constexpr (DMA) {
 #pragma unroll
-    for (int b = 0; b < S - 1; ++b)
-        copy_tiles(b, b);
+        for (int b = 0; b < S - 1; ++b) copy_tiles(b, b);
+    } else {
+        load_tiles(0);
+        store_tiles(0);
+    }
     int st = 0, fill = S - 1;
     for (int b = 0; b < blocks; ++b) {
-        if (S == 2) wait_vmcnt<0>();
+        if constexpr (!DMA) __builtin_amdgcn_s_waitcnt(0);  // (and the stores to LDS)
+        else if (S == 2) wait_vmcnt<0>();
         else if (b > 0) wait_vmcnt<(S - 2) * (Sh::kDma + 1)>();
         else wait_vmcnt<(S - 2) * Sh::kDma>();
         asm volatile("" ::: "memory");
         __builtin_amdgcn_s_barrier();
         asm volatile("" ::: "memory");
-        copy_tiles(b + S - 1, fill);
+        if constexpr (DMA) copy_tiles(b + S - 1, fill);
+        else if (b + 1 < blocks) load_tiles(b + 1);
         copy_scales(b / kSpan + 1, b % kSpan, scale_row(b % kSpan));  // a part of the next group's
         if (live) multiply(b, st);
+        if constexpr (!DMA) {
+            if (b + 1 < blocks) store_tiles(fill);
+        }
         st = st + 1 == S ? 0 : st + 1;
         fill = fill + 1 == S ? 0 : fill + 1;
     }
@@ -659,26 +579,232 @@ __global__ __launch_bounds__(Sh::kThreads, 2) void fp8_tile_kernel(Fp8Matmul p, 
     }
 }
 
-constexpr long kMaxGrid = 0x7FFFFF;  // workgroups of at most 512 threads in a launch
+// ---------------------------------------------------------------------------
+// Few rows: the matrix as a stream
+// ---------------------------------------------------------------------------
+//
+// A workgroup's WK waves share 16 NT matrix rows and up to 8 XB tokens; wave k
+// takes the blocks of columns k, k + WK, ... and copies both operands by DMA into a
+// ring of its own, STAGES blocks ahead, so that no wave waits for another until the
+// shares are added through LDS.  Rows of 128 bytes with the tiles' swizzle.
+// Without DMA, for rows at any address: through registers, as far ahead, into one
+// stage a wave.
+template <int NT_, int XB_, int WK_, int STAGES_, bool DMA_ = true> struct StreamShape {
+    static constexpr int NT = NT_, XB = XB_, MT = (XB + 1) / 2, WK = WK_, kStages = STAGES_;
+    static constexpr bool DMA = DMA_;
+    static constexpr int kThreads = WK * kWave, BO = 16 * NT, BM = 8 * XB;
+    static constexpr int kStage = 2 * NT * 1024 + 2 * MT * 1024;
+    static constexpr int kLoads = 2 * NT + XB + MT + 1;  // a step's, scales among them
+    static constexpr int kRing = (DMA ? kStages : 1) * kStage;
+    static constexpr int kRed = (WK - 1) * NT * MT * 1024;
+    static constexpr int kLds = WK * kRing > kRed ? WK * kRing : kRed;
+    static_assert(kLds <= 160 * 1024 && kStages * kLoads < 64, "LDS, vmcnt");
+    static_assert(kFp8Block % (16 * NT) == 0, "the matrix rows lie in one block");
+};
 
-template <class Sh> int launch_direct(const Fp8Matmul &p, hipStream_t stream) {
-    const long o_tiles = ((long)p.O + Sh::BO - 1) / Sh::BO;
-    const long tiles = row_tiles<Sh::BM>(p) * o_tiles;
-    if (tiles > kMaxGrid) return kErrSize;
-    if (tiles == 0) return kOk;
-    if (p.bf16)
-        hipLaunchKernelGGL((fp8_direct_kernel<Sh, true>), dim3((unsigned)tiles), dim3(Sh::kThreads),
-                           0, stream, p, (int)o_tiles);
-    else
-        hipLaunchKernelGGL((fp8_direct_kernel<Sh, false>), dim3((unsigned)tiles),
-                           dim3(Sh::kThreads), 0, stream, p, (int)o_tiles);
-    return hipGetLastError() == hipSuccess ? kOk : kErrLaunch;
+template <class Sh, bool BF16>
+__global__ __launch_bounds__(Sh::kThreads) void fp8_stream_kernel(Fp8Matmul p, int o_tiles) {
+    constexpr int NT = Sh::NT, MT = Sh::MT, XB = Sh::XB, WK = Sh::WK, S = Sh::kStages;
+    extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
+    const int slot = blockIdx.x / o_tiles;
+    RowTile rt = row_tile<Sh::BM>(p, slot);
+    if (rt.count <= 0) return;
+    rt.group = __builtin_amdgcn_readfirstlane(rt.group);
+    rt.first = __builtin_amdgcn_readfirstlane(rt.first);
+    rt.count = __builtin_amdgcn_readfirstlane(rt.count);
+    const int lane = threadIdx.x & (kWave - 1);
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+    const int l16 = lane & 15, quad = lane >> 4, dma_row = lane >> 3;
+    const int o0 = (blockIdx.x - slot * o_tiles) * Sh::BO;
+    const int blocks = (p.I - 1) / kFp8Block + 1;
+    const int o_blocks = (p.O - 1) / kFp8Block + 1;
+    const uint8_t *const w_base = p.w + ((long)rt.group * p.O + o0) * p.I;
+    const float *const ws_base = p.ws + ((long)rt.group * o_blocks + o0 / kFp8Block) * blocks;
+    const long x_first = p.row_ids ? 0 : rt.first, x_count = p.row_ids ? p.x_rows : rt.count;
+    const uint8_t *const x_base = p.x + x_first * p.I;
+    const float *const xs_base = p.xs + x_first * blocks;
+    const long w_bytes = (long)(p.O - o0) * p.I, x_bytes = x_count * p.I;
+    const long xs_bytes = x_count * blocks * 4, ws_bytes = (long)blocks * 4;
+    // buffer row of token m (the last one's for those past the end, row 0 for an id
+    // out of range: neither is stored as it is)
+    auto x_row = [&](int m, bool *bad = nullptr) -> unsigned {
+        m = min(m, rt.count - 1);
+        if (!p.row_ids) return m;
+        const int r = p.row_ids[rt.first + m];
+        const bool out = r < 0 || r >= p.x_rows;
+        if (bad) *bad = out;
+        return out ? 0 : r;
+    };
+    unsigned x_off[XB], xs_off[MT];  // bytes; x_off without DMA: rows
+    bool bad[MT];
+#pragma unroll
+    for (int q = 0; q < XB; ++q) x_off[q] = x_row(q * 8 + dma_row) * (Sh::DMA ? (unsigned)p.I : 1u);
+#pragma unroll
+    for (int m = 0; m < MT; ++m) {
+        bad[m] = false;
+        xs_off[m] = x_row(16 * m + l16, &bad[m]) * (unsigned)blocks * 4u;
+    }
+    const unsigned w_off = (unsigned)dma_row * (unsigned)p.I;
+    uint8_t *const ring = lds + wave * Sh::kRing;
+    float xs[S][MT], ws[S];
+    u32x4 held[Sh::DMA ? 1 : S][2 * NT + XB];
+    auto copy_scales = [&](int b, int st) {
+#pragma unroll
+        for (int m = 0; m < MT; ++m)
+            xs[st][m] = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(
+                buffer_of(xs_base, xs_bytes), b < blocks ? xs_off[m] : (unsigned)kOutside, b * 4, 0));
+        ws[st] = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(
+            buffer_of(ws_base, ws_bytes), b < blocks ? 0u : (unsigned)kOutside, b * 4, 0));
+    };
+    auto load = [&](int b, int st) {
+        if (b >= blocks) return;
+        const int k0 = b * kFp8Block;
+#pragma unroll
+        for (int q = 0; q < 2 * NT + XB; ++q) {
+            const int r = q < 2 * NT ? q : q - 2 * NT;
+            const int c = k0 + ((lane & 7) ^ ((r & 1) * 4 + dma_row / 2)) * 16;
+            const uint8_t *row = q < 2 * NT ? w_base + (long)min(r * 8 + dma_row, p.O - 1 - o0) * p.I
+                                            : x_base + (long)x_off[r] * p.I;
+            if (k0 + kFp8Block <= p.I) held[st][q] = load16_any(row + c);
+            else held[st][q] = load16_tail(row, c, p.I);
+        }
+        copy_scales(b, st);
+    };
+    auto store = [&](int st) {
+#pragma unroll
+        for (int q = 0; q < 2 * NT + XB; ++q)
+            *reinterpret_cast<u32x4 *>(ring + q * 1024 + lane * 16) = held[st][q];
+    };
+    auto copy = [&](int b, int st) {
+        LdsByte *stage = (LdsByte *)(ring + st * Sh::kStage);
+        const int k0 = b * kFp8Block;
+#pragma unroll
+        for (int q = 0; q < 2 * NT; ++q) {
+            const int chunk = (lane & 7) ^ ((q & 1) * 4 + dma_row / 2);
+            const bool past = k0 + chunk * 16 >= p.I;  // (of a block past the last, all)
+            dma16(buffer_of(w_base, w_bytes),
+                  past ? (unsigned)kOutside : w_off + (unsigned)(q * 8) * (unsigned)p.I + (unsigned)(chunk * 16),
+                  k0, stage + q * 1024);
+        }
+#pragma unroll
+        for (int q = 0; q < XB; ++q) {
+            const int chunk = (lane & 7) ^ ((q & 1) * 4 + dma_row / 2);
+            const bool past = k0 + chunk * 16 >= p.I;
+            dma16(buffer_of(x_base, x_bytes), past ? (unsigned)kOutside : x_off[q] + (unsigned)(chunk * 16), k0,
+                  stage + (2 * NT + q) * 1024);
+        }
+        copy_scales(b, st);
+    };
+    f32x4 acc[NT][MT];
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int m = 0; m < MT; ++m) acc[n][m] = f32x4{0, 0, 0, 0};
+    const int frag0 = l16 * kFp8Block + ((quad ^ (l16 >> 1)) << 4);
+    const int frag1 = l16 * kFp8Block + (((quad + 4) ^ (l16 >> 1)) << 4);
+    u32x4 wf[NT][2], xf[MT][2];
+    auto read = [&](int st) {
+        const uint8_t *stage = ring + st * Sh::kStage;
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+            wf[n][0] = *reinterpret_cast<const u32x4 *>(stage + n * 2048 + frag0);
+            wf[n][1] = *reinterpret_cast<const u32x4 *>(stage + n * 2048 + frag1);
+        }
+#pragma unroll
+        for (int m = 0; m < MT; ++m) {
+            xf[m][0] = *reinterpret_cast<const u32x4 *>(stage + (NT + m) * 2048 + frag0);
+            xf[m][1] = *reinterpret_cast<const u32x4 *>(stage + (NT + m) * 2048 + frag1);
+        }
+    };
+    auto multiply = [&](int st) {
+        f32x4 d[NT][MT];
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            const int h = q / 2, e = 2 * (q % 2);
+            bf16x8 x[MT];
+#pragma unroll
+            for (int m = 0; m < MT; ++m) x[m] = widen8(xf[m][h][e], xf[m][h][e + 1]);
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+                const bf16x8 w = widen8(wf[n][h][e], wf[n][h][e + 1]);
+#pragma unroll
+                for (int m = 0; m < MT; ++m)
+                    d[n][m] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
+                        w, x[m], q == 0 ? f32x4{0, 0, 0, 0} : d[n][m], 0, 0, 0);
+            }
+        }
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int m = 0; m < MT; ++m) {
+                const float f = ws[st] * xs[st][m];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) acc[n][m][i] = fmaf(d[n][m][i], f, acc[n][m][i]);
+            }
+    };
+    const int steps = (blocks - wave + WK - 1) / WK;  // (0 or less: none)
+#pragma unroll
+    for (int s = 0; s < S; ++s) {
+        if constexpr (Sh::DMA) copy(wave + s * WK, s);
+        else load(wave + s * WK, s);
+    }
+    for (int t = 0; t < steps; t += S) {
+#pragma unroll
+        for (int s = 0; s < S; ++s) {
+            if (t + s >= steps) break;
+            if constexpr (!Sh::DMA) {  // a wave's LDS accesses are done in their order
+                store(s);
+                read(0);
+                multiply(s);
+                load(wave + (t + s + S) * WK, s);
+                continue;
+            }
+            wait_vmcnt<(S - 1) * Sh::kLoads>();
+            asm volatile("" ::: "memory");
+            read(s);
+            // (the reads are done before the stage is filled again)
+            __builtin_amdgcn_s_waitcnt(0xC07F);  // lgkmcnt 0
+            asm volatile("" ::: "memory");
+            multiply(s);
+            copy(wave + (t + s + S) * WK, s);
+        }
+    }
+    if constexpr (Sh::DMA) wait_vmcnt<0>();
+    if constexpr (WK > 1) {
+        __syncthreads();  // the rings become the place of the shares
+        f32x4 *red = reinterpret_cast<f32x4 *>(lds);
+        if (wave > 0) {
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                for (int m = 0; m < MT; ++m) red[(((wave - 1) * NT + n) * MT + m) * kWave + lane] = acc[n][m];
+        }
+        __syncthreads();
+        if (wave > 0) return;
+#pragma unroll
+        for (int k = 0; k < WK - 1; ++k)
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                for (int m = 0; m < MT; ++m) acc[n][m] += red[((k * NT + n) * MT + m) * kWave + lane];
+    }
+#pragma unroll
+    for (int m = 0; m < MT; ++m) {
+        const int r = 16 * m + l16;
+        if (r >= rt.count) continue;
+        const float nan = __int_as_float(0x7fc00000);
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+            store4<BF16>(p, rt.first + r, o0 + 16 * n + 4 * quad, bad[m] ? f32x4{nan, nan, nan, nan} : acc[n][m]);
+    }
 }
 
-template <class Sh, bool FAST, bool BF16>
+constexpr long kMaxGrid = 0x7FFFFF;  // workgroups of at most 512 threads in a launch
+
+template <class Sh, bool FAST, bool BF16, bool DMA = true>
 int launch_tile(const Fp8Matmul &p, hipStream_t stream) {
     static const bool attr = [] {
-        return hipFuncSetAttribute(reinterpret_cast<const void *>(&fp8_tile_kernel<Sh, FAST, BF16>),
+        return hipFuncSetAttribute(reinterpret_cast<const void *>(&fp8_tile_kernel<Sh, FAST, BF16, DMA>),
                                    hipFuncAttributeMaxDynamicSharedMemorySize, Sh::kLds) == hipSuccess;
     }();
     (void)attr;
@@ -686,40 +812,133 @@ int launch_tile(const Fp8Matmul &p, hipStream_t stream) {
     const long tiles = o_tiles * slots;
     if (tiles > kMaxGrid - 8) return kErrSize;
     if (tiles == 0) return kOk;
-    hipLaunchKernelGGL((fp8_tile_kernel<Sh, FAST, BF16>), dim3((unsigned)((tiles + 7) / 8 * 8)),
+    hipLaunchKernelGGL((fp8_tile_kernel<Sh, FAST, BF16, DMA>), dim3((unsigned)((tiles + 7) / 8 * 8)),
                        dim3(Sh::kThreads), Sh::kLds, stream, p, (int)o_tiles, (int)slots);
     return hipGetLastError() == hipSuccess ? kOk : kErrLaunch;
 }
 
-// The tiles copy 16-byte chunks and reach a tile's rows, and gathered rows from
-// the first one, by 32-bit offsets.
-bool tiles_take(const Fp8Matmul &p) {
-    const long blocks = fp8_blocks(p.I);
-    return p.I % 16 == 0 && ((uintptr_t)p.w & 15) == 0 && ((uintptr_t)p.x & 15) == 0 && p.I <= (1 << 22) &&
-           (!p.row_ids || ((long)p.x_rows * p.I < kOutside && (long)p.x_rows * blocks * 4 < kOutside));
+template <class Sh, bool BF16> int launch_stream(const Fp8Matmul &p, hipStream_t stream) {
+    static const bool attr = [] {
+        return hipFuncSetAttribute(reinterpret_cast<const void *>(&fp8_stream_kernel<Sh, BF16>),
+                                   hipFuncAttributeMaxDynamicSharedMemorySize, Sh::kLds) == hipSuccess;
+    }();
+    (void)attr;
+    const long o_tiles = ((long)p.O + Sh::BO - 1) / Sh::BO;
+    const long tiles = row_tiles<Sh::BM>(p) * o_tiles;
+    if (tiles > kMaxGrid) return kErrSize;
+    if (tiles == 0) return kOk;
+    hipLaunchKernelGGL((fp8_stream_kernel<Sh, BF16>), dim3((unsigned)tiles), dim3(Sh::kThreads), Sh::kLds, stream,
+                       p, (int)o_tiles);
+    return hipGetLastError() == hipSuccess ? kOk : kErrLaunch;
+}
+
+// DMA takes 16-byte chunks, and a tile's rows by 32-bit offsets.
+bool dma_takes(const Fp8Matmul &p) {
+    return p.I <= (1 << 22) && p.I % 16 == 0 && ((uintptr_t)p.w & 15) == 0 && ((uintptr_t)p.x & 15) == 0 &&
+           (!p.row_ids || (long)p.x_rows * p.I < kOutside);
+}
+
+// ---- which kernel: the one that a model of its time says is the fastest.
+//
+// A workgroup takes `start` us and `step` us for each of its waves' blocks of
+// columns where every CU has at most one, `full` us a block where each CU holds
+// per_cu of them, and in between for numbers in between; workgroups that follow
+// others on their CU start in half the time.  The three numbers of each shape are
+// fitted to its times on MI355X over 260 products (out_width 60 .. 22528, in_width
+// 60 .. 11264, 1 .. 4096 rows, one matrix or up to 160), which they give within 12 %
+// on average; the choice takes 2.5 % longer than the best shape would, 1.4 times at
+// worst.  Some of those times (us; streams by matrix rows x tokens):
+//   22528 x 2048, 16 rows:   stream 16 x 16 10.5, tile 128 x 64 11.7, stream 32 x 32 17.5
+//                 100 rows:  tile 64 x 64 15.5, 128 x 64 17.0, 128 x 128 18.3
+//                 4096 rows: tile 256 x 256 234, 128 x 128 265, 128 x 64 329
+//   2048 x 11264, 1 row:     stream 16 x 8 on 8 waves by DMA 7.1, on 4 through registers 13.9
+//                 100 rows:  stream 32 x 32 16.7, 64 x 64 28.3, tile 64 x 64 41.1
+//                 400 rows:  stream 64 x 64 29.0, tile 64 x 64 42.3, 128 x 64 49.6
+//   2048 x 2048,  100 rows:  stream 32 x 32 6.4, tile 64 x 64 9.9, 128 x 64 12.4
+struct Variant {
+    int bo, bm, waves, per_cu;  // waves: those that share a reduction
+    float start, step, full;
+    bool dma;
+    int (*launch)(const Fp8Matmul &, hipStream_t);
+};
+
+template <bool BF16, int BO, int BM, int WO, int WM, int STAGES, bool DMA>
+constexpr Variant tile(int per_cu, float start, float step, float full) {
+    return Variant{BO, BM, 1, per_cu, start, step, full, DMA,
+                   &launch_tile<TileShape<BO, BM, WO, WM, STAGES>, BF16, BF16, DMA>};
+}
+template <bool BF16, int NT, int XB, int WK, int STAGES, bool DMA>
+constexpr Variant flow(int per_cu, float start, float step, float full) {
+    using Sh = StreamShape<NT, XB, WK, STAGES, DMA>;
+    return Variant{Sh::BO, Sh::BM, WK, per_cu, start, step, full, DMA, &launch_stream<Sh, BF16>};
+}
+
+constexpr Variant kBf16Variants[] = {
+    flow<true, 1, 1, 4, 2, false>(4, 3.7f, 0.49f, 0.96f),
+    flow<true, 1, 2, 4, 2, false>(4, 4.1f, 0.54f, 1.06f),
+    flow<true, 1, 2, 8, 2, false>(2, 3.9f, 0.74f, 1.20f),
+    flow<true, 2, 4, 4, 1, false>(2, 4.6f, 1.06f, 1.50f),
+    tile<true, 64, 64, 2, 2, 2, false>(4, 4.0f, 0.67f, 1.39f),
+    tile<true, 128, 128, 2, 2, 2, false>(2, 7.3f, 1.08f, 2.08f),
+    flow<true, 1, 1, 8, 4, true>(1, 4.2f, 0.30f, 0.49f),
+    flow<true, 2, 4, 4, 4, true>(1, 5.0f, 0.49f, 0.71f),
+    flow<true, 4, 8, 4, 2, true>(1, 7.5f, 1.06f, 1.67f),
+    tile<true, 64, 64, 2, 2, 2, true>(4, 3.5f, 0.44f, 1.26f),
+    tile<true, 128, 64, 4, 1, 3, true>(2, 4.5f, 0.51f, 1.03f),
+    tile<true, 128, 128, 2, 2, 2, true>(2, 6.0f, 0.68f, 1.40f),
+    tile<true, 256, 256, 2, 4, 2, true>(1, 10.4f, 1.34f, 2.07f),
+};
+constexpr Variant kF32Variants[] = {
+    flow<false, 1, 1, 4, 2, false>(4, 4.0f, 0.48f, 0.88f),
+    flow<false, 1, 2, 4, 2, false>(4, 4.2f, 0.53f, 1.06f),
+    flow<false, 1, 2, 8, 2, false>(2, 4.2f, 0.81f, 1.15f),
+    flow<false, 2, 4, 4, 1, false>(2, 4.9f, 1.02f, 1.29f),
+    tile<false, 64, 64, 2, 2, 2, false>(4, 5.5f, 0.68f, 1.45f),
+    tile<false, 128, 128, 2, 2, 2, false>(2, 10.1f, 1.42f, 2.38f),
+    flow<false, 1, 1, 8, 4, true>(1, 4.2f, 0.30f, 0.49f),
+    flow<false, 2, 4, 4, 4, true>(1, 4.9f, 0.47f, 0.63f),
+    flow<false, 4, 8, 4, 2, true>(1, 6.4f, 1.14f, 1.56f),
+    tile<false, 64, 64, 2, 2, 2, true>(4, 3.7f, 0.55f, 1.35f),
+    tile<false, 128, 64, 4, 1, 3, true>(2, 4.6f, 0.77f, 1.29f),
+    tile<false, 128, 128, 2, 2, 2, true>(2, 5.7f, 1.12f, 1.90f),
+};
+
+template <int N> int launch_best(const Variant (&variants)[N], const Fp8Matmul &p, hipStream_t stream) {
+    constexpr float kCus = 256.0f;
+    const bool dma = dma_takes(p);
+    const int blocks = fp8_blocks(p.I);
+    // the groups that rows spread by chance are expected to reach; every second one's
+    // last tile is half full
+    const float used =
+        p.groups ? p.groups * (1.0f - powf(1.0f - 1.0f / p.groups, (float)p.rows)) : 0.0f;
+    const Variant *best = nullptr;
+    float least = 0.0f;
+    for (const Variant &v : variants) {
+        if (v.dma && !dma) continue;
+        const float row_tiles = p.groups ? fmaxf(used, (float)p.rows / v.bm + 0.5f * used)
+                                         : (float)((p.rows - 1) / v.bm + 1);
+        const float share = row_tiles * (float)((p.O - 1) / v.bo + 1) / kCus, fill = share / v.per_cu;
+        const float rounds = 0.5f * (fill + ceilf(fill));
+        const float step = share <= 1.0f  ? v.step
+                           : fill <= 1.0f ? v.step + (v.full - v.step) * (share - 1.0f) / (v.per_cu - 1)
+                                          : v.full * rounds;
+        const float cost = v.start * (0.5f + 0.5f * fmaxf(1.0f, rounds)) +
+                           (float)((blocks - 1) / v.waves + 1) * step;
+        if (!best || cost < least) {
+            best = &v;
+            least = cost;
+        }
+    }
+    return best->launch(p, stream);
 }
 
 }  // namespace
 
 int fp8_matmul(const Fp8Matmul &p, hipStream_t stream) {
     if (p.rows == 0) return kOk;
-    const long per_group = p.groups ? (p.rows + p.groups - 1) / p.groups : p.rows;
-    if (tiles_take(p) && per_group > 32) {
-        static const int force = getenv("FP8_SHAPE") ? atoi(getenv("FP8_SHAPE")) : 0;
-        if (p.bf16) {
-            if (force == 1) return launch_tile<TileShape<256, 256, 2, 4, 2>, true, true>(p, stream);
-            if (force == 2) return launch_tile<TileShape<256, 128, 4, 2, 3>, true, true>(p, stream);
-            if (force == 3) return launch_tile<TileShape<128, 128, 2, 2, 2>, true, true>(p, stream);
-            if (force == 4) return launch_tile<TileShape<128, 64, 4, 1, 3>, true, true>(p, stream);
-        } else {
-            if (force == 1) return launch_tile<TileShape<256, 128, 4, 2, 3>, false, false>(p, stream);
-            if (force == 2) return launch_tile<TileShape<128, 256, 2, 4, 2>, false, false>(p, stream);
-            if (force == 3) return launch_tile<TileShape<128, 128, 2, 2, 2>, false, false>(p, stream);
-            if (force == 4) return launch_tile<TileShape<128, 64, 4, 1, 3>, false, false>(p, stream);
-        }
-    }
-    if (per_group <= 16) return launch_direct<DirectShape<1, 1, 1, 1, 4>>(p, stream);
-    return launch_direct<DirectShape<2, 2, 2, 2, 1>>(p, stream);
+    // the scales of a tile's rows, and of gathered rows, are reached by 32-bit offsets
+    if (p.I > (1 << 30) || (p.row_ids && (long)p.x_rows * fp8_blocks(p.I) * 4 >= kOutside)) return kErrSize;
+    return p.bf16 ? launch_best(kBf16Variants, p, stream) : launch_best(kF32Variants, p, stream);
 }
 
 }  // namespace mlh
