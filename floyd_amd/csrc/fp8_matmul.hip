@@ -881,6 +881,7 @@ constexpr Variant kBf16Variants[] = {
     tile<true, 64, 64, 2, 2, 2, false>(4, 4.0f, 0.67f, 1.39f),
     tile<true, 128, 128, 2, 2, 2, false>(2, 7.3f, 1.08f, 2.08f),
     flow<true, 1, 1, 8, 4, true>(1, 4.2f, 0.30f, 0.49f),
+    flow<true, 2, 2, 8, 2, true>(1, 2.6f, 0.77f, 1.10f),
     flow<true, 2, 4, 4, 4, true>(1, 5.0f, 0.49f, 0.71f),
     flow<true, 4, 8, 4, 2, true>(1, 7.5f, 1.06f, 1.67f),
     tile<true, 64, 64, 2, 2, 2, true>(4, 3.5f, 0.44f, 1.26f),
@@ -896,6 +897,7 @@ constexpr Variant kF32Variants[] = {
     tile<false, 64, 64, 2, 2, 2, false>(4, 5.5f, 0.68f, 1.45f),
     tile<false, 128, 128, 2, 2, 2, false>(2, 10.1f, 1.42f, 2.38f),
     flow<false, 1, 1, 8, 4, true>(1, 4.2f, 0.30f, 0.49f),
+    flow<false, 2, 2, 8, 2, true>(1, 2.6f, 0.77f, 1.10f),
     flow<false, 2, 4, 4, 4, true>(1, 4.9f, 0.47f, 0.63f),
     flow<false, 4, 8, 4, 2, true>(1, 6.4f, 1.14f, 1.56f),
     tile<false, 64, 64, 2, 2, 2, true>(4, 3.7f, 0.55f, 1.35f),
