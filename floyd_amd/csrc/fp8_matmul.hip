@@ -31,6 +31,7 @@ namespace {
 typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef int i32x8 __attribute__((ext_vector_type(8)));
+typedef unsigned u32x4_any __attribute__((ext_vector_type(4), aligned(2)));
 
 __device__ __forceinline__ bf16x8 widen8(unsigned lo, unsigned hi) {
     const bf16x2 a = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, 1.0f, false);
@@ -222,7 +223,9 @@ __device__ __forceinline__ void store_row(const Fp8Matmul &p, long row, int o, c
             if constexpr (BF16) u[i] = float_bf16(f[2 * i]) | (float_bf16(f[2 * i + 1]) << 16);
             else u[i] = __float_as_uint(f[i]);
         }
-        __builtin_memcpy(static_cast<uint8_t *>(p.y) + byte, &u, 16);
+        // past the L2: results of many rows would push the operands out of it (4096 x
+        // 22528 x 2048 bf16 206 us, stored through it 226)
+        __builtin_nontemporal_store(u, reinterpret_cast<u32x4_any *>(static_cast<uint8_t *>(p.y) + byte));
         return;
     }
 #pragma unroll
@@ -540,7 +543,9 @@ __global__ __launch_bounds__(Sh::kThreads, 2) void fp8_tile_kernel(Fp8Matmul p, 
         asm volatile("" ::: "memory");
         if constexpr (DMA) copy_tiles(b + S - 1, fill);
         else if (b + 1 < blocks) load_tiles(b + 1);
-        copy_scales(b / kSpan + 1, b % kSpan, scale_row(b % kSpan));  // a part of the next group's
+        // a part of the next group's scales; three stages count every step's copies alike
+        if (S > 2 || b % kSpan * kWaves + wave < Sh::kPieces)
+            copy_scales(b / kSpan + 1, b % kSpan, scale_row(b % kSpan));
         if (live) multiply(b, st);
         if constexpr (!DMA) {
             if (b + 1 < blocks) store_tiles(fill);
@@ -881,7 +886,7 @@ constexpr Variant kBf16Variants[] = {
     tile<true, 64, 64, 2, 2, 2, false>(4, 4.0f, 0.67f, 1.39f),
     tile<true, 128, 128, 2, 2, 2, false>(2, 7.3f, 1.08f, 2.08f),
     flow<true, 1, 1, 8, 4, true>(1, 4.2f, 0.30f, 0.49f),
-    flow<true, 2, 2, 8, 2, true>(1, 2.6f, 0.77f, 1.10f),
+    flow<true, 2, 2, 8, 2, true>(1, 4.4f, 0.60f, 0.72f),
     flow<true, 2, 4, 4, 4, true>(1, 5.0f, 0.49f, 0.71f),
     flow<true, 4, 8, 4, 2, true>(1, 7.5f, 1.06f, 1.67f),
     tile<true, 64, 64, 2, 2, 2, true>(4, 3.5f, 0.44f, 1.26f),
@@ -897,7 +902,7 @@ constexpr Variant kF32Variants[] = {
     tile<false, 64, 64, 2, 2, 2, false>(4, 5.5f, 0.68f, 1.45f),
     tile<false, 128, 128, 2, 2, 2, false>(2, 10.1f, 1.42f, 2.38f),
     flow<false, 1, 1, 8, 4, true>(1, 4.2f, 0.30f, 0.49f),
-    flow<false, 2, 2, 8, 2, true>(1, 2.6f, 0.77f, 1.10f),
+    flow<false, 2, 2, 8, 2, true>(1, 4.4f, 0.60f, 0.72f),
     flow<false, 2, 4, 4, 4, true>(1, 4.9f, 0.47f, 0.63f),
     flow<false, 4, 8, 4, 2, true>(1, 6.4f, 1.14f, 1.56f),
     tile<false, 64, 64, 2, 2, 2, true>(4, 3.7f, 0.55f, 1.35f),

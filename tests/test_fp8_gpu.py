@@ -110,7 +110,7 @@ def test_quantize_special_values(device, block_rows):
 @pytest.mark.parametrize("keep", ["no", "apart", "x", "resid"])
 @pytest.mark.parametrize("dtype", [MLK_F32, MLK_BF16])
 @pytest.mark.parametrize("rows,cols", [(1, 1), (2, 100), (3, 2048), (2, 2056), (5, 4100), (3, 8192),
-                                       (2, 8200), (2, 20001), (300, 640)])
+                                       (2, 8200), (3, 16384), (2, 20001), (300, 640)])
 def test_rmsnorm(device, dtype, rows, cols, keep):
     rng = np.random.default_rng(rows + 7 * cols)
     size = 2 if dtype == MLK_BF16 else 4
