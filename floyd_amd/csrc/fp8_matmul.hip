@@ -267,10 +267,12 @@ template <int BO_, int BM_, int WO_, int WM_, int STAGES_> struct TileShape {
     // offsets of the rows' scales: BM tokens, 8 matrix blocks, 8 that stand for none
     static constexpr int kRowOffsets = kIdle + 256;
     static constexpr int kLds = kRowOffsets + (BM + 16) * 4;
-    static constexpr int kWPer = BO / 8 / kWaves, kXPer = BM / 8 / kWaves;  // DMA blocks of a wave
+    // the waves that copy: with two on a SIMD one of them
+    static constexpr int kCopiers = kWaves == 8 ? 4 : kWaves;
+    static constexpr int kWPer = BO / 8 / kCopiers, kXPer = BM / 8 / kCopiers;  // DMA blocks of one
     static constexpr int kDma = kWPer + kXPer;
-    static_assert(BO % (8 * kWaves) == 0 && BM % (8 * kWaves) == 0, "whole DMA blocks");
-    static_assert((kPieces + kWaves - 1) / kWaves <= kSpan - (kStages - 2) && kMatrixBlocks <= 8 &&
+    static_assert(BO % (8 * kCopiers) == 0 && BM % (8 * kCopiers) == 0, "whole DMA blocks");
+    static_assert((kPieces - 1 + kCopiers - 1) / kCopiers <= kSpan - (kStages - 2) && kMatrixBlocks <= 8 &&
                       (BO % kFp8Block == 0 || kFp8Block % BO == 0),
                   "a group's scales land before its first step");
     static_assert(BO / 16 % WO == 0 && BM / 16 % WM == 0 && kFp8Block % (16 * NT) == 0,
@@ -366,7 +368,7 @@ __global__ __launch_bounds__(Sh::kThreads, 2) void fp8_tile_kernel(Fp8Matmul p, 
     unsigned x_off[Sh::kXPer];  // byte offsets; without DMA the rows (0 where there is none)
 #pragma unroll
     for (int q = 0; q < Sh::kXPer; ++q) {
-        const int r = x_row((wave + kWaves * q) * 8 + dma_row);
+        const int r = x_row((wave % Sh::kCopiers + Sh::kCopiers * q) * 8 + dma_row);
         if constexpr (DMA) x_off[q] = r < 0 ? (unsigned)kOutside : (unsigned)r * (unsigned)p.I;
         else x_off[q] = max(r, 0);
     }
@@ -381,17 +383,22 @@ __global__ __launch_bounds__(Sh::kThreads, 2) void fp8_tile_kernel(Fp8Matmul p, 
         row_off[i] = r < 0 ? (unsigned)kOutside : (unsigned)r * (unsigned)blocks * 4u;
     }
     __syncthreads();
-    auto scale_row = [&](int q) {  // for this wave's piece q of a group
-        return row_off[min(q * kWaves + wave, BM / 8 + 1) * 8 + sc_lane];
-    };
-    auto copy_scales = [&](int g, int q, unsigned row) {
-        const int piece = q * kWaves + wave;
+    // (pieces behind the last stand for none: three stages count every step's copies alike)
+    auto copy_scales = [&](int g, int piece) {
+        const unsigned row = row_off[min(piece, BM / 8 + 1) * 8 + sc_lane];
         const bool rows = piece < BM / 8;
         const bool in = g * kSpan + sc_step < blocks && row != (unsigned)kOutside;
         dma4(buffer_of(rows ? xs_base : ws_base, rows ? xs_bytes : ws_bytes),
              in ? row + sc_step * 4u : (unsigned)kOutside, g * kSpan * 4,
              (LdsByte *)(lds + (piece <= BM / 8 ? Sh::kScales + (g & 1) * Sh::kScaleGroup + piece * 256
                                                 : Sh::kIdle)));
+    };
+    // a step's part of the next group's scales
+    auto copy_next_scales = [&](int b) {
+        const int g = b / kSpan + 1, piece = b % kSpan * Sh::kCopiers + wave;
+        if (S > 2 || piece < Sh::kPieces) copy_scales(g, piece);
+        // (one piece more than the steps have copies)
+        if (Sh::kPieces > kSpan * Sh::kCopiers && b % kSpan == 0 && wave == 0) copy_scales(g, Sh::kPieces - 1);
     };
     // the operands of step b
     auto copy_tiles = [&](int b, int st) {
@@ -400,14 +407,14 @@ __global__ __launch_bounds__(Sh::kThreads, 2) void fp8_tile_kernel(Fp8Matmul p, 
 #pragma unroll
         for (int i = 0; i < Sh::kDma; ++i) {
             const int q = i < Sh::kWPer ? i : i - Sh::kWPer;
-            const int blk = wave + kWaves * q;
+            const int blk = wave + Sh::kCopiers * q;
             const int chunk = (lane & 7) ^ ((blk & 1) * 4 + dma_row / 2);
             // a row that ends inside the step, or before it: zeros past its end
             const bool past = k0 + kFp8Block > p.I && k0 + chunk * 16 >= p.I;
             if (i < Sh::kWPer)
                 dma16(buffer_of(w_base, w_bytes),
                       past ? (unsigned)kOutside
-                           : w_off + (unsigned)(q * kWaves * 8) * (unsigned)p.I + (unsigned)(chunk * 16),
+                           : w_off + (unsigned)(q * Sh::kCopiers * 8) * (unsigned)p.I + (unsigned)(chunk * 16),
                       k0, stage + blk * 1024);
             else
                 dma16(buffer_of(x_base, x_bytes),
@@ -424,7 +431,7 @@ __global__ __launch_bounds__(Sh::kThreads, 2) void fp8_tile_kernel(Fp8Matmul p, 
 #pragma unroll
         for (int i = 0; i < Sh::kDma; ++i) {
             const int q = i < Sh::kWPer ? i : i - Sh::kWPer;
-            const int blk = wave + kWaves * q;
+            const int blk = wave + Sh::kCopiers * q;
             const int c = k0 + ((lane & 7) ^ ((blk & 1) * 4 + dma_row / 2)) * 16;
             const uint8_t *row = i < Sh::kWPer ? w_base + (long)min(blk * 8 + dma_row, p.O - 1 - o0) * p.I
                                                : x_base + (long)x_off[q] * p.I;
@@ -437,7 +444,7 @@ __global__ __launch_bounds__(Sh::kThreads, 2) void fp8_tile_kernel(Fp8Matmul p, 
         for (int i = 0; i < Sh::kDma; ++i) {
             const int q = i < Sh::kWPer ? i : i - Sh::kWPer;
             *reinterpret_cast<u32x4 *>(lds + st * Sh::kStage + (i < Sh::kWPer ? 0 : BO * kFp8Block) +
-                                       (wave + kWaves * q) * 1024 + lane * 16) = held[i];
+                                       (wave + Sh::kCopiers * q) * 1024 + lane * 16) = held[i];
         }
     };
 
@@ -523,14 +530,21 @@ __global__ __launch_bounds__(Sh::kThreads, 2) void fp8_tile_kernel(Fp8Matmul p, 
     // wave's part visible and frees the stage read last.  (A bare barrier:
     // __syncthreads() would wait for the DMA in flight as well.)
 #pragma unroll
-    for (int q = 0; q < (Sh::kPieces + kWaves - 1) / kWaves; ++q) copy_scales(0, q, scale_row(q));
+    for (int q = 0; q < (Sh::kPieces + kWaves - 1) / kWaves; ++q) copy_scales(0, q * kWaves + wave);
     static_assert(DMA || S == 2, "one stage ahead");
+    static_assert(S == 2 || Sh::kCopiers == kWaves, "the waits below");
+    // Eight waves: the first four, one on each SIMD, hand the copies to the memory pipe,
+    // which holds them up until it has taken them, while the other four multiply.
+    const bool copier = wave < Sh::kCopiers;
     if constexpr (DMA) {
 #pragma unroll
-        for (int b = 0; b < S - 1; ++b) copy_tiles(b, b);
+        for (int b = 0; b < S - 1; ++b)
+            if (copier) copy_tiles(b, b);
     } else {
-        load_tiles(0);
-        store_tiles(0);
+        if (copier) {
+            load_tiles(0);
+            store_tiles(0);
+        }
     }
     int st = 0, fill = S - 1;
     for (int b = 0; b < blocks; ++b) {
@@ -541,14 +555,14 @@ __global__ __launch_bounds__(Sh::kThreads, 2) void fp8_tile_kernel(Fp8Matmul p, 
         asm volatile("" ::: "memory");
         __builtin_amdgcn_s_barrier();
         asm volatile("" ::: "memory");
-        if constexpr (DMA) copy_tiles(b + S - 1, fill);
-        else if (b + 1 < blocks) load_tiles(b + 1);
-        // a part of the next group's scales; three stages count every step's copies alike
-        if (S > 2 || b % kSpan * kWaves + wave < Sh::kPieces)
-            copy_scales(b / kSpan + 1, b % kSpan, scale_row(b % kSpan));
+        if (copier) {
+            if constexpr (DMA) copy_tiles(b + S - 1, fill);
+            else if (b + 1 < blocks) load_tiles(b + 1);
+            copy_next_scales(b);
+        }
         if (live) multiply(b, st);
         if constexpr (!DMA) {
-            if (b + 1 < blocks) store_tiles(fill);
+            if (copier && b + 1 < blocks) store_tiles(fill);
         }
         st = st + 1 == S ? 0 : st + 1;
         fill = fill + 1 == S ? 0 : fill + 1;
