@@ -17,6 +17,9 @@ constexpr float kFp8Top = 448.0f;
 // is below 448 * 2^-126 (a subnormal scale would lose bits of its own)
 constexpr float kFp8TinyScale = 0x1p-126f;
 
+// Columns of a row are counted in 32 bits, with room for a step past the last.
+constexpr int kFp8MaxWidth = 1 << 30;
+
 inline int fp8_blocks(int n) { return (n - 1) / kFp8Block + 1; }  // n > 0
 
 // Rows to quantise.  bf16: x (and resid, sum) are bfloat16, else f32.

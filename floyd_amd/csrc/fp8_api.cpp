@@ -61,6 +61,13 @@ int finish(int status, const char *what) {
     return status;
 }
 
+int check_rows(const char *what, int rows, const char *name, int width) {
+    if (rows < 0) return refuse(what, "rows must be >= 0");
+    if (width <= 0 || width > kFp8MaxWidth)
+        return refuse(what, std::string(name) + " must be > 0 and at most 2^30");
+    return kOk;
+}
+
 bool type_ok(int type) { return type == MLK_F32 || type == MLK_BF16; }
 unsigned size_of(int type) { return type == MLK_BF16 ? 2 : 4; }
 
@@ -83,7 +90,7 @@ int mlk_quantize_fp8(int type, const void *x, int rows, int cols, int block_rows
                      float *s) {
     const char *what = "mlk_quantize_fp8";
     if (!type_ok(type)) return refuse(what, "type must be MLK_F32 or MLK_BF16");
-    if (rows < 0 || cols <= 0) return refuse(what, "rows must be >= 0 and cols > 0");
+    if (int e = check_rows(what, rows, "cols", cols)) return e;
     if (block_rows != 1 && block_rows != kFp8Block) return refuse(what, "block_rows must be 1 or 128");
     if (rows == 0) return kOk;
     const Pointer list[] = {{x, "x", size_of(type), false}, {q, "q", 1, false}, {s, "s", 4, false}};
@@ -97,7 +104,7 @@ int mlk_rmsnorm_fp8(int type, const void *x, const void *resid, const float *nor
                     int rows, int cols, void *sum, uint8_t *q, float *s) {
     const char *what = "mlk_rmsnorm_fp8";
     if (!type_ok(type)) return refuse(what, "type must be MLK_F32 or MLK_BF16");
-    if (rows < 0 || cols <= 0) return refuse(what, "rows must be >= 0 and cols > 0");
+    if (int e = check_rows(what, rows, "cols", cols)) return e;
     if (!(eps >= 0.0f) || isinf(eps)) return refuse(what, "eps must be finite and >= 0");
     if (rows == 0) return kOk;
     const unsigned size = size_of(type);
@@ -113,7 +120,7 @@ int mlk_rmsnorm_fp8(int type, const void *x, const void *resid, const float *nor
 int mlk_swiglu_fp8(int type, const void *gate_up, int rows, int width, uint8_t *q, float *s) {
     const char *what = "mlk_swiglu_fp8";
     if (!type_ok(type)) return refuse(what, "type must be MLK_F32 or MLK_BF16");
-    if (rows < 0 || width <= 0) return refuse(what, "rows must be >= 0 and width > 0");
+    if (int e = check_rows(what, rows, "width", width)) return e;
     if (rows == 0) return kOk;
     const Pointer list[] = {{gate_up, "gate_up", size_of(type), false}, {q, "q", 1, false},
                             {s, "s", 4, false}};
@@ -128,8 +135,8 @@ int mlk_matmul_fp8(int out_type, const uint8_t *w, const float *ws, const uint8_
                    const void *resid) {
     const char *what = "mlk_matmul_fp8";
     if (!type_ok(out_type)) return refuse(what, "out_type must be MLK_F32 or MLK_BF16");
-    if (rows < 0 || out_width <= 0 || in_width <= 0)
-        return refuse(what, "rows must be >= 0, out_width and in_width > 0");
+    if (int e = check_rows(what, rows, "out_width", out_width)) return e;
+    if (int e = check_rows(what, rows, "in_width", in_width)) return e;
     if (rows == 0) return kOk;
     const unsigned size = size_of(out_type);
     const Pointer list[] = {{w, "w", 1, false},   {ws, "ws", 4, false}, {x, "x", 1, false},
@@ -157,8 +164,10 @@ int mlk_matmul_fp8_grouped(int out_type, const uint8_t *w, const float *ws, cons
                            int groups, const int *offsets, const int *row_ids, int entries) {
     const char *what = "mlk_matmul_fp8_grouped";
     if (!type_ok(out_type)) return refuse(what, "out_type must be MLK_F32 or MLK_BF16");
-    if (entries < 0 || x_rows < 0 || out_width <= 0 || in_width <= 0 || groups <= 0)
-        return refuse(what, "entries and x_rows must be >= 0, out_width, in_width and groups > 0");
+    if (entries < 0 || x_rows < 0 || groups <= 0)
+        return refuse(what, "entries and x_rows must be >= 0, groups > 0");
+    if (int e = check_rows(what, entries, "out_width", out_width)) return e;
+    if (int e = check_rows(what, entries, "in_width", in_width)) return e;
     if (!row_ids && x_rows < entries)
         return refuse(what, "without row_ids x needs a row for each entry");
     if (entries == 0) return kOk;

@@ -148,10 +148,10 @@ template <int BM> __device__ __forceinline__ RowTile row_tile(const Fp8Matmul &p
 }
 
 // Row tiles that `rows` entries in `groups` groups can need.
-template <int BM> long row_tiles(const Fp8Matmul &p) {
-    if (p.groups == 0) return ((long)p.rows + BM - 1) / BM;
+long row_tiles(const Fp8Matmul &p, int bm) {
+    if (p.groups == 0) return ((long)p.rows + bm - 1) / bm;
     const long used = p.groups < p.rows ? p.groups : p.rows;  // groups that can hold a row
-    return (p.rows + used * (BM - 1)) / BM;
+    return (p.rows + used * (bm - 1)) / bm;
 }
 
 // Four neighbouring outputs of a row; those from O on are left out.
@@ -246,38 +246,37 @@ __device__ __forceinline__ void store_row(const Fp8Matmul &p, long row, int o, c
 // ---------------------------------------------------------------------------
 //
 // A workgroup of WO x WM waves makes BO matrix rows x BM tokens; a wave NT x MT
-// results of 16 x 16.  Each step of 128 columns is copied by DMA into one of
-// `STAGES` LDS stages while the ones before it are multiplied: rows of 128 bytes as
-// they lie in memory, 16-byte chunk c of row r at chunk c ^ (r / 2 & 7), so
-// that the rows an operand read touches lie on different banks; the row and
-// matrix scales behind them, copied in pieces of kSpan steps: a scale a
-// token and step is 4 bytes of its own cache line, and copying each step's alone
-// asked the L2 for as many lines as the operands.
+// results of 16 x 16.  Each step of 128 columns is copied by DMA into one of two LDS
+// stages while the step before it is multiplied: rows of 128 bytes as they lie in
+// memory, 16-byte chunk c of row r at chunk c ^ (r / 2 & 7), so that the rows an
+// operand read touches lie on different banks; the row and matrix scales behind
+// them, copied in pieces of kSpan steps: a scale a token and step is 4 bytes of its
+// own cache line, and copying each step's alone asked the L2 for as many lines as
+// the operands.
 constexpr int kSpan = 8;
-template <int BO_, int BM_, int WO_, int WM_, int STAGES_> struct TileShape {
-    static constexpr int BO = BO_, BM = BM_, WO = WO_, WM = WM_, kStages = STAGES_;
+template <int BO_, int BM_, int WO_, int WM_> struct TileShape {
+    static constexpr int BO = BO_, BM = BM_, WO = WO_, WM = WM_;
     static constexpr int kWaves = WO * WM, kThreads = kWaves * kWave;
     static constexpr int NT = BO / 16 / WO, MT = BM / 16 / WM;
     static constexpr int kStage = (BO + BM) * kFp8Block;
     // scales: two groups of kSpan steps, each BM / 8 pieces of 8 tokens by kSpan steps and
-    // one of matrix blocks; behind them the place of copies that stand for none
+    // one of matrix blocks
     static constexpr int kPieces = BM / 8 + 1, kMatrixBlocks = (BO + kFp8Block - 1) / kFp8Block;
-    static constexpr int kScales = kStages * kStage, kScaleGroup = kPieces * 256;
-    static constexpr int kIdle = kScales + 2 * kScaleGroup;
-    // offsets of the rows' scales: BM tokens, 8 matrix blocks, 8 that stand for none
-    static constexpr int kRowOffsets = kIdle + 256;
-    static constexpr int kLds = kRowOffsets + (BM + 16) * 4;
+    static constexpr int kScales = 2 * kStage, kScaleGroup = kPieces * 256;
+    // offsets of the rows' scales: BM tokens, 8 matrix blocks
+    static constexpr int kRowOffsets = kScales + 2 * kScaleGroup;
+    static constexpr int kLds = kRowOffsets + (BM + 8) * 4;
     // the waves that copy: with two on a SIMD one of them
     static constexpr int kCopiers = kWaves == 8 ? 4 : kWaves;
     static constexpr int kWPer = BO / 8 / kCopiers, kXPer = BM / 8 / kCopiers;  // DMA blocks of one
     static constexpr int kDma = kWPer + kXPer;
     static_assert(BO % (8 * kCopiers) == 0 && BM % (8 * kCopiers) == 0, "whole DMA blocks");
-    static_assert((kPieces - 1 + kCopiers - 1) / kCopiers <= kSpan - (kStages - 2) && kMatrixBlocks <= 8 &&
+    static_assert((kPieces - 1 + kCopiers - 1) / kCopiers <= kSpan && kMatrixBlocks <= 8 &&
                       (BO % kFp8Block == 0 || kFp8Block % BO == 0),
                   "a group's scales land before its first step");
     static_assert(BO / 16 % WO == 0 && BM / 16 % WM == 0 && kFp8Block % (16 * NT) == 0,
                   "a wave's matrix rows lie in one block");
-    static_assert(kLds <= 160 * 1024 && (kStages - 1) * (kDma + 1) < 64, "LDS, vmcnt");
+    static_assert(kLds <= 160 * 1024, "LDS");
 };
 
 template <int N> __device__ __forceinline__ void wait_vmcnt() {
@@ -321,7 +320,7 @@ constexpr int kTileGroup = 4;  // row tiles that share matrix rows, one after th
 
 template <class Sh, bool FAST, bool BF16, bool DMA>
 __global__ __launch_bounds__(Sh::kThreads, 2) void fp8_tile_kernel(Fp8Matmul p, int o_tiles, int slots) {
-    constexpr int NT = Sh::NT, MT = Sh::MT, BO = Sh::BO, BM = Sh::BM, S = Sh::kStages;
+    constexpr int NT = Sh::NT, MT = Sh::MT, BO = Sh::BO, BM = Sh::BM;
     constexpr int kWaves = Sh::kWaves;
     extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
     // Workgroups go to the 8 XCDs in turn: each XCD gets a run of neighbouring
@@ -378,25 +377,23 @@ __global__ __launch_bounds__(Sh::kThreads, 2) void fp8_tile_kernel(Fp8Matmul p, 
     const long xs_bytes = x_count * blocks * 4, ws_bytes = (long)(o_blocks - o0 / kFp8Block) * blocks * 4;
     const int sc_lane = lane & 7, sc_step = lane >> 3;
     unsigned *const row_off = reinterpret_cast<unsigned *>(lds + Sh::kRowOffsets);
-    for (int i = threadIdx.x; i < BM + 16; i += Sh::kThreads) {
+    for (int i = threadIdx.x; i < BM + 8; i += Sh::kThreads) {
         const int r = i < BM ? x_row(i) : i - BM < Sh::kMatrixBlocks ? i - BM : -1;
         row_off[i] = r < 0 ? (unsigned)kOutside : (unsigned)r * (unsigned)blocks * 4u;
     }
     __syncthreads();
-    // (pieces behind the last stand for none: three stages count every step's copies alike)
     auto copy_scales = [&](int g, int piece) {
-        const unsigned row = row_off[min(piece, BM / 8 + 1) * 8 + sc_lane];
+        const unsigned row = row_off[piece * 8 + sc_lane];
         const bool rows = piece < BM / 8;
         const bool in = g * kSpan + sc_step < blocks && row != (unsigned)kOutside;
         dma4(buffer_of(rows ? xs_base : ws_base, rows ? xs_bytes : ws_bytes),
              in ? row + sc_step * 4u : (unsigned)kOutside, g * kSpan * 4,
-             (LdsByte *)(lds + (piece <= BM / 8 ? Sh::kScales + (g & 1) * Sh::kScaleGroup + piece * 256
-                                                : Sh::kIdle)));
+             (LdsByte *)(lds + Sh::kScales + (g & 1) * Sh::kScaleGroup + piece * 256));
     };
     // a step's part of the next group's scales
     auto copy_next_scales = [&](int b) {
         const int g = b / kSpan + 1, piece = b % kSpan * Sh::kCopiers + wave;
-        if (S > 2 || piece < Sh::kPieces) copy_scales(g, piece);
+        if (piece < Sh::kPieces) copy_scales(g, piece);
         // (one piece more than the steps have copies)
         if (Sh::kPieces > kSpan * Sh::kCopiers && b % kSpan == 0 && wave == 0) copy_scales(g, Sh::kPieces - 1);
     };
@@ -409,7 +406,7 @@ __global__ __launch_bounds__(Sh::kThreads, 2) void fp8_tile_kernel(Fp8Matmul p, 
             const int q = i < Sh::kWPer ? i : i - Sh::kWPer;
             const int blk = wave + Sh::kCopiers * q;
             const int chunk = (lane & 7) ^ ((blk & 1) * 4 + dma_row / 2);
-            // a row that ends inside the step, or before it: zeros past its end
+            // a row that ends inside the step: zeros past its end
             const bool past = k0 + kFp8Block > p.I && k0 + chunk * 16 >= p.I;
             if (i < Sh::kWPer)
                 dma16(buffer_of(w_base, w_bytes),
@@ -525,49 +522,38 @@ __global__ __launch_bounds__(Sh::kThreads, 2) void fp8_tile_kernel(Fp8Matmul p, 
             }
         }
     };
-    // A wave's DMA completes in order: a step has landed when at most the copies of
-    // the later steps in flight remain.  The barrier after the wait makes every
-    // wave's part visible and frees the stage read last.  (A bare barrier:
-    // __syncthreads() would wait for the DMA in flight as well.)
-#pragma unroll
-    for (int q = 0; q < (Sh::kPieces + kWaves - 1) / kWaves; ++q) copy_scales(0, q * kWaves + wave);
-    static_assert(DMA || S == 2, "one stage ahead");
-    static_assert(S == 2 || Sh::kCopiers == kWaves, "the waits below");
+    for (int piece = wave; piece < Sh::kPieces; piece += kWaves) copy_scales(0, piece);
     // Eight waves: the first four, one on each SIMD, hand the copies to the memory pipe,
     // which holds them up until it has taken them, while the other four multiply.
     const bool copier = wave < Sh::kCopiers;
-    if constexpr (DMA) {
-#pragma unroll
-        for (int b = 0; b < S - 1; ++b)
-            if (copier) copy_tiles(b, b);
-    } else {
-        if (copier) {
+    if (copier) {
+        if constexpr (DMA) {
+            copy_tiles(0, 0);
+        } else {
             load_tiles(0);
             store_tiles(0);
         }
     }
-    int st = 0, fill = S - 1;
     for (int b = 0; b < blocks; ++b) {
-        if constexpr (!DMA) __builtin_amdgcn_s_waitcnt(0);  // (and the stores to LDS)
-        else if (S == 2) wait_vmcnt<0>();
-        else if (b > 0) wait_vmcnt<(S - 2) * (Sh::kDma + 1)>();
-        else wait_vmcnt<(S - 2) * Sh::kDma>();
+        const int st = b & 1;
+        // The wait lands this wave's part of the step; the barrier makes every wave's
+        // visible and frees the stage read last.
+        if constexpr (DMA) wait_vmcnt<0>();
+        else __builtin_amdgcn_s_waitcnt(0);  // (the stores to LDS)
         asm volatile("" ::: "memory");
         __builtin_amdgcn_s_barrier();
         asm volatile("" ::: "memory");
-        if (copier) {
-            if constexpr (DMA) copy_tiles(b + S - 1, fill);
-            else if (b + 1 < blocks) load_tiles(b + 1);
+        const bool more = copier && b + 1 < blocks;
+        if (more) {
+            if constexpr (DMA) copy_tiles(b + 1, st ^ 1);
+            else load_tiles(b + 1);
             copy_next_scales(b);
         }
         if (live) multiply(b, st);
         if constexpr (!DMA) {
-            if (copier && b + 1 < blocks) store_tiles(fill);
+            if (more) store_tiles(st ^ 1);
         }
-        st = st + 1 == S ? 0 : st + 1;
-        fill = fill + 1 == S ? 0 : fill + 1;
     }
-    wait_vmcnt<0>();  // no copy is in flight when the LDS is given back
 
     // Results go to memory through LDS, 16 tokens of a wave at a time: the lanes of a
     // result hold 16 different rows, whose pieces the memory pipe takes one by one,
@@ -818,8 +804,6 @@ __global__ __launch_bounds__(Sh::kThreads) void fp8_stream_kernel(Fp8Matmul p, i
     }
 }
 
-constexpr long kMaxGrid = 0x7FFFFF;  // workgroups of at most 512 threads in a launch
-
 template <class Sh, bool FAST, bool BF16, bool DMA = true>
 int launch_tile(const Fp8Matmul &p, hipStream_t stream) {
     static const bool attr = [] {
@@ -827,10 +811,8 @@ int launch_tile(const Fp8Matmul &p, hipStream_t stream) {
                                    hipFuncAttributeMaxDynamicSharedMemorySize, Sh::kLds) == hipSuccess;
     }();
     (void)attr;
-    const long o_tiles = ((long)p.O + Sh::BO - 1) / Sh::BO, slots = row_tiles<Sh::BM>(p);
+    const long o_tiles = ((long)p.O + Sh::BO - 1) / Sh::BO, slots = row_tiles(p, Sh::BM);
     const long tiles = o_tiles * slots;
-    if (tiles > kMaxGrid - 8) return kErrSize;
-    if (tiles == 0) return kOk;
     hipLaunchKernelGGL((fp8_tile_kernel<Sh, FAST, BF16, DMA>), dim3((unsigned)((tiles + 7) / 8 * 8)),
                        dim3(Sh::kThreads), Sh::kLds, stream, p, (int)o_tiles, (int)slots);
     return hipGetLastError() == hipSuccess ? kOk : kErrLaunch;
@@ -843,9 +825,7 @@ template <class Sh, bool BF16> int launch_stream(const Fp8Matmul &p, hipStream_t
     }();
     (void)attr;
     const long o_tiles = ((long)p.O + Sh::BO - 1) / Sh::BO;
-    const long tiles = row_tiles<Sh::BM>(p) * o_tiles;
-    if (tiles > kMaxGrid) return kErrSize;
-    if (tiles == 0) return kOk;
+    const long tiles = row_tiles(p, Sh::BM) * o_tiles;
     hipLaunchKernelGGL((fp8_stream_kernel<Sh, BF16>), dim3((unsigned)tiles), dim3(Sh::kThreads), Sh::kLds, stream,
                        p, (int)o_tiles);
     return hipGetLastError() == hipSuccess ? kOk : kErrLaunch;
@@ -863,17 +843,20 @@ bool dma_takes(const Fp8Matmul &p) {
 // columns where every CU has at most one, `full` us a block where each CU holds
 // per_cu of them, and in between for numbers in between; workgroups that follow
 // others on their CU start in half the time.  The three numbers of each shape are
-// fitted to its times on MI355X over 260 products (out_width 60 .. 22528, in_width
-// 60 .. 11264, 1 .. 4096 rows, one matrix or up to 160), which they give within 12 %
-// on average; the choice takes 2.5 % longer than the best shape would, 1.4 times at
-// worst.  Some of those times (us; streams by matrix rows x tokens):
-//   22528 x 2048, 16 rows:   stream 16 x 16 10.5, tile 128 x 64 11.7, stream 32 x 32 17.5
-//                 100 rows:  tile 64 x 64 15.5, 128 x 64 17.0, 128 x 128 18.3
-//                 4096 rows: tile 256 x 256 234, 128 x 128 265, 128 x 64 329
-//   2048 x 11264, 1 row:     stream 16 x 8 on 8 waves by DMA 7.1, on 4 through registers 13.9
-//                 100 rows:  stream 32 x 32 16.7, 64 x 64 28.3, tile 64 x 64 41.1
-//                 400 rows:  stream 64 x 64 29.0, tile 64 x 64 42.3, 128 x 64 49.6
-//   2048 x 2048,  100 rows:  stream 32 x 32 6.4, tile 64 x 64 9.9, 128 x 64 12.4
+// fitted to its times on MI355X over 210 products (out_width 333 .. 22528, in_width
+// 777 .. 11264, 1 .. 4096 rows, one matrix, 8 or 64), so that the choice costs
+// little: 0.6 % more than the best shape's time on them, and 1.4 % (25 % at worst)
+// on 110 others of sizes drawn by chance.  Some of those times (bf16, us; streams by
+// matrix rows x tokens, "regs" without DMA):
+//   22528 x 2048, 16 rows:   stream 16 x 16 regs 10.5, tile 64 x 64 11.3, stream 32 x 16 14.5
+//                 100 rows:  tile 64 x 64 14.5, 128 x 128 18.4
+//                 2048 rows: tile 256 x 256 102, 128 x 128 121
+//   2048 x 11264, 1 row:     stream 16 x 8 7.1, 32 x 16 8.8
+//                 40 rows:   stream 32 x 16 10.8, 16 x 16 regs 16.0, 32 x 32 16.4
+//                 100 rows:  stream 32 x 32 16.6, 32 x 16 20.0, 32 x 32 regs 24.7
+//                 230 rows:  stream 32 x 32 regs 27.2, 32 x 32 31.9, 64 x 64 33.4
+//                 400 rows:  stream 64 x 64 33.5, tile 64 x 64 44.3
+//                 1500 rows: tile 64 x 64 59.2, 128 x 128 66.4
 struct Variant {
     int bo, bm, waves, per_cu;  // waves: those that share a reduction
     float start, step, full;
@@ -881,10 +864,10 @@ struct Variant {
     int (*launch)(const Fp8Matmul &, hipStream_t);
 };
 
-template <bool BF16, int BO, int BM, int WO, int WM, int STAGES, bool DMA>
+template <bool BF16, int BO, int BM, int WO, int WM, bool DMA>
 constexpr Variant tile(int per_cu, float start, float step, float full) {
     return Variant{BO, BM, 1, per_cu, start, step, full, DMA,
-                   &launch_tile<TileShape<BO, BM, WO, WM, STAGES>, BF16, BF16, DMA>};
+                   &launch_tile<TileShape<BO, BM, WO, WM>, BF16, BF16, DMA>};
 }
 template <bool BF16, int NT, int XB, int WK, int STAGES, bool DMA>
 constexpr Variant flow(int per_cu, float start, float step, float full) {
@@ -893,51 +876,52 @@ constexpr Variant flow(int per_cu, float start, float step, float full) {
 }
 
 constexpr Variant kBf16Variants[] = {
-    flow<true, 1, 1, 4, 2, false>(4, 3.7f, 0.49f, 0.96f),
-    flow<true, 1, 2, 4, 2, false>(4, 4.1f, 0.54f, 1.06f),
-    flow<true, 1, 2, 8, 2, false>(2, 3.9f, 0.74f, 1.20f),
-    flow<true, 2, 4, 4, 1, false>(2, 4.6f, 1.06f, 1.50f),
-    tile<true, 64, 64, 2, 2, 2, false>(4, 4.0f, 0.67f, 1.39f),
-    tile<true, 128, 128, 2, 2, 2, false>(2, 7.3f, 1.08f, 2.08f),
-    flow<true, 1, 1, 8, 4, true>(1, 4.2f, 0.30f, 0.49f),
-    flow<true, 2, 2, 8, 2, true>(1, 4.4f, 0.60f, 0.72f),
-    flow<true, 2, 4, 4, 4, true>(1, 5.0f, 0.49f, 0.71f),
-    flow<true, 4, 8, 4, 2, true>(1, 7.5f, 1.06f, 1.67f),
-    tile<true, 64, 64, 2, 2, 2, true>(4, 3.5f, 0.44f, 1.26f),
-    tile<true, 128, 64, 4, 1, 3, true>(2, 4.5f, 0.51f, 1.03f),
-    tile<true, 128, 128, 2, 2, 2, true>(2, 6.0f, 0.68f, 1.40f),
-    tile<true, 256, 256, 2, 4, 2, true>(1, 10.4f, 1.34f, 2.07f),
+    flow<true, 1, 1, 4, 2, false>(4, 4.0f, 0.35f, 0.75f),
+    flow<true, 1, 2, 4, 2, false>(4, 4.5f, 0.43f, 0.84f),
+    flow<true, 2, 4, 4, 1, false>(2, 5.0f, 0.77f, 1.10f),
+    tile<true, 64, 64, 2, 2, false>(4, 5.6f, 0.48f, 1.14f),
+    tile<true, 128, 128, 2, 2, false>(2, 10.9f, 0.84f, 1.38f),
+    flow<true, 1, 1, 8, 4, true>(1, 3.4f, 0.34f, 0.60f),
+    flow<true, 2, 2, 8, 2, true>(1, 4.3f, 0.59f, 0.68f),
+    flow<true, 2, 4, 4, 4, true>(1, 4.8f, 0.53f, 0.67f),
+    flow<true, 4, 8, 4, 2, true>(1, 7.4f, 1.19f, 1.42f),
+    tile<true, 64, 64, 2, 2, true>(4, 3.4f, 0.46f, 0.99f),
+    tile<true, 128, 128, 2, 2, true>(2, 4.6f, 0.80f, 1.18f),
+    tile<true, 256, 256, 2, 4, true>(1, 10.4f, 1.28f, 2.04f),
 };
 constexpr Variant kF32Variants[] = {
-    flow<false, 1, 1, 4, 2, false>(4, 4.0f, 0.48f, 0.88f),
-    flow<false, 1, 2, 4, 2, false>(4, 4.2f, 0.53f, 1.06f),
-    flow<false, 1, 2, 8, 2, false>(2, 4.2f, 0.81f, 1.15f),
-    flow<false, 2, 4, 4, 1, false>(2, 4.9f, 1.02f, 1.29f),
-    tile<false, 64, 64, 2, 2, 2, false>(4, 5.5f, 0.68f, 1.45f),
-    tile<false, 128, 128, 2, 2, 2, false>(2, 10.1f, 1.42f, 2.38f),
-    flow<false, 1, 1, 8, 4, true>(1, 4.2f, 0.30f, 0.49f),
-    flow<false, 2, 2, 8, 2, true>(1, 4.4f, 0.60f, 0.72f),
-    flow<false, 2, 4, 4, 4, true>(1, 4.9f, 0.47f, 0.63f),
-    flow<false, 4, 8, 4, 2, true>(1, 6.4f, 1.14f, 1.56f),
-    tile<false, 64, 64, 2, 2, 2, true>(4, 3.7f, 0.55f, 1.35f),
-    tile<false, 128, 64, 4, 1, 3, true>(2, 4.6f, 0.77f, 1.29f),
-    tile<false, 128, 128, 2, 2, 2, true>(2, 5.7f, 1.12f, 1.90f),
+    flow<false, 1, 1, 4, 2, false>(4, 4.1f, 0.33f, 0.87f),
+    flow<false, 1, 2, 4, 2, false>(4, 4.5f, 0.43f, 0.86f),
+    flow<false, 2, 4, 4, 1, false>(2, 4.7f, 0.80f, 1.08f),
+    tile<false, 64, 64, 2, 2, false>(4, 5.4f, 0.53f, 1.48f),
+    tile<false, 128, 128, 2, 2, false>(2, 13.1f, 1.33f, 1.99f),
+    flow<false, 1, 1, 8, 4, true>(1, 3.1f, 0.36f, 0.62f),
+    flow<false, 2, 2, 8, 2, true>(1, 4.3f, 0.59f, 0.68f),
+    flow<false, 2, 4, 4, 4, true>(1, 4.8f, 0.52f, 0.60f),
+    flow<false, 4, 8, 4, 2, true>(1, 7.4f, 1.05f, 1.32f),
+    tile<false, 64, 64, 2, 2, true>(4, 4.0f, 0.54f, 1.19f),
+    tile<false, 128, 128, 2, 2, true>(2, 6.3f, 1.04f, 1.80f),
 };
+
+constexpr long kMaxGrid = 0x7FFFF0;  // workgroups of at most 512 threads in a launch
 
 template <int N> int launch_best(const Variant (&variants)[N], const Fp8Matmul &p, hipStream_t stream) {
     constexpr float kCus = 256.0f;
     const bool dma = dma_takes(p);
     const int blocks = fp8_blocks(p.I);
-    // the groups that rows spread by chance are expected to reach; every second one's
-    // last tile is half full
+    // the groups that rows spread by chance are expected to reach
     const float used =
         p.groups ? p.groups * (1.0f - powf(1.0f - 1.0f / p.groups, (float)p.rows)) : 0.0f;
     const Variant *best = nullptr;
     float least = 0.0f;
     for (const Variant &v : variants) {
         if (v.dma && !dma) continue;
-        const float row_tiles = p.groups ? fmaxf(used, (float)p.rows / v.bm + 0.5f * used)
-                                         : (float)((p.rows - 1) / v.bm + 1);
+        if (row_tiles(p, v.bm) * ((p.O - 1) / v.bo + 1) > kMaxGrid) continue;
+        float row_tiles = (float)((p.rows - 1) / v.bm + 1);
+        if (p.groups) {  // tiles of a group: half of one is spare, but for less than one
+            const float each = (float)p.rows / (used * v.bm);
+            row_tiles = used * fmaxf(1.0f, each > 1.0f ? each + 0.5f : 2.0f * each - 0.5f);
+        }
         const float share = row_tiles * (float)((p.O - 1) / v.bo + 1) / kCus, fill = share / v.per_cu;
         const float rounds = 0.5f * (fill + ceilf(fill));
         const float step = share <= 1.0f  ? v.step
@@ -950,15 +934,15 @@ template <int N> int launch_best(const Variant (&variants)[N], const Fp8Matmul &
             least = cost;
         }
     }
-    return best->launch(p, stream);
+    return best ? best->launch(p, stream) : kErrSize;
 }
 
 }  // namespace
 
 int fp8_matmul(const Fp8Matmul &p, hipStream_t stream) {
     if (p.rows == 0) return kOk;
-    // the scales of a tile's rows, and of gathered rows, are reached by 32-bit offsets
-    if (p.I > (1 << 30) || (p.row_ids && (long)p.x_rows * fp8_blocks(p.I) * 4 >= kOutside)) return kErrSize;
+    // the scales of gathered rows are reached by 32-bit offsets
+    if (p.row_ids && (long)p.x_rows * fp8_blocks(p.I) * 4 >= kOutside) return kErrSize;
     return p.bf16 ? launch_best(kBf16Variants, p, stream) : launch_best(kF32Variants, p, stream);
 }
 

@@ -119,8 +119,9 @@ int mlk_fill_normal(float *out, int64_t n, uint64_t seed, float mean,
  * matrices, the form that fp8 checkpoints of this architecture come in.  A
  * [rows, cols] tensor of codes is dense, its scales are
  * [rows or ceil(rows / 128), ceil(cols / 128)] f32; the last block of a row
- * and of a column may be narrower.  Any width and any alignment of codes is
- * taken; widths that are multiples of 16 at 16-byte addresses are faster.
+ * and of a column may be narrower.  Any width up to 2^30 and any alignment of
+ * codes is taken; widths that are multiples of 16 at 16-byte addresses are
+ * faster.
  *
  * Quantising: scale = max(amax / 448, 2^-126) with amax the block's largest
  * magnitude, code = the e4m3 value nearest to x * (1 / scale), ties to even;
@@ -153,7 +154,8 @@ int mlk_swiglu_fp8(int type, const void *gate_up, int rows, int width,
 /* y[r, o] = sum_i x[r, i] W[o, i] (+ resid[r, o]) for codes x [rows, in_width]
  * with scales xs and codes w [out_width, in_width] with scales ws; y and
  * resid of out_type, MLK_F32 or MLK_BF16 (rounded once, resid added before;
- * y may be resid itself). */
+ * y may be resid itself).  A block's product is scaled by its two scales'
+ * product, which has to be finite in f32. */
 int mlk_matmul_fp8(int out_type, const uint8_t *w, const float *ws,
                    const uint8_t *x, const float *xs, void *y, int out_width,
                    int in_width, int rows, const void *resid);
@@ -163,9 +165,9 @@ int mlk_matmul_fp8(int out_type, const uint8_t *w, const float *ws,
  * groups + 1 numbers that do not decrease; a group may be empty).  Row j of
  * y is the product of x row row_ids[j], or of x row j where row_ids == NULL.
  * Rows of y before offsets[0] and from offsets[groups] on are left as they
- * were.  A row whose row_ids[j] is outside [0, x_rows) becomes NaN; offsets
- * outside [0, entries] or that decrease leave rows out, and nothing is read
- * or written out of range. */
+ * were.  A row whose row_ids[j] is outside [0, x_rows) becomes NaN.  With
+ * offsets that decrease or leave [0, entries] the rows of y are unspecified,
+ * but nothing is read or written out of range. */
 int mlk_matmul_fp8_grouped(int out_type, const uint8_t *w, const float *ws,
                            const uint8_t *x, const float *xs, int x_rows,
                            void *y, int out_width, int in_width, int groups,

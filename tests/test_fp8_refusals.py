@@ -38,6 +38,13 @@ def grouped(dtype=MLK_F32, w=P, ws=P, x=P, xs=P, y=P, out=64, inp=256, groups=3,
     (quantize, dict(rows=-1), "rows"),
     (quantize, dict(cols=0), "cols"),
     (quantize, dict(block_rows=64), "block_rows"),
+    (quantize, dict(cols=(1 << 30) + 1), "cols"),
+    (norm, dict(cols=(1 << 31) - 1), "cols"),
+    (swiglu, dict(width=(1 << 31) - 1), "width"),
+    (matmul, dict(inp=(1 << 30) + 1), "in_width"),
+    (matmul, dict(out=(1 << 31) - 1), "out_width"),
+    (grouped, dict(inp=(1 << 31) - 1), "in_width"),
+    (grouped, dict(out=0), "out_width"),
     (quantize, dict(x=None), "x is null"),
     (quantize, dict(q=None), "q is null"),
     (quantize, dict(s=None), "s is null"),
