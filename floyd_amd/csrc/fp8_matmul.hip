@@ -32,6 +32,7 @@ typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef int i32x8 __attribute__((ext_vector_type(8)));
 typedef unsigned u32x4_any __attribute__((ext_vector_type(4), aligned(2)));
+typedef unsigned u32x4_word __attribute__((ext_vector_type(4), aligned(4)));
 
 __device__ __forceinline__ bf16x8 widen8(unsigned lo, unsigned hi) {
     const bf16x2 a = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, 1.0f, false);
@@ -68,6 +69,22 @@ __device__ __forceinline__ u32x4 load16_any(const uint8_t *p) {
     u32x4 v;
     __builtin_memcpy(&v, p, 16);
     return v;
+}
+
+// Rows at any byte, read by words (333 x 1001 x 1999 f32 11.2 us, by loads of 16 bytes at
+// any byte 12.6): 8 neighbouring lanes hold 128 bytes of a row from its first word on, 16
+// each; a lane's last bytes are in the next lane's first word, and the 8th loads them.  No
+// word is read that holds none of the row's bytes.
+__device__ __forceinline__ const uint8_t *word_of(const uint8_t *p) {
+    return reinterpret_cast<const uint8_t *>((uintptr_t)p & ~(uintptr_t)3);
+}
+// 16 bytes of a lane that start `start` < 4 bytes into the words v
+__device__ __forceinline__ u32x4 shift_in(const u32x4 &v, unsigned end, unsigned start, bool last) {
+    // lane + 1's first word (row_shl:1)
+    const unsigned next = (unsigned)__builtin_amdgcn_update_dpp((int)end, (int)v[0], 0x101, 0xF, 0xF, false);
+    const unsigned e = last ? end : next;
+    return u32x4{__builtin_amdgcn_alignbyte(v[1], v[0], start), __builtin_amdgcn_alignbyte(v[2], v[1], start),
+                 __builtin_amdgcn_alignbyte(v[3], v[2], start), __builtin_amdgcn_alignbyte(e, v[3], start)};
 }
 
 // columns c .. c + 15 of a row of `width` codes, zeros past its end; nothing
@@ -593,7 +610,8 @@ __global__ __launch_bounds__(Sh::kThreads, 2) void fp8_tile_kernel(Fp8Matmul p, 
 // ring of its own, STAGES blocks ahead, so that no wave waits for another until the
 // shares are added through LDS.  Rows of 128 bytes with the tiles' swizzle.
 // Without DMA, for rows at any address: through registers, as far ahead, into one
-// stage a wave.
+// stage a wave.  BYTES: some row does not start at a word; then the pieces are read by
+// words and moved into place, as a load of 16 bytes at any byte takes longer.
 template <int NT_, int XB_, int WK_, int STAGES_, bool DMA_ = true> struct StreamShape {
     static constexpr int NT = NT_, XB = XB_, MT = (XB + 1) / 2, WK = WK_, kStages = STAGES_;
     static constexpr bool DMA = DMA_;
@@ -607,7 +625,7 @@ template <int NT_, int XB_, int WK_, int STAGES_, bool DMA_ = true> struct Strea
     static_assert(kFp8Block % (16 * NT) == 0, "the matrix rows lie in one block");
 };
 
-template <class Sh, bool BF16>
+template <class Sh, bool BF16, bool BYTES>
 __global__ __launch_bounds__(Sh::kThreads) void fp8_stream_kernel(Fp8Matmul p, int o_tiles) {
     constexpr int NT = Sh::NT, MT = Sh::MT, XB = Sh::XB, WK = Sh::WK, S = Sh::kStages;
     extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
@@ -652,7 +670,23 @@ __global__ __launch_bounds__(Sh::kThreads) void fp8_stream_kernel(Fp8Matmul p, i
     const unsigned w_off = (unsigned)dma_row * (unsigned)p.I;
     uint8_t *const ring = lds + wave * Sh::kRing;
     float xs[S][MT], ws[S];
-    u32x4 held[Sh::DMA ? 1 : S][2 * NT + XB];
+    constexpr int kPer = 2 * NT + XB;
+    u32x4 held[Sh::DMA ? 1 : S][kPer];
+    unsigned end[BYTES ? S : 1][kPer];
+    auto row_of = [&](int q) -> const uint8_t * {
+        return q < 2 * NT ? w_base + (long)min(q * 8 + dma_row, p.O - 1 - o0) * p.I
+                          : x_base + (long)x_off[q - 2 * NT] * p.I;
+    };
+    // chunk of row q where this lane's 16 bytes lie in LDS, or come from
+    auto chunk_of = [&](int q) {
+        return (lane & 7) ^ (((q < 2 * NT ? q : q - 2 * NT) & 1) * 4 + dma_row / 2);
+    };
+    unsigned starts = 0;  // of the rows in their words, 2 bits a piece
+    if constexpr (BYTES) {
+        static_assert(kPer <= 16, "starts");
+#pragma unroll
+        for (int q = 0; q < kPer; ++q) starts |= ((unsigned)(uintptr_t)row_of(q) & 3) << (2 * q);
+    }
     auto copy_scales = [&](int b, int st) {
 #pragma unroll
         for (int m = 0; m < MT; ++m)
@@ -664,21 +698,33 @@ __global__ __launch_bounds__(Sh::kThreads) void fp8_stream_kernel(Fp8Matmul p, i
     auto load = [&](int b, int st) {
         if (b >= blocks) return;
         const int k0 = b * kFp8Block;
+        if (k0 + kFp8Block <= p.I) {
 #pragma unroll
-        for (int q = 0; q < 2 * NT + XB; ++q) {
-            const int r = q < 2 * NT ? q : q - 2 * NT;
-            const int c = k0 + ((lane & 7) ^ ((r & 1) * 4 + dma_row / 2)) * 16;
-            const uint8_t *row = q < 2 * NT ? w_base + (long)min(r * 8 + dma_row, p.O - 1 - o0) * p.I
-                                            : x_base + (long)x_off[r] * p.I;
-            if (k0 + kFp8Block <= p.I) held[st][q] = load16_any(row + c);
-            else held[st][q] = load16_tail(row, c, p.I);
+            for (int q = 0; q < kPer; ++q) {
+                const uint8_t *from = row_of(q) + k0 + (BYTES ? lane & 7 : chunk_of(q)) * 16;
+                if constexpr (BYTES) held[st][q] = *reinterpret_cast<const u32x4_word *>(word_of(from));
+                else held[st][q] = load16_any(from);
+            }
+            if constexpr (BYTES) {
+                if ((lane & 7) == 7) {
+#pragma unroll
+                    for (int q = 0; q < kPer; ++q)
+                        end[st][q] = *reinterpret_cast<const unsigned *>(word_of(row_of(q) + k0 + kFp8Block - 1));
+                }
+            }
+        } else {
+#pragma unroll
+            for (int q = 0; q < kPer; ++q)
+                held[st][q] = load16_tail(row_of(q), k0 + (BYTES ? lane & 7 : chunk_of(q)) * 16, p.I);
         }
         copy_scales(b, st);
     };
-    auto store = [&](int st) {
+    auto store = [&](int b, int st) {
+        const bool shift = BYTES && b * kFp8Block + kFp8Block <= p.I;
 #pragma unroll
-        for (int q = 0; q < 2 * NT + XB; ++q)
-            *reinterpret_cast<u32x4 *>(ring + q * 1024 + lane * 16) = held[st][q];
+        for (int q = 0; q < kPer; ++q)
+            *reinterpret_cast<u32x4 *>(ring + q * 1024 + dma_row * kFp8Block + (BYTES ? chunk_of(q) : lane & 7) * 16) =
+                shift ? shift_in(held[st][q], end[st][q], starts >> (2 * q) & 3, (lane & 7) == 7) : held[st][q];
     };
     auto copy = [&](int b, int st) {
         LdsByte *stage = (LdsByte *)(ring + st * Sh::kStage);
@@ -758,7 +804,7 @@ __global__ __launch_bounds__(Sh::kThreads) void fp8_stream_kernel(Fp8Matmul p, i
         for (int s = 0; s < S; ++s) {
             if (t + s >= steps) break;
             if constexpr (!Sh::DMA) {  // a wave's LDS accesses are done in their order
-                store(s);
+                store(wave + (t + s) * WK, s);
                 read(0);
                 multiply(s);
                 load(wave + (t + s + S) * WK, s);
@@ -818,17 +864,23 @@ int launch_tile(const Fp8Matmul &p, hipStream_t stream) {
     return hipGetLastError() == hipSuccess ? kOk : kErrLaunch;
 }
 
-template <class Sh, bool BF16> int launch_stream(const Fp8Matmul &p, hipStream_t stream) {
+template <class Sh, bool BF16, bool BYTES> int launch_stream_of(const Fp8Matmul &p, hipStream_t stream) {
     static const bool attr = [] {
-        return hipFuncSetAttribute(reinterpret_cast<const void *>(&fp8_stream_kernel<Sh, BF16>),
+        return hipFuncSetAttribute(reinterpret_cast<const void *>(&fp8_stream_kernel<Sh, BF16, BYTES>),
                                    hipFuncAttributeMaxDynamicSharedMemorySize, Sh::kLds) == hipSuccess;
     }();
     (void)attr;
     const long o_tiles = ((long)p.O + Sh::BO - 1) / Sh::BO;
     const long tiles = row_tiles(p, Sh::BM) * o_tiles;
-    hipLaunchKernelGGL((fp8_stream_kernel<Sh, BF16>), dim3((unsigned)tiles), dim3(Sh::kThreads), Sh::kLds, stream,
-                       p, (int)o_tiles);
+    hipLaunchKernelGGL((fp8_stream_kernel<Sh, BF16, BYTES>), dim3((unsigned)tiles), dim3(Sh::kThreads), Sh::kLds,
+                       stream, p, (int)o_tiles);
     return hipGetLastError() == hipSuccess ? kOk : kErrLaunch;
+}
+
+template <class Sh, bool BF16> int launch_stream(const Fp8Matmul &p, hipStream_t stream) {
+    if constexpr (!Sh::DMA)
+        if (((uintptr_t)p.w | (uintptr_t)p.x | (unsigned)p.I) & 3) return launch_stream_of<Sh, BF16, true>(p, stream);
+    return launch_stream_of<Sh, BF16, false>(p, stream);
 }
 
 // DMA takes 16-byte chunks, and a tile's rows by 32-bit offsets.
