@@ -343,7 +343,7 @@ def test_grouped(device, dtype, counts, out, inp, spare, gather):
 @pytest.mark.parametrize("dtype", [MLK_F32, MLK_BF16])
 @pytest.mark.parametrize("groups,each,out,inp", [
     (5, 167, 545, 65), (8, 424, 1116, 272), (8, 167, 362, 1984), (4, 372, 150, 1088),
-    (5, 900, 835, 1222), (32, 230, 2048, 272)])
+    (5, 900, 835, 1222), (32, 230, 2048, 272), (270, 60, 130, 64), (300, 40, 130, 66)])
 def test_grouped_of_each_kernel(device, dtype, groups, each, out, inp, gather):
     rng = np.random.default_rng(groups + each)
     counts = rng.multinomial(groups * each, np.full(groups, 1.0 / groups))
