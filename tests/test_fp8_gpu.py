@@ -376,6 +376,113 @@ def test_grouped_bad_offsets_stay_in_range(device, offsets):
     run_grouped(np.random.default_rng(7), MLK_F32, [10, 10, 10], 64, 256, False, offsets=offsets)
 
 
+# ---- past 32 bits -------------------------------------------------------------------
+
+
+def zeros(nbytes):
+    buf = DeviceBuffer(nbytes)
+    buf.zero()
+    return buf
+
+
+@pytest.mark.parametrize("dtype", [MLK_F32, MLK_BF16])
+@pytest.mark.parametrize("x_rows", [1_900_000, 2_200_000])  # codes up to 3.9e9 and 4.5e9 bytes in
+@pytest.mark.parametrize("entries", [5, 300])
+def test_grouped_rows_past_32_bits(device, dtype, x_rows, entries):
+    inp, out = 2048, 96
+    rng = np.random.default_rng(x_rows + entries)
+    where = np.array([0, 1 << 20, (1 << 20) + 1, x_rows - 2, x_rows - 1])
+    rows, scales = fp8_matrix(rng, 5, inp, block_rows=1)
+    w, ws = fp8_matrix(rng, 2, out, inp, block_rows=128)
+    x, xs = zeros(x_rows * inp), zeros(x_rows * U.blocks(inp) * 4)
+    for i, r in enumerate(where):
+        x.upload(rows[i], int(r) * inp)
+        xs.upload(scales[i], int(r) * U.blocks(inp) * 4)
+    take = rng.integers(0, 5, entries)
+    ends = np.array([0, entries // 2, entries], np.int32)
+    bufs = [put(a) for a in (w, ws, ends, where[take].astype(np.int32))]
+    size = 2 if dtype == MLK_BF16 else 4
+    y = Out(entries * out * size)
+    native.matmul_fp8_grouped(dtype, bufs[0][1], bufs[1][1], x.ptr, xs.ptr, y.ptr, out, inp, 2,
+                              bufs[2][1], entries, row_ids=bufs[3][1], x_rows=x_rows)
+    got = y.get(np.uint16 if dtype == MLK_BF16 else F32, (entries, out))
+    got = (U.from_bf16(got) if dtype == MLK_BF16 else got).astype(np.float64)
+    for g in range(2):
+        at = slice(ends[g], ends[g + 1])
+        want, *parts = U.product(rows[take[at]], scales[take[at]], w[g], ws[g])
+        assert np.all(np.abs(got[at] - want) <=
+                      U.product_tolerance(want, *parts, inp, dtype == MLK_BF16))
+
+
+@pytest.mark.parametrize("dtype", [MLK_F32, MLK_BF16])
+def test_matmul_outputs_past_32_bits(device, dtype):
+    rows, out, inp = 800_000, 4096, 16  # 3.3e9 outputs
+    size = 2 if dtype == MLK_BF16 else 4
+    rng = np.random.default_rng(8)
+    where = np.array([0, (1 << 19) - 1, 1 << 19, rows - 1])
+    x, xs = fp8_matrix(rng, 4, inp, block_rows=1)
+    w, ws = fp8_matrix(rng, out, inp, block_rows=128)
+    xb, xsb, y = zeros(rows * inp), zeros(rows * 4), zeros(rows * out * size)
+    for i, r in enumerate(where):
+        xb.upload(x[i], int(r) * inp)
+        xsb.upload(xs[i], int(r) * 4)
+    (wb, wat), (wsb, wsat) = put(w), put(ws)
+    native.matmul_fp8(dtype, wat, wsat, xb.ptr, xsb.ptr, y.ptr, out, inp, rows)
+    want, *parts = U.product(x, xs, w, ws)
+    room = U.product_tolerance(want, *parts, inp, dtype == MLK_BF16)
+    for i, r in enumerate(where):
+        got = y.download(np.uint16 if dtype == MLK_BF16 else F32, out, int(r) * out * size)
+        got = (U.from_bf16(got) if dtype == MLK_BF16 else got).astype(np.float64)
+        assert np.all(np.abs(got - want[i]) <= room[i])
+    for r in (1, rows - 2):  # rows of zeros between them
+        assert not y.download(np.uint8, out * size, r * out * size).any()
+
+
+@pytest.mark.parametrize("what", ["rows", "matrix", "norm", "swiglu"])
+def test_rows_past_32_bits(device, what):
+    rows, cols = 640_000, 4096  # 2.6e9 values, 5.2e9 bytes of bf16
+    rng = np.random.default_rng(9)
+    width = cols * (2 if what == "swiglu" else 1)
+    where = np.array([0, (1 << 19) - 1, 1 << 19, rows - 1])
+    raw, v = typed(MLK_BF16, rows_of(rng, 4, width))
+    x, q = zeros(rows * width * 2), DeviceBuffer(rows * cols)
+    per = U.blocks(cols)
+    s = DeviceBuffer((U.blocks(rows) if what == "matrix" else rows) * per * 4)
+    for i, r in enumerate(where):
+        x.upload(raw[i], int(r) * width * 2)
+    norm = put(np.ones(cols, F32))
+    if what == "rows":
+        native.quantize_fp8(MLK_BF16, x.ptr, rows, cols, 1, q.ptr, s.ptr)
+    elif what == "matrix":
+        native.quantize_fp8(MLK_BF16, x.ptr, rows, cols, 128, q.ptr, s.ptr)
+    elif what == "norm":
+        native.rmsnorm_fp8(MLK_BF16, x.ptr, norm[1], rows, cols, q.ptr, s.ptr)
+    else:
+        native.swiglu_fp8(MLK_BF16, x.ptr, rows, cols, q.ptr, s.ptr)
+    v = v.astype(np.float64)
+    for i, r in enumerate(where):
+        code = q.download(np.uint8, cols, int(r) * cols)[None]
+        at = int(r) // (128 if what == "matrix" else 1)
+        scale = s.download(F32, per, at * per * 4)[None]
+        if what == "rows":
+            one, sc = U.quantize(v[i:i + 1].astype(F32), 1)
+            np.testing.assert_array_equal(code, one)
+            np.testing.assert_array_equal(scale, sc)
+        elif what == "matrix":  # the rows of one block are one below the other
+            near = v[(where // 128) == at].astype(F32)
+            one, sc = U.quantize(near, 128)
+            np.testing.assert_array_equal(scale, sc)
+            mine = np.flatnonzero(where[where // 128 == at] == r)[0]
+            np.testing.assert_array_equal(code[0], one[mine])
+        elif what == "norm":
+            h = v[i:i + 1]
+            h = h / np.sqrt((h * h).mean(1, keepdims=True) + F32(1e-5).astype(np.float64))
+            U.check_codes(code, scale, h, ((cols / 256 + 18) / 2 + 6) * U.HALF_F32)  # as above
+        else:
+            g, u = v[i:i + 1, :cols], v[i:i + 1, cols:]
+            U.check_codes(code, scale, g / (1.0 + np.exp(-g)) * u, 9 * U.HALF_F32)
+
+
 # ---- calls at once, and the operators one after the other ---------------------------
 
 
