@@ -292,7 +292,7 @@ __device__ __forceinline__ void store_row(const Fp8Matmul &p, long row, int o, c
 // own cache line, and copying each step's alone asked the L2 for as many lines as
 // the operands.
 //
-// 256 x 256 (bf16 outputs, 160 KB of LDS) asks the L2 for least: 4096 x 22528 x 2048
+// 256 x 256 (bf16 outputs, 146 KB of LDS) asks the L2 for least: 4096 x 22528 x 2048
 // 197 us, 1920 TFLOP/s, on 128 x 128 228.  A tile there takes 2 us to its first copies,
 // 3 to the first step, 1.7 a step (1.1 of it matrix instructions), and 5 for its
 // results, which all CUs store at once.  f32 outputs, 128 x 128: 366 us, 1030 TFLOP/s,
