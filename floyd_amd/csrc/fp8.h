@@ -22,6 +22,13 @@ constexpr int kFp8MaxWidth = 1 << 30;
 
 inline int fp8_blocks(int n) { return (n - 1) / kFp8Block + 1; }  // n > 0
 
+// Scalar offset of a copy of column block b, `bytes` a block.  The range check takes it
+// from the buffer's length before it looks at a lane's offset, so it has to stay inside
+// the buffer: a copy past the last block, whose lanes are all out of range, takes 0.
+__host__ __device__ constexpr int fp8_scalar_offset(int b, int blocks, int bytes) {
+    return b < blocks ? b * bytes : 0;
+}
+
 // Rows to quantise.  bf16: x (and resid, sum) are bfloat16, else f32.
 struct Fp8Rows {
     bool bf16 = false;

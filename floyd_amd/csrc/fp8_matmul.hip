@@ -432,7 +432,7 @@ __global__ __launch_bounds__(Sh::kThreads, 2) void fp8_tile_kernel(Fp8Matmul p, 
         const bool rows = piece < BM / 8;
         const bool in = g * kSpan + sc_step < blocks && row != (unsigned)kOutside;
         dma4(buffer_of(rows ? xs_base : ws_base, rows ? xs_bytes : ws_bytes),
-             in ? row + sc_step * 4u : (unsigned)kOutside, g * kSpan * 4,
+             in ? row + sc_step * 4u : (unsigned)kOutside, fp8_scalar_offset(g * kSpan, blocks, 4),
              (LdsByte *)(lds + Sh::kScales + (g & 1) * Sh::kScaleGroup + piece * 256));
     };
     // a step's part of the next group's scales
@@ -720,12 +720,13 @@ __global__ __launch_bounds__(Sh::kThreads) void fp8_stream_kernel(Fp8Matmul p, i
         for (int q = 0; q < kPer; ++q) starts |= ((unsigned)(uintptr_t)row_of(q) & 3) << (2 * q);
     }
     auto copy_scales = [&](int b, int st) {
+        const int at = fp8_scalar_offset(b, blocks, 4);
 #pragma unroll
         for (int m = 0; m < MT; ++m)
             xs[st][m] = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(
-                buffer_of(xs_base, xs_bytes), b < blocks ? xs_off[m] : (unsigned)kOutside, b * 4, 0));
+                buffer_of(xs_base, xs_bytes), b < blocks ? xs_off[m] : (unsigned)kOutside, at, 0));
         ws[st] = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(
-            buffer_of(ws_base, ws_bytes), b < blocks ? 0u : (unsigned)kOutside, b * 4, 0));
+            buffer_of(ws_base, ws_bytes), b < blocks ? 0u : (unsigned)kOutside, at, 0));
     };
     auto load = [&](int b, int st) {
         if (b >= blocks) return;
@@ -760,20 +761,20 @@ __global__ __launch_bounds__(Sh::kThreads) void fp8_stream_kernel(Fp8Matmul p, i
     };
     auto copy = [&](int b, int st) {
         LdsByte *stage = (LdsByte *)(ring + st * Sh::kStage);
-        const int k0 = b * kFp8Block;
+        const int k0 = b * kFp8Block, at = fp8_scalar_offset(b, blocks, kFp8Block);
 #pragma unroll
         for (int q = 0; q < 2 * NT; ++q) {
             const int chunk = (lane & 7) ^ ((q & 1) * 4 + dma_row / 2);
             const bool past = k0 + chunk * 16 >= p.I;  // (of a block past the last, all)
             dma16(buffer_of(w_base, w_bytes),
                   past ? (unsigned)kOutside : w_off + (unsigned)(q * 8) * (unsigned)p.I + (unsigned)(chunk * 16),
-                  k0, stage + q * 1024);
+                  at, stage + q * 1024);
         }
 #pragma unroll
         for (int q = 0; q < XB; ++q) {
             const int chunk = (lane & 7) ^ ((q & 1) * 4 + dma_row / 2);
             const bool past = k0 + chunk * 16 >= p.I;
-            dma16(buffer_of(x_base, x_bytes), past ? (unsigned)kOutside : x_off[q] + (unsigned)(chunk * 16), k0,
+            dma16(buffer_of(x_base, x_bytes), past ? (unsigned)kOutside : x_off[q] + (unsigned)(chunk * 16), at,
                   stage + (2 * NT + q) * 1024);
         }
         copy_scales(b, st);
