@@ -22,6 +22,14 @@ constexpr int kFp8MaxWidth = 1 << 30;
 
 inline int fp8_blocks(int n) { return (n - 1) / kFp8Block + 1; }  // n > 0
 
+// Offsets from a buffer's first row stay below this; a load at it is out of the buffer.
+constexpr long kFp8Outside = 0xF0000000L;
+// Whether the scales of `rows` rows, a tile's or all that row_ids may name, are reached by
+// such offsets.
+inline bool fp8_scales_in_reach(long rows, int I) {
+    return rows * fp8_blocks(I) * 4 < kFp8Outside;
+}
+
 // Scalar offset of a copy of column block b, `bytes` a block.  The range check takes it
 // from the buffer's length before it looks at a lane's offset, so it has to stay inside
 // the buffer: a copy past the last block, whose lanes are all out of range, takes 0.

@@ -10,9 +10,9 @@ using namespace mlh;
 
 namespace {
 
-int refuse(const char *what, const std::string &why) {
+int refuse(const char *what, const std::string &why, int status = kErrArgs) {
     set_last_error(std::string(what) + ": " + why);
-    return kErrArgs;
+    return status;
 }
 
 // One pointer of a call: its name, how its values are aligned, whether it may
@@ -170,6 +170,9 @@ int mlk_matmul_fp8_grouped(int out_type, const uint8_t *w, const float *ws, cons
     if (int e = check_rows(what, entries, "in_width", in_width)) return e;
     if (!row_ids && x_rows < entries)
         return refuse(what, "without row_ids x needs a row for each entry");
+    if (row_ids && !fp8_scales_in_reach(x_rows, in_width))
+        return refuse(what, "with row_ids x_rows * ceil(in_width / 128) must be below 0x3C000000",
+                      kErrSize);
     if (entries == 0) return kOk;
     if (x_rows == 0) return refuse(what, "x has no rows");
     const Pointer list[] = {{w, "w", 1, false},   {ws, "ws", 4, false},

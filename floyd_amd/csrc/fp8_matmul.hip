@@ -327,8 +327,7 @@ template <int N> __device__ __forceinline__ void wait_vmcnt() {
     __builtin_amdgcn_s_waitcnt((N & 15) | ((N >> 4) << 14) | (7 << 4) | (15 << 8));
 }
 
-// Offsets from a tile's first row stay below this; a load at it is out of the buffer.
-constexpr long kOutside = 0xF0000000L;
+constexpr long kOutside = kFp8Outside;
 
 // Buffer of `bytes` from base: loads at offsets of that and more read zero.
 __device__ __forceinline__ __amdgpu_buffer_rsrc_t buffer_of(const void *base, long bytes) {
@@ -1001,6 +1000,7 @@ template <int N> int launch_best(const Variant (&variants)[N], const Fp8Matmul &
     float least = 0.0f;
     for (const Variant &v : variants) {
         if (v.dma && !dma) continue;
+        if (!fp8_scales_in_reach(v.bm, p.I)) continue;
         if (row_tiles(p, v.bm) * ((p.O - 1) / v.bo + 1) > kMaxGrid) continue;
         float row_tiles = (float)((p.rows - 1) / v.bm + 1);
         if (p.groups) {  // tiles of a group: half of one is spare, but for less than one
@@ -1026,8 +1026,7 @@ template <int N> int launch_best(const Variant (&variants)[N], const Fp8Matmul &
 
 int fp8_matmul(const Fp8Matmul &p, hipStream_t stream) {
     if (p.rows == 0) return kOk;
-    // the scales of gathered rows are reached by 32-bit offsets
-    if (p.row_ids && (long)p.x_rows * fp8_blocks(p.I) * 4 >= kOutside) return kErrSize;
+    if (p.row_ids && !fp8_scales_in_reach(p.x_rows, p.I)) return kErrSize;
     return p.bf16 ? launch_best(kBf16Variants, p, stream) : launch_best(kF32Variants, p, stream);
 }
 

@@ -164,6 +164,7 @@ int mlk_matmul_fp8(int out_type, const uint8_t *w, const float *ws,
  * other, group g's from offsets[g] to offsets[g + 1] (device memory,
  * groups + 1 numbers that do not decrease; a group may be empty).  Row j of
  * y is the product of x row row_ids[j], or of x row j where row_ids == NULL.
+ * With row_ids x_rows * ceil(in_width / 128) has to be below 0x3C000000 (-4).
  * Rows of y before offsets[0] and from offsets[groups] on are left as they
  * were.  A row whose row_ids[j] is outside [0, x_rows) becomes NaN.  With
  * offsets that decrease or leave [0, entries] the rows of y are unspecified,
