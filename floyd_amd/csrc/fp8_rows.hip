@@ -161,19 +161,35 @@ __device__ __forceinline__ void store_codes(const float (&v)[kVec], float inv, u
 // the hardware's 2^x and reciprocal (one last place each): with expf and a division
 // the arithmetic took longer than the memory, 12288 rows of 1408 bf16 22.8 against
 // 15.0 us.
-__device__ __forceinline__ float silu_times(float g, float u) {
+// FAR: below the gate kFarGate, where 1 + exp(-g) is exp(-g), silu(g) is g exp(g), by
+// 2^100 exp(g) = 2^(100 - t) (1 - r ln 2).  The reciprocal would soon be below f32's
+// normal range, which the hardware gives as 0, and exp(-g) infinite.
+constexpr float kFarGate = -80.0f;
+template <bool FAR> __device__ __forceinline__ float silu_times(float g, float u) {
+#pragma clang fp contract(off)  // (100 - t is to be that of the rounded t)
     constexpr float kLog2e = 1.44269502f, kLog2eRest = 1.92596299e-8f, kLn2 = 0.693147182f;
     const float t = -g * kLog2e;
     const float r = fmaf(-g, kLog2eRest, fmaf(-g, kLog2e, -t));
-    const float p = __builtin_amdgcn_exp2f(t);
-    // (an overflowing exp has no rest: infinity times 0)
-    const float e = fabsf(t) < 128.0f ? fmaf(p, r * kLn2, p) : p;
-    return g * __builtin_amdgcn_rcpf(1.0f + e) * u;
+    const float p = __builtin_amdgcn_exp2f(FAR ? 100.0f - t : t);
+    // (2^x of 0 or infinity has no rest: r may be infinite)
+    const float e = fabsf(t) < (FAR ? 256.0f : 128.0f) ? fmaf(p, r * (FAR ? -kLn2 : kLn2), p) : p;
+    return FAR ? g * e * u * 0x1p-100f : g * __builtin_amdgcn_rcpf(1.0f + e) * u;
 }
 
 __device__ __forceinline__ void swiglu8(float (&g)[kVec], const float (&u)[kVec]) {
+    float v[kVec], least = g[0];
 #pragma unroll
-    for (int i = 0; i < kVec; ++i) g[i] = silu_times(g[i], u[i]);
+    for (int i = 0; i < kVec; ++i) {
+        v[i] = silu_times<false>(g[i], u[i]);
+        least = fminf(least, g[i]);  // (passes NaN by)
+    }
+    if (least < kFarGate) {
+#pragma unroll
+        for (int i = 0; i < kVec; ++i)
+            if (g[i] < kFarGate) v[i] = silu_times<true>(g[i], u[i]);
+    }
+#pragma unroll
+    for (int i = 0; i < kVec; ++i) g[i] = v[i];
 }
 
 // Blocks of 1 x 128, each on its own: plain rows, or gate and up halves.
