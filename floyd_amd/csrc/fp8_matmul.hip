@@ -298,7 +298,7 @@ __device__ __forceinline__ void store_row(const Fp8Matmul &p, long row, int o, c
 // the operands.
 //
 // 256 x 256 (bf16 outputs, 146 KB of LDS) asks the L2 for least: 4096 x 22528 x 2048
-// 197 us, 1920 TFLOP/s, on 128 x 128 228.  A tile there takes 2 us to its first copies,
+// 199 us, 1900 TFLOP/s, on 128 x 128 237.  A tile there takes 2 us to its first copies,
 // 3 to the first step, 1.7 a step (1.1 of it matrix instructions), and 5 for its
 // results, which all CUs store at once.  f32 outputs, 128 x 128: 366 us, 1030 TFLOP/s,
 // bound by the widening beside the matrix instructions.
@@ -646,8 +646,9 @@ __global__ __launch_bounds__(Sh::kThreads, 2) void fp8_tile_kernel(Fp8Matmul p, 
 // words and moved into place, as a load of 16 bytes at any byte takes longer.
 //
 // Bound by the matrix where it is read once: 22528 x 2048, 1 row, 9.4 us, 4.9 TB/s; the
-// experts of 8 tokens, 2816 x 2048, 35 us, 5.7 TB/s.  With more rows each strip of 8 or
-// 16 reads it from the L2 again: 2048 x 11264, 61 rows, 11.4 us.
+// 27 of 64 experts that 8 tokens reach, 2816 x 2048, 34 us, 4.6 TB/s.  With more rows
+// each strip of 8 or 16 reads it from the L2 again, two steps a wave in flight: 2048 x
+// 11264, 61 rows, 11.4 us.
 template <int NT_, int XB_, int WK_, int STAGES_, bool DMA_ = true> struct StreamShape {
     static constexpr int NT = NT_, XB = XB_, MT = (XB + 1) / 2, WK = WK_, kStages = STAGES_;
     static constexpr bool DMA = DMA_;

@@ -121,7 +121,8 @@ int mlk_fill_normal(float *out, int64_t n, uint64_t seed, float mean,
  * [rows or ceil(rows / 128), ceil(cols / 128)] f32; the last block of a row
  * and of a column may be narrower.  Any width up to 2^30 and any alignment of
  * codes is taken; widths that are multiples of 16 at 16-byte addresses are
- * faster.
+ * faster.  (A product of more than 2^23 - 16 tiles of 128 x 128 results, those
+ * of a group its own, may be refused with -4.)
  *
  * Quantising: scale = max(amax / 448, 2^-126) with amax the block's largest
  * magnitude, code = the e4m3 value nearest to x * (1 / scale), ties to even;
