@@ -36,8 +36,8 @@ def listed():
     return [
         # one decoded token of one request: the smallest call
         batch("append_f32_1", "append", "f32", "bf16", 1, 1000, 1000),
-        # chunks of 8 prompts, 4093 new rows in all, that go to 4 bits
-        batch("append_fp4_4093", "append", "bf16", "fp4", 8, 512, 4096, new=910),
+        # chunks of 8 prompts, 4095 new rows in all, that go to 4 bits
+        batch("append_fp4_4095", "append", "bf16", "fp4", 8, 512, 4096, new=910),
         # a request's prefix read back for an attention on expanded heads
         batch("gather_fp4_8192", "gather", "bf16", "fp4", 1, 8192, 8192),
         # ragged prefixes of several requests
