@@ -13,6 +13,7 @@
 // All three are bound by memory: 16 lanes hold a block of 128 columns, 8 values
 // a lane, so a wave reads 2 KB (f32) or 1 KB (bf16) of a row in one piece and
 // stores its codes 8 bytes a lane.
+#include "bf16.h"
 #include "fp8.h"
 #include "mlh_device.h"
 #include "mlh_host.h"
@@ -30,15 +31,6 @@ constexpr int kGroups = kThreads / kLanes;    // blocks a workgroup holds at onc
 
 template <bool BF16> struct Elem { using type = float; };
 template <> struct Elem<true> { using type = uint16_t; };
-
-__device__ __forceinline__ float bf16_value(unsigned bits) { return __uint_as_float(bits << 16); }
-
-// to the nearest bf16, ties to even; a NaN stays one
-__device__ __forceinline__ unsigned bf16_bits(float v) {
-    const unsigned u = __float_as_uint(v);
-    if (v != v) return (u >> 16) | 0x40u;
-    return (u + 0x7FFFu + ((u >> 16) & 1u)) >> 16;
-}
 
 // The bits of columns c .. c + 7 of a row at any address, zeros from `cols` on.
 // (Turned into values apart from the loads: a branch that uses what it loads waits

@@ -1,0 +1,305 @@
+// logprobs.hip -- log probabilities of given tokens, entropies and the most likely tokens
+// of rows of logits (gfx950, wave64).
+//
+//   m = max x, Z = sum exp(x - m), T = sum (x - m) exp(x - m)
+//   log p_t = (x_t - m) - log Z,   H = log Z - T / Z
+//
+// A row is cut into pieces, one a workgroup, which holds its piece in registers: one pass
+// over the memory.  A second launch joins a row's pieces.  The sums go into 64 bits 16
+// bytes of logits at a time; those among which the piece's maximum may be are added one by
+// one, since next to its 1 what makes a likely token's log p would be lost.
+//
+// The top k: the k-th largest of the threads' own largest is a bound that at least k values
+// reach, and only values of k threads do, so what is left to be put in order is few however
+// the values lie.  (value, index) are compared as one whole number, all different.
+#include "bf16.h"
+#include "latent.h"
+#include "mlh_device.h"
+#include "mlh_host.h"
+
+namespace mlh {
+
+namespace {
+
+constexpr int kThreads = 256;
+constexpr int kWaves = kThreads / kWave;
+constexpr int kFew = 8, kMany = 32;  // values a thread holds
+// Pieces of kMany values a thread, where that gives the chip's 256 CUs two workgroups each.
+constexpr long kManyFrom = 512;
+
+typedef u32x4 u32x4_any __attribute__((aligned(2)));
+typedef unsigned long long Rank;  // value, then the lower index first; 0: none
+
+__device__ __forceinline__ Rank rank_of(float v, unsigned index) {
+    if (v != v) return 0;
+    const unsigned u = __float_as_uint(v + 0.0f);  // (-0 is 0)
+    return (Rank)(u ^ ((int)u < 0 ? 0xFFFFFFFFu : 0x80000000u)) << 32 | (0xFFFFFFFFu - index);
+}
+__device__ __forceinline__ unsigned index_of(Rank r) { return 0xFFFFFFFFu - (unsigned)r; }
+__device__ __forceinline__ float value_of(Rank r) {
+    const unsigned u = (unsigned)(r >> 32);
+    return __uint_as_float(u ^ ((int)u < 0 ? 0x80000000u : 0xFFFFFFFFu));
+}
+
+struct Stats {
+    double sum, mean;  // Z, T
+    float top;         // m
+    float pad;
+};
+
+__device__ __forceinline__ double wave_sum64(double v) {
+#pragma unroll
+    for (int o = 32; o >= 1; o >>= 1) v += __shfl_xor(v, o, kWave);
+    return v;
+}
+
+// The largest `top` ranks among `n` candidates in LDS, in order, into out[0 .. top).
+__device__ __forceinline__ void put_in_order(const Rank *found, int n, int top, Rank *out) {
+    for (int i = threadIdx.x; i < n; i += kThreads) {
+        const Rank mine = found[i];
+        int above = 0;
+        for (int j = 0; j < n; ++j) above += found[j] > mine;
+        if (above < top) out[above] = mine;
+    }
+    for (int i = n + threadIdx.x; i < top; i += kThreads) out[i] = 0;
+}
+
+// The `top`-th largest of the threads' ranks (0 where fewer have one).
+__device__ __forceinline__ Rank bound_of(Rank mine, int top, Rank *all, Rank *bound) {
+    all[threadIdx.x] = mine;
+    if (threadIdx.x == 0) *bound = 0;
+    __syncthreads();
+    int above = 0;
+#pragma unroll 16
+    for (int j = 0; j < kThreads; ++j) above += all[j] > mine;
+    if (mine && above == top - 1) *bound = mine;
+    __syncthreads();
+    return *bound;
+}
+
+__device__ __forceinline__ float from_bits(unsigned w, int half) {
+    return __uint_as_float(half ? w & 0xFFFF0000u : w << 16);
+}
+
+// Log probability and entropy from a row's sums.
+__device__ __forceinline__ void finish(const TokenLogprobs &p, int r, float top, double sum, double mean) {
+    const double rest = log(sum);
+    // (sums of a row with nothing above -inf, with +inf or NaN are NaN already)
+    const int token = p.tokens[r];
+    float at = NAN;
+    if ((unsigned)token < (unsigned)p.vocab) {
+        const long i = (long)r * p.stride + token;
+        at = p.bf16 ? bf16_value(static_cast<const uint16_t *>(p.logits)[i]) : static_cast<const float *>(p.logits)[i];
+    }
+    p.logprobs[r] = (float)((double)at - (double)top - rest);
+    if (p.entropy) p.entropy[r] = (float)(rest - mean / sum);
+}
+
+__device__ __forceinline__ void finish_top(const TokenLogprobs &p, int r, int k, Rank rank, float top, double sum) {
+    const long at = (long)r * p.top + k;
+    p.top_ids[at] = rank ? (int)index_of(rank) : -1;
+    p.top_logprobs[at] = rank ? (float)((double)value_of(rank) - (double)top - log(sum)) : NAN;
+}
+
+template <bool BF16, bool TOP, int N>
+__global__ __launch_bounds__(kThreads) void logprobs_piece_kernel(TokenLogprobs p, int pieces, Stats *stats,
+                                                                  Rank *ranks) {
+    constexpr int kVec = BF16 ? 8 : 4, kVecs = N / kVec;
+    __shared__ float tops[kWaves];
+    __shared__ double sums[kWaves][2];
+    __shared__ Rank all[TOP ? kThreads : 1], found[TOP ? kLogprobsMaxTop * N : 1], sorted[TOP ? kLogprobsMaxTop : 1];
+    __shared__ Rank bound;
+    __shared__ int count;
+    const int t = threadIdx.x, wave = t / kWave, lane = t % kWave;
+    const int r = blockIdx.x / pieces, piece = blockIdx.x - r * pieces;
+    using T = typename std::conditional<BF16, uint16_t, float>::type;
+    const T *row = static_cast<const T *>(p.logits) + (long)r * p.stride;
+    const int base = piece * kThreads * N;
+    const auto first = [&](int k) { return base + (k * kThreads + t) * kVec; };
+    u32x4 bits[kVecs];
+#pragma unroll
+    for (int k = 0; k < kVecs; ++k) {
+        const int i = first(k);
+        if (i + kVec <= p.vocab) {
+            bits[k] = *reinterpret_cast<const u32x4_any *>(row + i);
+        } else {
+            constexpr unsigned kLowest = BF16 ? 0xFF80FF80u : 0xFF800000u;  // -inf
+            bits[k] = u32x4{kLowest, kLowest, kLowest, kLowest};
+#pragma unroll
+            for (int x = 0; x < kVec; ++x) {
+                if (i + x >= p.vocab) break;
+                if constexpr (BF16)
+                    bits[k][x / 2] = x % 2 ? (bits[k][x / 2] & 0xFFFFu) | (unsigned)row[i + x] << 16
+                                           : (bits[k][x / 2] & 0xFFFF0000u) | row[i + x];
+                else bits[k][x] = __float_as_uint(row[i + x]);
+            }
+        }
+    }
+    const auto value = [&](int k, int x) {
+        if constexpr (BF16) return from_bits(bits[k][x / 2], x % 2);
+        else return __uint_as_float(bits[k][x]);
+    };
+    float vec_top[kVecs], mine = -INFINITY;
+#pragma unroll
+    for (int k = 0; k < kVecs; ++k) {
+        vec_top[k] = -INFINITY;
+#pragma unroll
+        for (int x = 0; x < kVec; ++x) vec_top[k] = fmaxf(vec_top[k], value(k, x));
+        mine = fmaxf(mine, vec_top[k]);
+    }
+    const float wave_top = wave_max(mine);
+    if (lane == 0) tops[wave] = wave_top;
+    if (TOP && t == 0) count = 0;
+    __syncthreads();
+    const float top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
+    double sum = 0.0, mean = 0.0;
+#pragma unroll
+    for (int k = 0; k < kVecs; ++k) {
+        float e[kVec], s = 0.0f, m = 0.0f;
+#pragma unroll
+        for (int x = 0; x < kVec; ++x) {
+            const float d = value(k, x) - top;
+            e[x] = expf(d);
+            // (-inf has no part; a piece of nothing else has top -inf and d NaN)
+            if (value(k, x) == -INFINITY) e[x] = 0.0f;
+            else m += e[x] * d;
+            s += e[x];
+        }
+        if (vec_top[k] - top > -0.7f) {
+#pragma unroll
+            for (int x = 0; x < kVec; ++x) sum += (double)e[x];
+        } else {
+            sum += (double)s;
+        }
+        mean += (double)m;
+    }
+    sum = wave_sum64(sum);
+    mean = wave_sum64(mean);
+    if (lane == 0) sums[wave][0] = sum, sums[wave][1] = mean;
+    __syncthreads();
+    sum = (sums[0][0] + sums[1][0]) + (sums[2][0] + sums[3][0]);
+    mean = (sums[0][1] + sums[1][1]) + (sums[2][1] + sums[3][1]);
+    if constexpr (TOP) {
+        unsigned at = 0;
+        bool any = false;
+#pragma unroll
+        for (int k = kVecs - 1; k >= 0; --k)
+#pragma unroll
+            for (int x = kVec - 1; x >= 0; --x)
+                if (value(k, x) == mine && first(k) + x < p.vocab) at = first(k) + x, any = true;
+        const Rank least = bound_of(any ? rank_of(mine, at) : 0, p.top, all, &bound);
+#pragma unroll
+        for (int k = 0; k < kVecs; ++k) {
+            if (rank_of(vec_top[k], first(k)) < least) continue;
+#pragma unroll
+            for (int x = 0; x < kVec; ++x) {
+                const Rank rank = first(k) + x < p.vocab ? rank_of(value(k, x), first(k) + x) : 0;
+                if (rank && rank >= least) found[atomicAdd(&count, 1)] = rank;
+            }
+        }
+        __syncthreads();
+        put_in_order(found, count, p.top, sorted);
+        __syncthreads();
+    }
+    if (pieces == 1) {
+        if (top == -INFINITY) sum = NAN;
+        if (t == 0) finish(p, r, top, sum, mean);
+        if (TOP && t < p.top) finish_top(p, r, t, sorted[t], top, sum);
+        return;
+    }
+    if (t == 0) stats[blockIdx.x] = {sum, mean, top, 0.0f};
+    if (TOP && t < p.top) ranks[(long)blockIdx.x * p.top + t] = sorted[t];
+}
+
+// Joins a row's pieces.
+template <bool TOP>
+__global__ __launch_bounds__(kThreads) void logprobs_join_kernel(TokenLogprobs p, int pieces, const Stats *stats,
+                                                                 const Rank *ranks) {
+    __shared__ float tops[kWaves];
+    __shared__ double sums[kWaves][2];
+    __shared__ Rank all[TOP ? kThreads : 1], sorted[TOP ? kLogprobsMaxTop : 1];
+    extern __shared__ __attribute__((aligned(16))) Rank found[];
+    __shared__ Rank bound;
+    __shared__ int count;
+    const int t = threadIdx.x, wave = t / kWave, lane = t % kWave, r = blockIdx.x;
+    const Stats *its = stats + (long)r * pieces;
+    float mine = -INFINITY;
+    for (int i = t; i < pieces; i += kThreads) mine = fmaxf(mine, its[i].top);
+    mine = wave_max(mine);
+    if (lane == 0) tops[wave] = mine;
+    if (TOP && t == 0) count = 0;
+    __syncthreads();
+    const float top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
+    double sum = 0.0, mean = 0.0;
+    for (int i = t; i < pieces; i += kThreads) {
+        const Stats s = its[i];
+        // x - top = (x - s.top) + off: T moves by off Z
+        if (s.top == -INFINITY) {
+            sum += s.sum;  // 0, or NaN
+            continue;
+        }
+        const double off = (double)s.top - (double)top, by = exp(off);
+        sum += by * s.sum;
+        mean += by == 0.0 ? 0.0 : by * (s.mean + off * s.sum);
+    }
+    sum = wave_sum64(sum);
+    mean = wave_sum64(mean);
+    if (lane == 0) sums[wave][0] = sum, sums[wave][1] = mean;
+    __syncthreads();
+    sum = (sums[0][0] + sums[1][0]) + (sums[2][0] + sums[3][0]);
+    mean = (sums[0][1] + sums[1][1]) + (sums[2][1] + sums[3][1]);
+    if (top == -INFINITY) sum = NAN;
+    if (t == 0) finish(p, r, top, sum, mean);
+    if constexpr (TOP) {
+        const Rank *from = ranks + (long)r * pieces * p.top;
+        const int n = pieces * p.top;
+        Rank best = 0;
+        for (int i = t; i < n; i += kThreads) best = from[i] > best ? from[i] : best;
+        const Rank least = bound_of(best, p.top, all, &bound);
+        for (int i = t; i < n; i += kThreads) {
+            const Rank rank = from[i];
+            if (rank && rank >= least) found[atomicAdd(&count, 1)] = rank;
+        }
+        __syncthreads();
+        put_in_order(found, count, p.top, sorted);
+        __syncthreads();
+        if (t < p.top) finish_top(p, r, t, sorted[t], top, sum);
+    }
+}
+
+int values_of(int rows, int vocab) {
+    const long pieces = (vocab - 1) / (kThreads * kMany) + 1;
+    return pieces * rows >= kManyFrom ? kMany : kFew;
+}
+
+template <bool BF16, bool TOP, int N> int launch(const TokenLogprobs &p, hipStream_t stream) {
+    const int pieces = (p.vocab - 1) / (kThreads * N) + 1;
+    const size_t blocks = (size_t)pieces * p.rows;
+    Stats *stats = static_cast<Stats *>(p.workspace);
+    Rank *ranks = reinterpret_cast<Rank *>(stats + blocks);
+    logprobs_piece_kernel<BF16, TOP, N><<<(unsigned)blocks, kThreads, 0, stream>>>(p, pieces, stats, ranks);
+    if (hipGetLastError() != hipSuccess) return kErrLaunch;
+    if (pieces == 1) return kOk;
+    // ranks of the `top` threads that reach the bound
+    const size_t found = TOP ? sizeof(Rank) * p.top * (((size_t)pieces * p.top - 1) / kThreads + 1) : 0;
+    logprobs_join_kernel<TOP><<<p.rows, kThreads, found, stream>>>(p, pieces, stats, ranks);
+    return hipGetLastError() == hipSuccess ? kOk : kErrLaunch;
+}
+
+template <bool BF16, bool TOP> int launch(const TokenLogprobs &p, hipStream_t stream) {
+    return values_of(p.rows, p.vocab) == kMany ? launch<BF16, TOP, kMany>(p, stream) : launch<BF16, TOP, kFew>(p, stream);
+}
+
+}  // namespace
+
+size_t token_logprobs_workspace(int rows, int vocab, int top) {
+    const size_t pieces = (vocab - 1) / (kThreads * values_of(rows, vocab)) + 1;
+    return pieces == 1 ? 0 : pieces * rows * (sizeof(Stats) + sizeof(Rank) * top);
+}
+
+int token_logprobs(const TokenLogprobs &p, hipStream_t stream) {
+    if (p.bf16) return p.top ? launch<true, true>(p, stream) : launch<true, false>(p, stream);
+    return p.top ? launch<false, true>(p, stream) : launch<false, false>(p, stream);
+}
+
+}  // namespace mlh

@@ -11,7 +11,7 @@ import numpy as np
 HERE = os.path.dirname(os.path.abspath(__file__))
 LIBRARY_PATH = os.path.join(HERE, "lib", "libfloyd_amd.so")
 
-MLK_F32, MLK_Q8, MLK_Q4, MLK_BF16 = 0, 1, 2, 3
+MLK_F32, MLK_Q8, MLK_Q4, MLK_BF16, MLK_FP4 = 0, 1, 2, 3, 4
 
 _c = ctypes
 _vp = _c.c_void_p
@@ -63,6 +63,16 @@ SIGNATURES = {
                                   _c.c_int, _vp]),
     "mlk_matmul_fp8_grouped": (_c.c_int, [_c.c_int, _vp, _vp, _vp, _vp, _c.c_int, _vp, _c.c_int,
                                           _c.c_int, _c.c_int, _vp, _vp, _c.c_int]),
+    "mlk_latent_row_bytes": (_c.c_size_t, [_c.c_int, _c.c_int, _c.c_int]),
+    "mlk_latent_append": (_c.c_int, [_vp, _c.c_int, _vp, _c.c_long, _vp, _c.c_float, _vp,
+                                     _c.c_int, _vp, _c.c_long, _c.c_int, _c.c_int, _vp]),
+    "mlk_latent_gather": (_c.c_int, [_vp, _c.c_int, _c.c_int, _vp]),
+    "mlk_latent_attend_workspace": (_c.c_size_t, []),
+    "mlk_latent_attend": (_c.c_int, [_vp, _c.c_int, _vp, _vp, _c.c_int, _c.c_int, _c.c_float,
+                                     _vp, _c.c_size_t]),
+    "mlk_token_logprobs_workspace": (_c.c_size_t, [_c.c_int, _c.c_int, _c.c_int]),
+    "mlk_token_logprobs": (_c.c_int, [_c.c_int, _vp, _c.c_long, _c.c_int, _c.c_int, _vp, _vp,
+                                      _vp, _c.c_int, _vp, _vp, _vp, _c.c_size_t]),
     # include/fm_backend.h
     "fm_init": (_c.c_int, []),
     "fm_device_name": (_c.c_char_p, []),
@@ -276,3 +286,74 @@ def matmul_fp8_grouped(out_dtype, w, ws, x, xs, y, out_width, in_width, groups, 
                                         entries if x_rows is None else x_rows, _ptr(y),
                                         out_width, in_width, groups, _ptr(offsets),
                                         _ptr(row_ids), entries), "mlk_matmul_fp8_grouped")
+
+
+class LatentBatch(_c.Structure):
+    """A batch's sequences and the pages of their latent caches (MlkLatentBatch): cache_type
+    MLK_BF16 or MLK_FP4, `data` [pages, page_size] rows of latent_row_bytes(), tables [seqs,
+    table_width], lengths [seqs], row_starts [seqs + 1] or None (one row each).  The buffers
+    stay the caller's."""
+    _fields_ = [("type", _c.c_int), ("data", _vp), ("latent", _c.c_int), ("rope", _c.c_int),
+                ("pages", _c.c_int), ("page_size", _c.c_int), ("seqs", _c.c_int),
+                ("tables", _vp), ("table_width", _c.c_int), ("lengths", _vp),
+                ("row_starts", _vp)]
+
+    def __init__(self, cache_type, data, latent, rope, pages, page_size, seqs, tables,
+                 table_width, lengths, row_starts=None):
+        super().__init__(cache_type, _ptr(data), latent, rope, pages, page_size, seqs,
+                         _ptr(tables), table_width, _ptr(lengths), _ptr(row_starts))
+
+
+def latent_row_bytes(cache_type, latent, rope):
+    """Bytes of a cached row (mlk_latent_row_bytes)."""
+    n = load().mlk_latent_row_bytes(cache_type, latent, rope)
+    if n == 0:
+        raise NativeError(f"no latent rows of type {cache_type} and widths {latent}, {rope}")
+    return n
+
+
+def latent_append(batch, dtype, kv, rows, norm_w, inv_freq, eps=1e-5, stride=None, query=None,
+                  query_stride=None, heads=0, head_width=0, q=None):
+    """Norm, rotation and the place in the pages of the batch's new rows, and the rotation of
+    their queries (mlk_latent_append); strides default to dense rows."""
+    if stride is None:
+        stride = batch.latent + batch.rope
+    if query_stride is None:
+        query_stride = heads * head_width
+    check(load().mlk_latent_append(_c.byref(batch), dtype, _ptr(kv), stride, _ptr(norm_w), eps,
+                                   _ptr(inv_freq), rows, _ptr(query), query_stride, heads,
+                                   head_width, _ptr(q)), "mlk_latent_append")
+
+
+def latent_gather(batch, dtype, out, rows):
+    """Cached rows of the batch's token rows as values (mlk_latent_gather)."""
+    check(load().mlk_latent_gather(_c.byref(batch), dtype, rows, _ptr(out)), "mlk_latent_gather")
+
+
+def latent_attend_workspace():
+    return load().mlk_latent_attend_workspace()
+
+
+def latent_attend(batch, dtype, q, out, rows, heads, scale, workspace, workspace_bytes=None):
+    """Attention of the batch's token rows over their sequences' cached rows
+    (mlk_latent_attend); workspace_bytes defaults to a DeviceBuffer's own."""
+    if workspace_bytes is None:
+        workspace_bytes = workspace.nbytes
+    check(load().mlk_latent_attend(_c.byref(batch), dtype, _ptr(q), _ptr(out), rows, heads, scale,
+                                   _ptr(workspace), workspace_bytes), "mlk_latent_attend")
+
+
+def token_logprobs_workspace(rows, vocab, top=0):
+    return load().mlk_token_logprobs_workspace(rows, vocab, top)
+
+
+def token_logprobs(dtype, logits, rows, vocab, tokens, logprobs, workspace, workspace_bytes=None,
+                   stride=None, entropy=None, top=0, top_ids=None, top_logprobs=None):
+    """Log probabilities of the rows' tokens, entropies and the `top` most likely tokens
+    (mlk_token_logprobs); stride defaults to vocab, workspace_bytes to a DeviceBuffer's own."""
+    if workspace_bytes is None:
+        workspace_bytes = 0 if workspace is None else workspace.nbytes
+    check(load().mlk_token_logprobs(dtype, _ptr(logits), vocab if stride is None else stride, rows,
+                                    vocab, _ptr(tokens), _ptr(logprobs), _ptr(entropy), top,
+                                    _ptr(top_ids), _ptr(top_logprobs), _ptr(workspace),
+                                    workspace_bytes), "mlk_token_logprobs")

@@ -19,6 +19,7 @@
  *   mlk_quantize       quant_int8 / quant_int4 (tools/convert_moonlight.py:46-66)
  *   mlk_sample         choose_token (moonlight_chat.c:96-131), the caller-side
  *                      sampler, on device logits
+ * The fp8 and latent entry points and mlk_token_logprobs have no counterpart there.
  */
 #ifndef MOONLIGHT_KERNELS_H
 #define MOONLIGHT_KERNELS_H
@@ -31,8 +32,9 @@ extern "C" {
 #endif
 
 /* Weight formats of mlk_gemv; MLK_F32 and MLK_BF16 are also the types of the
- * values that the fp8 entry points take and return beside their codes. */
-enum { MLK_F32 = 0, MLK_Q8 = 1, MLK_Q4 = 2, MLK_BF16 = 3 };
+ * values that the fp8 and latent entry points take and return, MLK_BF16 and
+ * MLK_FP4 those of cached latent rows. */
+enum { MLK_F32 = 0, MLK_Q8 = 1, MLK_Q4 = 2, MLK_BF16 = 3, MLK_FP4 = 4 };
 
 /* ---- device plumbing (no counterpart in the reference: Metal used shared
  *      memory buffers, moonlight_metal.m:733-755) ---------------------------- */
@@ -184,6 +186,106 @@ int mlk_matmul_fp8_grouped(int out_type, const uint8_t *w, const float *ws,
                            void *y, int out_width, int in_width, int groups,
                            const int *offsets, const int *row_ids,
                            int entries);
+
+/* ---- latent caches of a batch of requests, in pages -----------------------
+ * No counterpart in the reference, which serves one request.  The compressed
+ * cache of one layer, for any number of sequences: a key is a latent row, which
+ * is its value too, and a rope row.  Keys are held in pages of page_size rows,
+ * and key j of sequence s is row j % page_size of page
+ * tables[s * table_width + j / page_size].  A row is
+ *   MLK_BF16  latent values, then rope values, all bf16;
+ *   MLK_FP4   latent / 2 bytes of e2m1 codes, 2j in the low half of byte j; 16
+ *             bytes of scales, that of values 32b .. 32b + 31 in byte
+ *             4 * (b % 4) + b / 4, a power of two e from -100 to 125 as e + 127
+ *             (the others are not used); then rope values, bf16.  A value is
+ *             code * 2^e, with codes sign * {0, 0.5, 1, 1.5, 2, 3, 4, 6}; scale
+ *             byte 255 makes its 32 values NaN.
+ * mlk_latent_row_bytes gives its length.
+ *
+ * The batch's token rows are dense: those of sequence s are row_starts[s] to
+ * row_starts[s + 1] (row s alone where row_starts is NULL), its newest ones: the
+ * last of them is key lengths[s] - 1, the one before it key lengths[s] - 2.  A row
+ * with a key below 0 (a length shorter than its rows, 0 for a slot that is not
+ * in use) is padding: it writes no key, sees none and reads as zeros.
+ *
+ * tables, lengths and row_starts are device memory, read when the work runs.
+ * Nothing out of range is read or written whatever they hold: a key whose page is
+ * outside [0, pages), or behind the table's last page, is not written and makes
+ * the rows that read it NaN; a sequence whose row_starts decrease or leave
+ * [0, rows] has no rows.  Rows of no sequence are left as they were.
+ *
+ * Limits: latent a multiple of 64 up to 512, rope a multiple of 16 up to 64;
+ * data 16-byte aligned, other pointers to their values.  Calls queue on the library
+ * stream and return, as the fp8 entry points do, with the same rules for
+ * pointers, other streams and overlap; they allocate nothing and keep nothing.
+ * A workspace is scratch for one call: calls from several threads need one each. */
+typedef struct {
+    int type;              /* of the latent values: MLK_BF16 or MLK_FP4 */
+    void *data;            /* [pages, page_size] rows */
+    int latent, rope;      /* values of a row */
+    int pages, page_size;
+    int seqs;
+    const int *tables;     /* [seqs, table_width] pages of each sequence */
+    int table_width;
+    const int *lengths;    /* [seqs] keys of each, the batch's rows included */
+    const int *row_starts; /* [seqs + 1], or NULL: one row each */
+} MlkLatentBatch;
+
+/* Bytes of a cached row; 0 for a type or widths that are not supported. */
+size_t mlk_latent_row_bytes(int type, int latent, int rope);
+
+/* Writes each token row's key: kv [rows, kv_stride] of `type` (MLK_F32 or
+ * MLK_BF16) holds latent values, of which RMSNorm(...) * norm_w is cached (the
+ * values themselves where norm_w is NULL), then rope values, rotated by the
+ * key's position p: with a = p * inv_freq[i] pair (2i, 2i + 1) becomes values i and
+ * i + rope / 2, x cos a - y sin a and y cos a + x sin a.  With `query` != NULL
+ * the last rope values of each head of query [rows, query_stride] (heads of
+ * head_width values) are rotated likewise into the last rope values of each head
+ * of q [rows, heads, latent + rope].  Strides are in values.
+ *
+ * Everything is computed in 64 bits and rounded once, to the nearest, ties to
+ * even; an fp4 scale is the least power of two, from 2^-100 on, with the largest
+ * magnitude at most 6 times it.  32 values with a NaN, an infinity or a magnitude
+ * of 2^127 and more among them get scale byte 255. */
+int mlk_latent_append(const MlkLatentBatch *batch, int type, const void *kv,
+                      long kv_stride, const float *norm_w, float eps,
+                      const float *inv_freq, int rows, const void *query,
+                      long query_stride, int heads, int head_width, void *q);
+
+/* out [rows, latent + rope] of `type`: the cached rows of the batch's token rows.
+ * (With row_starts the sums of the lengths, every key of every sequence.) */
+int mlk_latent_gather(const MlkLatentBatch *batch, int type, int rows, void *out);
+
+/* Attention in the absorbed form: for each head of each token row
+ *   out = sum_j p_j latent_j,  p = softmax_j(scale * q . [latent_j | rope_j])
+ * over the keys j up to the row's own.  q [rows, heads, latent + rope] and out
+ * [rows, heads, latent] are of `type`.  Scores, sums and results are f32; with
+ * MLK_BF16 the p of a key is rounded to bf16 before it is multiplied with its
+ * row (the softmax's sum is that of the rounded ones), with MLK_F32 nothing is.
+ * A NaN or an infinity in a key's row makes NaN of values of the rows that see it and of no
+ * others.  The workspace has at least mlk_latent_attend_workspace() bytes
+ * (device memory, 16-byte aligned). */
+size_t mlk_latent_attend_workspace(void);
+int mlk_latent_attend(const MlkLatentBatch *batch, int type, const void *q,
+                      void *out, int rows, int heads, float scale,
+                      void *workspace, size_t workspace_bytes);
+
+/* ---- log probabilities -----------------------------------------------------
+ * Of each row of logits (f32 or bf16, [rows, stride], the first vocab values of
+ * it): logprobs[r] = log softmax(row)[tokens[r]], NaN where tokens[r] is outside
+ * [0, vocab); entropy[r] (unless NULL) of the softmax in nats; top_ids and
+ * top_logprobs [rows, top] (top 0 .. 32, at most vocab) the most likely tokens,
+ * the lower index first among equal ones.  A logit of -inf has probability 0; a row
+ * with a NaN, +inf or nothing above -inf has NaN for every result but the ids
+ * (a NaN counts as the largest there).  Sums are 64 bits.  The workspace (device
+ * memory, 16-byte aligned) has at least mlk_token_logprobs_workspace() bytes; pointers,
+ * streams and overlap as for the latent entry points. */
+size_t mlk_token_logprobs_workspace(int rows, int vocab, int top);
+int mlk_token_logprobs(int type, const void *logits, long stride, int rows,
+                       int vocab, const int *tokens, float *logprobs,
+                       float *entropy, int top, int *top_ids,
+                       float *top_logprobs, void *workspace,
+                       size_t workspace_bytes);
 
 #ifdef __cplusplus
 }
