@@ -5,8 +5,9 @@
 //           rope part    k_i = x cos a - y sin a, k_(i + R/2) = y cos a + x sin a with
 //                        (x, y) = pair i, a = position * inv_freq[i]; queries likewise
 //
-// in 64 bits up to the one rounding: codes of 4 bits are a function of the inputs then,
-// whatever order a sum is formed in, and the angle of a far position keeps its bits.
+// in 64 bits: codes of 4 bits are a function of the inputs then, whatever order a sum is
+// formed in, and the angle of a far position keeps its bits.  Results are rounded to f32, bf16
+// ones from there.
 #include "bf16.h"
 #include "latent.h"
 #include "mlh_device.h"
@@ -27,7 +28,7 @@ template <bool BF16> __device__ __forceinline__ double value(typename Elem<BF16>
     else return (double)v;
 }
 template <bool BF16> __device__ __forceinline__ void store(typename Elem<BF16>::type *p, double v) {
-    if constexpr (BF16) *p = (uint16_t)bf16_bits(v);
+    if constexpr (BF16) *p = (uint16_t)bf16_bits((float)v);
     else *p = (float)v;
 }
 
@@ -143,13 +144,13 @@ __global__ __launch_bounds__(kThreads) void latent_append_kernel(MlkLatentBatch 
                 row[latent / 2 + 4 * (g % 4) + g / 4] = (uint8_t)(bad ? 255 : e + kFp4Bias);
         }
     } else if (has) {
-        reinterpret_cast<unsigned *>(row)[t] = bf16_bits(c0) | (bf16_bits(c1) << 16);
+        reinterpret_cast<unsigned *>(row)[t] = bf16_bits((float)c0) | (bf16_bits((float)c1) << 16);
     }
     if (t < half) {
         const double x = value<BF16>(kv[latent + 2 * t]), y = value<BF16>(kv[latent + 2 * t + 1]);
         uint16_t *rope = reinterpret_cast<uint16_t *>(row + latent_part_bytes(FP4, latent));
-        rope[t] = (uint16_t)bf16_bits(x * turn[t][0] - y * turn[t][1]);
-        rope[half + t] = (uint16_t)bf16_bits(y * turn[t][0] + x * turn[t][1]);
+        rope[t] = (uint16_t)bf16_bits((float)(x * turn[t][0] - y * turn[t][1]));
+        rope[half + t] = (uint16_t)bf16_bits((float)(y * turn[t][0] + x * turn[t][1]));
     }
 }
 

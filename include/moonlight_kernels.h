@@ -243,8 +243,8 @@ size_t mlk_latent_row_bytes(int type, int latent, int rope);
  * head_width values) are rotated likewise into the last rope values of each head
  * of q [rows, heads, latent + rope].  Strides are in values.
  *
- * Everything is computed in 64 bits and rounded once, to the nearest, ties to
- * even; an fp4 scale is the least power of two, from 2^-100 on, with the largest
+ * Everything is computed in 64 bits.  Codes are the nearest to that, f32 results
+ * too, bf16 results the nearest to the f32 one, ties to even; an fp4 scale is the least power of two, from 2^-100 on, with the largest
  * magnitude at most 6 times it.  32 values with a NaN, an infinity or a magnitude
  * of 2^127 and more among them get scale byte 255. */
 int mlk_latent_append(const MlkLatentBatch *batch, int type, const void *kv,

@@ -13,16 +13,9 @@ GUARD = 256
 
 
 def bf16_round(v):
-    """f64 -> bf16 bits, rounded once, ties to even."""
-    v = np.asarray(v, F64)
-    f = v.astype(F32)
-    with np.errstate(invalid="ignore"):
-        lossy = f.astype(F64) != v
-        u = f.view(np.uint32).astype(np.int64)
-        u = np.where(lossy & (np.abs(f.astype(F64)) > np.abs(v)), u - 1, u)
-        u = np.where(lossy, u | 1, u)
-    out = ((u + 0x7FFF + ((u >> 16) & 1)) >> 16) & 0xFFFF
-    return np.where(np.isnan(v), 0x7FC0, out).astype(np.uint16)
+    """f64 -> f32 -> bf16 bits, ties to even."""
+    with np.errstate(over="ignore"):
+        return U.to_bf16(np.where(np.isnan(v), np.nan, v).astype(F32))
 
 
 def fp4_nearest(a):
