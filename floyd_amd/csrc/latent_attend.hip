@@ -4,14 +4,13 @@
 //   s_j = scale * q . [latent_j | rope_j],  out = sum_j exp(s_j - m) latent_j / sum_j exp(s_j - m)
 //
 // for each (token row, head); a sequence's (row, head) pairs are taken 16 at a time
-// (a tile: the 16 columns of a matrix instruction), and a tile's keys a unit at a time,
-// 16 for each wave of a workgroup.  The units of all tiles, in order, are dealt out in
-// equal runs to as many workgroups as the chip holds, so ragged lengths leave none of them
-// idle; a tile whose units fell to several is joined by latent_join_kernel from their
-// partial sums.
+// (a tile: the 16 columns of a matrix instruction), and a tile's keys 16 at a time (a
+// unit; more where units could not be counted in 32 bits).  The units of all tiles, in order, are dealt out in equal runs to as many
+// workgroups as the chip holds, so ragged lengths leave none of them idle; a tile whose
+// units fell to several is joined by latent_join_kernel from their partial sums.
 //
-// Each wave takes 16 of a unit's keys, with a running maximum and sum of its own, and the
-// waves meet at the end of a tile.  The keys are read straight into the matrix operand
+// The waves of a workgroup take its units in turn, with a running maximum and sum of
+// their own, and meet at the end of a tile.  The keys are read straight into the matrix operand
 // (lane (k, g): 8 values of key k at a step), so the scores S[key][column] come from
 // v_mfma_f32_16x16x32_bf16; their registers hold 4 keys of a column, which is the operand
 // layout of the second product O[latent][column] += V^T P on v_mfma_f32_16x16x16_bf16.
@@ -19,6 +18,10 @@
 // the wave's own, written in rows and read transposed (ds_read_b64_tr_b16).  The next
 // keys are on their way from when the first product has taken the present ones, and the
 // page numbers of those after them.
+//
+// What runs once costs its instructions' way from memory, about 4 cycles a byte: loops are
+// entered a step early rather than with a copy of their loads before them, and unrolled
+// only where registers are counted.
 #include "bf16.h"
 #include "latent.h"
 #include "mlh_device.h"
@@ -34,7 +37,8 @@ typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef u32x4 u32x4_any __attribute__((aligned(2)));
 
 constexpr int kCols = 16;       // (row, head) pairs of a tile
-constexpr int kTileKeys = 16;   // keys of a wave's step
+constexpr int kStepKeys = 16, kStepShift = 4;  // keys of a wave's step
+constexpr int kLeastUnits = 4;  // that a workgroup takes, where there are as many
 constexpr int kSteps = kLatentMax / 32;          // product steps over a latent row
 constexpr int kRopeSteps = kLatentRopeMax / 32;  // and over a rope row
 constexpr int kAllSteps = kSteps + kRopeSteps;
@@ -50,28 +54,54 @@ template <bool BF16> constexpr int kAheadOf = BF16 ? 2 : 3;  // steps that queri
 // A wave's keys in LDS: rows 32 bytes apart from a multiple of the banks, so that neither
 // the rows of a transposed read nor those of a write share them.
 constexpr int kKeyStride = 2 * kLatentMax + 32;
-constexpr int kKeyBytes = kTileKeys * kKeyStride;
-// The waves' results in LDS, kJoinDims latent values of each column at a time.
+constexpr int kKeyBytes = kStepKeys * kKeyStride;
+// The waves' results in LDS, kJoinDims latent values of each column at a time, each wave's
+// where its keys were (the others may still read theirs).
 constexpr int kJoinDims = 256;
 constexpr int kJoinStride = kJoinDims + 4;
 static_assert(kCols * kJoinStride * 4 <= kKeyBytes, "the results fit where the keys were");
 constexpr int kQueryStride = kLatentMax + kLatentRopeMax + 8;
 template <bool BF16> constexpr int kQueryBytes = (BF16 ? 1 : 3) * kCols * kQueryStride * 2;
 
+// What latent_join_kernel has to know of a tile, told by the workgroup that ends it: its
+// sequence and number in it, and the workgroups that its units fell to (-1: to one, there is
+// nothing to join).  Where a batch has few tiles a record belongs to the tile: of sequence s,
+// the tile that begins with pair b of all (row, head) pairs has record b / 16 + s.  Those
+// are different, but not every record has a tile, and one that has none tells of an
+// earlier call's.  Else a record belongs to the workgroup, which ends at most one tile that
+// another one began.
+struct __attribute__((aligned(16))) Record {
+    int seq, tile, first, last;
+};
+constexpr int kMaxTileRecords = 2048;
+
 // Partial sums of tiles: slot 2w holds the tile that workgroup w found begun, slot 2w + 1
 // the one that it left unfinished.
 struct Parts {
     float *sums;    // [2 groups][kCols][kLatentMax]
     float *stats;   // [2 groups][2][kCols] maxima, then sums
-    int *records;   // [groups][kRecord]
+    Record *records;
+    int tiles;      // records of tiles, else 0: of workgroups
 };
-// Of a workgroup's first tile, if it was begun by another one and ends here: sequence,
-// tile, first workgroup; else -1.
-constexpr int kRecord = 4;
-
 constexpr size_t kSumsBytes = 2L * kMaxGroups * kCols * kLatentMax * 4;
 constexpr size_t kStatsBytes = 2L * kMaxGroups * 2 * kCols * 4;
-constexpr size_t kRecordBytes = (size_t)kMaxGroups * kRecord * 4;
+constexpr size_t kRecordBytes = (size_t)kMaxTileRecords * sizeof(Record);
+static_assert(kMaxGroups <= kMaxTileRecords, "records of workgroups");
+
+// n / d of n below 2^31 by a product: m is the whole number above 2^(31 + l) / d with l the
+// least for which 2^l >= d.
+struct Divisor {
+    unsigned m, shift;
+    __host__ static Divisor of(unsigned d) {
+        unsigned l = 0;
+        while ((1ull << l) < d) ++l;
+        return {(unsigned)((1ull << (31 + l)) / d + 1), l};
+    }
+    // ((2^32 / 2) / d would not fit for d = 1)
+    __device__ __forceinline__ unsigned quotient(unsigned n) const {
+        return shift ? __umulhi(n, m) >> (shift - 1) : n;
+    }
+};
 
 struct Params {
     MlkLatentBatch b;
@@ -80,6 +110,9 @@ struct Params {
     int rows, heads;
     float scale;  // times log2(e)
     int groups;
+    int keys;     // that a table can hold
+    int shift;    // a unit is kStepKeys << shift keys
+    Divisor page, head;
     Parts parts;
 };
 
@@ -89,100 +122,108 @@ struct Work {
     int keys;    // that its table can hold
     int per;     // units of a tile
     int tiles;
-    __device__ __forceinline__ long units() const { return (long)per * tiles; }
 };
 
-template <int UNIT> __device__ __forceinline__ Work work_of(const Params &p, int s) {
+__device__ __forceinline__ Work work_of(const Params &p, const LatentSeq &seq) {
     Work w;
-    w.seq = latent_seq(p.b, s, p.rows);
-    const long room = (long)p.b.table_width * p.b.page_size;
-    const int length = w.seq.length < 0 ? 0 : w.seq.length;
-    w.keys = length < room ? length : (int)room;
-    w.per = w.keys > UNIT ? (w.keys - 1) / UNIT + 1 : 1;
+    w.seq = seq;
+    const int length = seq.length < 0 ? 0 : seq.length;
+    w.keys = length < p.keys ? length : p.keys;
+    w.per = w.keys > 0 ? ((w.keys - 1) >> (kStepShift + p.shift)) + 1 : 1;
     // (rows * heads is below 2^31 - 15)
-    w.tiles = (int)(((unsigned)w.seq.count * (unsigned)p.heads + (kCols - 1)) / kCols);
+    w.tiles = (int)(((unsigned)seq.count * (unsigned)p.heads + (kCols - 1)) / kCols);
     return w;
 }
 
-// a / b, in 32 bits where both fit: a quarter of the instructions.
-__device__ __forceinline__ long quotient(long a, long b) {
-    if (((unsigned long)a | (unsigned long)b) >> 32) return a / b;
-    return (unsigned)a / (unsigned)b;
-}
-
-__device__ __forceinline__ long wave_sum_long(long v) {
+__device__ __forceinline__ int wave_sum_int(int v) {
 #pragma unroll
     for (int o = 32; o >= 1; o >>= 1) v += __shfl_xor(v, o, kWave);
+    return v;
+}
+
+// The sum of a value over this lane and those before it.
+__device__ __forceinline__ int wave_scan(int v) {
+    v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xF, 0xF, false);  // row_shr:1
+    v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xF, 0xF, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xF, 0xF, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xF, 0xF, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xA, 0xF, false);  // row_bcast:15
+    v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xC, 0xF, false);  // row_bcast:31
     return v;
 }
 
 // A workgroup's run of units: `length` of them from the one that is `offset` after the first
 // of sequence `seq`; `begin` is that one's place among all.
 struct Run {
-    int seq;
-    long offset, begin, length, total;
-    int groups;   // workgroups that have one: of `share` units, the first `rest` of one more
-    long share;
-    int rest;
-    __device__ __forceinline__ int owner(long unit) const {
-        const long longer = (share + 1) * rest;
-        return (int)(unit < longer ? quotient(unit, share + 1) : rest + quotient(unit - longer, share));
+    int seq, offset, begin, length;
+    int share, rest;  // workgroups have `share` units each, the first `rest` of them one more
+    // Of `total` units, dealt to no more workgroups than leaves each kLeastUnits: then no
+    // run between those of one tile is empty, and a tile has no more parts than pay.
+    __device__ __forceinline__ void deal(int total, int groups, int group) {
+        const int most = (total + kLeastUnits - 1) / kLeastUnits;
+        groups = most < groups ? most : groups;
+        offset = begin = length = share = seq = rest = 0;
+        if (group >= groups) return;
+        share = (int)((unsigned)total / (unsigned)groups);
+        rest = total - share * groups;
+        begin = share * group + (group < rest ? group : rest);
+        length = share + (group < rest ? 1 : 0);
+    }
+    __device__ __forceinline__ int owner(int unit) const {
+        const int longer = (share + 1) * rest;
+        return (int)(unit < longer ? (unsigned)unit / (unsigned)(share + 1)
+                                   : rest + (unsigned)(unit - longer) / (unsigned)share);
     }
 };
 
-template <int WAVES> __device__ __forceinline__ Run find_run(const Params &p, int group) {
-    constexpr int kThreads = WAVES * kWave, kUnit = WAVES * kTileKeys;
-    __shared__ long sums[WAVES];
-    __shared__ long at[2];
+// The sequences are in LDS (`held`) where a workgroup has a thread for each.
+template <int WAVES> __device__ __forceinline__ Run find_run(const Params &p, int group, LatentSeq *held) {
+    constexpr int kThreads = WAVES * kWave;
+    __shared__ int sums[WAVES], at[2];
     const int t = threadIdx.x, wave = t / kWave, lane = t % kWave;
-    const auto units_of = [&](int s) { return s < p.b.seqs ? work_of<kUnit>(p, s).units() : 0L; };
-    const long first_units = units_of(t);
-    long mine = first_units;
-    for (int s = t + kThreads; s < p.b.seqs; s += kThreads) mine += units_of(s);
-    mine = wave_sum_long(mine);
-    if (lane == 0) sums[wave] = mine;
-    __syncthreads();
+    const auto seq_of = [&](int s) { return s < p.b.seqs ? latent_seq(p.b, s, p.rows) : LatentSeq{0, 0, 0}; };
+    const auto units_of = [&](const LatentSeq &q) {
+        const Work w = work_of(p, q);
+        return w.per * w.tiles;
+    };
     Run r;
-    r.total = 0;
-#pragma unroll
-    for (int w = 0; w < WAVES; ++w) r.total += sums[w];
-    // (no workgroup's run is empty between those of a tile)
-    r.groups = r.total < p.groups ? (int)r.total : p.groups;
-    r.seq = 0;
-    r.offset = r.begin = r.length = r.share = 0;
-    r.rest = 0;
-    if (group >= r.groups) return r;
-    r.share = quotient(r.total, r.groups);
-    r.rest = (int)(r.total - r.share * r.groups);
-    r.begin = r.share * group + (group < r.rest ? group : r.rest);
-    r.length = r.share + (group < r.rest ? 1 : 0);
-    long before = 0;
-    for (int s0 = 0; s0 < p.b.seqs; s0 += kThreads) {
-        const long units = s0 == 0 ? first_units : units_of(s0 + t);
-        long upto = units;
-#pragma unroll
-        for (int o = 1; o < kWave; o <<= 1) {
-            const long below = __shfl_up(upto, o, kWave);
-            if (lane >= o) upto += below;
-        }
+    const LatentSeq mine = seq_of(t);
+    int units = units_of(mine), all = units, total = 0;
+    if (p.b.seqs <= kThreads) {
+        held[t] = mine;
+    } else {
+        for (int s = t + kThreads; s < p.b.seqs; s += kThreads) all += units_of(seq_of(s));
+        all = wave_sum_int(all);
+        if (lane == 0) sums[wave] = all;
+        __syncthreads();
+        for (int w = 0; w < WAVES; ++w) total += sums[w];
+        r.deal(total, p.groups, group);
+    }
+    int before = 0;
+    for (int s0 = 0;; s0 += kThreads) {
+        if (s0) units = units_of(seq_of(s0 + t));
+        const int upto = wave_scan(units);
         __syncthreads();
         if (lane == kWave - 1) sums[wave] = upto;
         __syncthreads();
-        long first = before + upto - units;
+        int first = before + upto - units;
 #pragma unroll
         for (int w = 0; w < WAVES; ++w) {
             if (w < wave) first += sums[w];
             before += sums[w];
         }
+        if (p.b.seqs <= kThreads) r.deal(before, p.groups, group);
         if (r.begin >= first && r.begin < first + units) {
             at[0] = s0 + t;
             at[1] = r.begin - first;
         }
-        if (r.begin < before) break;
+        if (r.begin < before || s0 + kThreads >= p.b.seqs) break;
     }
     __syncthreads();
-    r.seq = (int)at[0];
-    r.offset = at[1];
+    if (r.length > 0) {
+        r.seq = at[0];
+        r.offset = at[1];
+    }
     return r;
 }
 
@@ -301,80 +342,96 @@ constexpr float kSlack = 8.0f;
 
 template <bool FP4, bool BF16, bool FULL>
 __global__ __launch_bounds__(kWavesOf<BF16> *kWave, 1) void latent_attend_kernel(Params p) {
-    constexpr int kWaves = kWavesOf<BF16>, kThreads = kWaves * kWave, kUnit = kWaves * kTileKeys;
+    constexpr int kWaves = kWavesOf<BF16>, kThreads = kWaves * kWave;
     constexpr int kParts = BF16 ? 1 : 3;  // bf16 parts of a query value and of a probability
     extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
-    __shared__ float tops[kWaves][kCols], sums[kWaves][kCols];
+    __shared__ __attribute__((aligned(16))) float tops[kCols][kWaves], sums[kCols][kWaves];
+    __shared__ LatentSeq held[kThreads];
     const int t = threadIdx.x, wave = t / kWave, lane = t % kWave;
     const int g = lane / 16, c = lane % 16;
     const int latent = FULL ? kLatentMax : p.b.latent, rope = FULL ? kLatentRopeMax : p.b.rope;
     const int width = latent + rope, dims = latent / 16;
     const int row_bytes = latent_row_bytes(FP4, latent, rope);
-    const uint8_t *data = static_cast<const uint8_t *>(p.b.data);
     uint8_t *keys_lds = lds + wave * kKeyBytes;
     uint16_t *query_lds = reinterpret_cast<uint16_t *>(lds + kWaves * kKeyBytes);
 
     const int group = blockIdx.x;
-    const Run run = find_run<kWaves>(p, group);
-    int *record = p.parts.records + kRecord * group;
-    if (t == 0) record[0] = -1;
-    long left = run.length, offset = run.offset;
+    const Run run = find_run<kWaves>(p, group, held);
+    if (t == 0 && !p.parts.tiles) p.parts.records[group].first = -1;
+    int left = run.length, offset = run.offset;
     for (int s = run.seq; left > 0 && s < p.b.seqs; ++s, offset = 0) {
-        const Work w = work_of<kUnit>(p, s);
-        while (left > 0 && offset < w.units()) {
-            const int tile = (int)quotient(offset, w.per), from = (int)(offset - (long)tile * w.per);
-            const int upto = left < w.per - from ? from + (int)left : w.per;
-            left -= upto - from;
-            offset += upto - from;
+        const Work w = work_of(p, p.b.seqs <= kThreads ? held[s] : latent_seq(p.b, s, p.rows));
+        while (left > 0 && offset < w.per * w.tiles) {
+            const int tile = (int)((unsigned)offset / (unsigned)w.per), first = offset - tile * w.per;
+            const int last = left < w.per - first ? first + left : w.per;
+            left -= last - first;
+            offset += last - first;
 
             // the tile's columns, and the keys that they see, as far as the table goes
-            const unsigned pair0 = (unsigned)tile * kCols, pairs = (unsigned)w.seq.count * (unsigned)p.heads;
-            const int used = pairs - pair0 < kCols ? (int)(pairs - pair0) : kCols;
+            const int pair0 = tile * kCols, pairs = w.seq.count * p.heads;
+            const int used = pairs - pair0 < kCols ? pairs - pair0 : kCols;
             const long base = (long)w.seq.begin * p.heads + pair0;  // among all (row, head) pairs
-            const long sees = (long)w.seq.length - w.seq.count + 1 + (pair0 + (c < used ? c : 0)) / (unsigned)p.heads;
+            // (the row's own key, and those before it; 32 bits: both are below 2^31)
+            const long sees = (long)w.seq.length - w.seq.count + 1 +
+                              (int)p.head.quotient((unsigned)(pair0 + (c < used ? c : 0)));
             const int within = sees < 0 ? 0 : sees < w.keys ? (int)sees : w.keys;
             const int limit = c < used ? within : 0;
             const int least = __builtin_amdgcn_readlane(within, 0);
             const int most = __builtin_amdgcn_readlane(within, used - 1);
+            // in steps of 16 keys
+            const int from = first << p.shift, seen_steps = (most + kStepKeys - 1) >> kStepShift;
+            const int upto = (last << p.shift) < seen_steps ? last << p.shift : seen_steps;
 
-            // the wave's first keys, and the pages of its second ones
-            const auto key_of = [&](int unit) { return unit * kUnit + wave * kTileKeys + c; };
-            const auto slot_of = [&](int unit) {
-                const int j = key_of(unit);
-                return unit < upto && j < most ? latent_slot(p.b, s, (unsigned)j) : 0L;
+            // A key's page, loaded a step before the key; keys that nothing sees are taken from
+            // page 0 (and out of the products).
+            const int *table = p.b.tables + (long)s * p.b.table_width;
+            const auto page_of = [&](int step, unsigned *in_page) {
+                const unsigned j = (unsigned)step * kStepKeys + c, at = p.page.quotient(j);
+                *in_page = j - at * (unsigned)p.b.page_size;
+                int page = 0;
+                if (step < upto && j < (unsigned)most) page = table[at];
+                return page;
             };
-            long slot = slot_of(from);
-            Raw<FP4> raw;
-            load_key<FP4, FULL>(raw, data + (slot < 0 ? 0 : slot) * row_bytes, g, latent, rope);
-            long next_slot = slot_of(from + 1);
+            unsigned in_page = 0, next_in_page;
+            int page = 0, next_page = page_of(from + wave, &next_in_page);
 
-            // the queries, 8 values a thread and pass, into LDS
-            __syncthreads();  // (the tile before is done with it)
-#pragma unroll 1
-            for (int i = t; i < kCols * (kLatentMax + kLatentRopeMax) / 8; i += kThreads) {
-                constexpr int kPieces = (kLatentMax + kLatentRopeMax) / 8;
-                const int col = i / kPieces, d = 8 * (i % kPieces);
+            // the queries into LDS, 8 values a thread and pass
+            constexpr int kPieces = (kLatentMax + kLatentRopeMax) / 8;
+            constexpr int kLoads = (kCols * kPieces + kThreads - 1) / kThreads;
+            u32x4 pieces[kLoads][BF16 ? 1 : 2];
+#pragma unroll
+            for (int y = 0; y < kLoads; ++y) {
+                const int i = t + y * kThreads, col = i / kPieces, d = 8 * (i % kPieces);
                 const bool in = col < used && (FULL || (d < kLatentMax ? d < latent : d - kLatentMax < rope));
-                const long at = (base + (in ? col : 0)) * width + (!in ? 0 : d < kLatentMax ? d : latent + d - kLatentMax);
+                const long at = (base + col) * width + (FULL || d < kLatentMax ? d : latent + d - kLatentMax);
+#pragma unroll
+                for (int h = 0; h < (BF16 ? 1 : 2); ++h) {
+                    pieces[y][h] = u32x4{0, 0, 0, 0};
+                    if (!in) continue;
+                    if constexpr (BF16) pieces[y][h] = *reinterpret_cast<const u32x4_any *>(static_cast<const uint16_t *>(p.q) + at);
+                    else __builtin_memcpy(&pieces[y][h], static_cast<const float *>(p.q) + at + 4 * h, 16);
+                }
+            }
+            __syncthreads();  // (the tile before is done with them)
+#pragma unroll
+            for (int y = 0; y < kLoads; ++y) {
+                const int i = t + y * kThreads, col = i / kPieces, d = 8 * (i % kPieces);
+                if (kCols * kPieces % kThreads && i >= kCols * kPieces) break;
+                uint16_t *to = query_lds + col * kQueryStride + d;
                 if constexpr (BF16) {
-                    u32x4 v = *reinterpret_cast<const u32x4_any *>(static_cast<const uint16_t *>(p.q) + at);
-                    if (!in) v = u32x4{0, 0, 0, 0};
-                    *reinterpret_cast<u32x4 *>(query_lds + col * kQueryStride + d) = v;
+                    *reinterpret_cast<u32x4 *>(to) = pieces[y][0];
                 } else {
-                    float x[8];
-                    __builtin_memcpy(x, static_cast<const float *>(p.q) + at, sizeof(x));
                     u32x4 v[3];
 #pragma unroll
                     for (int k = 0; k < 4; ++k) {
                         unsigned lo[3], hi[3];
-                        split3(in ? x[2 * k] : 0.0f, lo);
-                        split3(in ? x[2 * k + 1] : 0.0f, hi);
+                        split3(__uint_as_float(pieces[y][k / 2][2 * (k % 2)]), lo);
+                        split3(__uint_as_float(pieces[y][k / 2][2 * (k % 2) + 1]), hi);
 #pragma unroll
-                        for (int y = 0; y < 3; ++y) v[y][k] = lo[y] | hi[y] << 16;
+                        for (int x = 0; x < 3; ++x) v[x][k] = lo[x] | hi[x] << 16;
                     }
 #pragma unroll
-                    for (int y = 0; y < 3; ++y)
-                        *reinterpret_cast<u32x4 *>(query_lds + (y * kCols + col) * kQueryStride + d) = v[y];
+                    for (int x = 0; x < 3; ++x) *reinterpret_cast<u32x4 *>(to + x * kCols * kQueryStride) = v[x];
                 }
             }
             __syncthreads();
@@ -386,54 +443,65 @@ __global__ __launch_bounds__(kWavesOf<BF16> *kWave, 1) void latent_attend_kernel
 #pragma unroll
             for (int d = 0; d < kDims; ++d) out[d] = f32x4{0.f, 0.f, 0.f, 0.f};
 
-            for (int unit = from; unit < upto; ++unit) {
-                const int key0 = unit * kUnit + wave * kTileKeys;
-                if (key0 >= most) break;
-                unsigned bad = (unsigned)__ballot(slot < 0) & 0xFFFFu;  // keys without a place
+            Raw<FP4> raw;
+            for (int step = from + wave - kWaves;; step += kWaves) {
+                const bool live = step >= from && step < upto;
+                const int key0 = step * kStepKeys;
                 f32x4 score[kParts];
 #pragma unroll
                 for (int k = 0; k < kParts; ++k) score[k] = f32x4{0.f, 0.f, 0.f, 0.f};
-                // (queries come from LDS a few steps ahead of their product, and no more:
-                // registers are what limits a wave here)
-                constexpr int kAhead = kAheadOf<BF16>;
-                u32x4 ahead[2][kAhead][kParts];
-                const auto fetch = [&](int j0) {
+                if (live) {
+                    // (queries come from LDS a few steps ahead of their product, and no more:
+                    // registers are what limits a wave here)
+                    constexpr int kAhead = kAheadOf<BF16>;
+                    u32x4 ahead[2][kAhead][kParts];
+                    const auto fetch = [&](int j0) {
 #pragma unroll
-                    for (int x = 0; x < kAhead; ++x) {
-                        const int j = j0 + x;
-                        const int at = j < kSteps ? dim_of<FP4>(j, g) : kLatentMax + 32 * (j - kSteps) + 8 * g;
+                        for (int x = 0; x < kAhead; ++x) {
+                            const int j = j0 + x;
+                            const int at = j < kSteps ? dim_of<FP4>(j, g) : kLatentMax + 32 * (j - kSteps) + 8 * g;
 #pragma unroll
-                        for (int k = 0; k < kParts; ++k)
-                            ahead[j0 / kAhead % 2][x][k] =
-                                *reinterpret_cast<const u32x4 *>(query_lds + (k * kCols + c) * kQueryStride + at);
+                            for (int k = 0; k < kParts; ++k)
+                                ahead[j0 / kAhead % 2][x][k] =
+                                    *reinterpret_cast<const u32x4 *>(query_lds + (k * kCols + c) * kQueryStride + at);
+                        }
+                    };
+                    fetch(0);
+#pragma unroll
+                    for (int j0 = 0; j0 < kAllSteps; j0 += kAhead) {
+                        __builtin_amdgcn_sched_barrier(0);
+                        if (j0 + kAhead < kAllSteps) fetch(j0 + kAhead);
+#pragma unroll
+                        for (int x = 0; x < kAhead; ++x) {
+                            const int j = j0 + x;
+                            const u32x4 v = operand<FP4, FULL>(raw, j, g, latent);
+                            if (j < kSteps)
+                                *reinterpret_cast<u32x4 *>(keys_lds + c * kKeyStride + 2 * dim_of<FP4>(j, g)) = v;
+#pragma unroll
+                            for (int k = 0; k < kParts; ++k)
+                                score[k] = mfma32(v, ahead[j0 / kAhead % 2][x][k], score[k]);
+                        }
                     }
-                };
-                fetch(0);
-#pragma unroll
-                for (int j0 = 0; j0 < kAllSteps; j0 += kAhead) {
                     __builtin_amdgcn_sched_barrier(0);
-                    if (j0 + kAhead < kAllSteps) fetch(j0 + kAhead);
-#pragma unroll
-                    for (int x = 0; x < kAhead; ++x) {
-                        const int j = j0 + x;
-                        const u32x4 v = operand<FP4, FULL>(raw, j, g, latent);
-                        if (j < kSteps)
-                            *reinterpret_cast<u32x4 *>(keys_lds + c * kKeyStride + 2 * dim_of<FP4>(j, g)) = v;
-#pragma unroll
-                        for (int k = 0; k < kParts; ++k) score[k] = mfma32(v, ahead[j0 / kAhead % 2][x][k], score[k]);
-                    }
                 }
-                __builtin_amdgcn_sched_barrier(0);
-                slot = next_slot;
-                if (unit + 1 < upto)
-                    load_key<FP4, FULL>(raw, data + (slot < 0 ? 0 : slot) * row_bytes, g, latent, rope);
-                next_slot = slot_of(unit + 2);
+                // the page of the step after the next, then the next step's keys
+                const unsigned bad_pages = (unsigned)__ballot((unsigned)page >= (unsigned)p.b.pages) & 0xFFFFu;
+                page = next_page;
+                in_page = next_in_page;
+                next_page = page_of(step + 2 * kWaves, &next_in_page);
+                if (step + kWaves < upto) {
+                    const long slot = (unsigned)page < (unsigned)p.b.pages ? (long)page * p.b.page_size + in_page : 0;
+                    load_key<FP4, FULL>(raw, static_cast<const uint8_t *>(p.b.data) + slot * row_bytes, g, latent, rope);
+                }
+                if (!live) {
+                    if (step < from) continue;
+                    break;
+                }
                 f32x4 sc = score[0];
                 if constexpr (!BF16) sc += score[1] + score[2];
 
-                const bool edge = bad || key0 + kTileKeys > least;
                 bool hidden[4] = {false, false, false, false};
-                if (edge) {
+                if (bad_pages || key0 + kStepKeys > least) {
                     // Keys that not every column sees, or that have no place: those that a
                     // column does not see must not reach it by 0 * NaN either, so rows that
                     // are not finite (or not there) are taken out of the second product and
@@ -444,7 +512,7 @@ __global__ __launch_bounds__(kWavesOf<BF16> *kWave, 1) void latent_attend_kernel
                     for (int j = 0; j < kSteps; ++j)
                         odd |= not_finite(*reinterpret_cast<const u32x4 *>(keys_lds + c * kKeyStride + 2 * dim_of<FP4>(j, g)));
                     const unsigned long long which = __ballot(odd && there);
-                    bad |= (unsigned)(which | which >> 16 | which >> 32 | which >> 48) & 0xFFFFu;
+                    const unsigned bad = bad_pages | ((unsigned)(which | which >> 16 | which >> 32 | which >> 48) & 0xFFFFu);
                     if (!there || (bad >> c & 1u)) {
 #pragma unroll 1
                         for (int j = 0; j < kSteps; ++j)
@@ -458,17 +526,17 @@ __global__ __launch_bounds__(kWavesOf<BF16> *kWave, 1) void latent_attend_kernel
                 }
                 float high = -INFINITY;
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const float x = hidden[i] ? -INFINITY : sc[i] * p.scale;
-                    high = fmaxf(high, x);
-                }
+                for (int i = 0; i < 4; ++i) high = fmaxf(high, hidden[i] ? -INFINITY : sc[i] * p.scale);
                 if (__any(high > top + kSlack)) {
                     const float next = fmaxf(top, groups_max(high));
                     const float by = top == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(top - next);
+                    const bool begun = __any(top != -INFINITY);  // (else there is nothing yet, or NaN)
                     sum *= by;
                     top = next;
+                    if (begun) {
 #pragma unroll
-                    for (int d = 0; d < kDims; ++d) out[d] *= by;
+                        for (int d = 0; d < kDims; ++d) out[d] *= by;
+                    }
                 }
                 const float to = top == -INFINITY ? 0.0f : top;
                 s16x4 probs[kParts];
@@ -526,111 +594,145 @@ __global__ __launch_bounds__(kWavesOf<BF16> *kWave, 1) void latent_attend_kernel
             sum += __shfl_xor(sum, 16, kWave);
             sum += __shfl_xor(sum, 32, kWave);
             if (g == 0) {
-                tops[wave][c] = top;
-                sums[wave][c] = sum;
+                tops[c][wave] = top;
+                sums[c][wave] = sum;
             }
-            __syncthreads();
-            float all = tops[0][c];
-#pragma unroll
-            for (int k = 1; k < kWaves; ++k) all = fmaxf(all, tops[k][c]);
-            const float by = top == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(top - all);
-            const bool whole = from == 0 && upto == w.per;
-            const int part = 2 * group + (from == 0 ? 1 : 0);
+            const int busy = upto - from < kWaves ? upto - from : kWaves;  // waves that had a step
+            const bool whole = first == 0 && last == w.per;
+            const int part = 2 * group + (first == 0 ? 1 : 0);
             // a thread's column of the results, 4 values at a time
-            constexpr int kColThreads = kThreads / kCols;
-            const int col = t / kColThreads;
-            float col_top = tops[0][col], col_sum = 0.0f;
-#pragma unroll
-            for (int k = 1; k < kWaves; ++k) col_top = fmaxf(col_top, tops[k][col]);
-#pragma unroll
-            for (int k = 0; k < kWaves; ++k)
-                col_sum += sums[k][col] * (tops[k][col] == -INFINITY
-                                               ? 0.0f  // (times 0, or NaN where a column is)
-                                               : __builtin_amdgcn_exp2f(tops[k][col] - col_top));
-            const float over = col_top == -INFINITY && !(col_sum != col_sum) ? 0.0f : 1.0f / col_sum;
+            constexpr int kColThreads = kThreads / kCols, kPasses = kJoinDims / (4 * kColThreads);
+            const int col = t / kColThreads, at = 4 * (t % kColThreads);
+            float col_top = -INFINITY, col_sum = 0.0f, by[kWaves], over = 0.0f;
             float *results = reinterpret_cast<float *>(lds);
 #pragma unroll
             for (int round = 0; round < kLatentMax / kJoinDims; ++round) {
                 if (!FULL && round * kJoinDims >= latent) break;
                 if (round) __syncthreads();
+                if (wave < busy) {
 #pragma unroll
-                for (int d = 0; d < kJoinDims / 16; ++d)
-                    *reinterpret_cast<f32x4 *>(results + (wave * kCols + c) * kJoinStride + 16 * d + 4 * g) =
-                        out[round * (kJoinDims / 16) + d] * by;
+                    for (int d = 0; d < kJoinDims / 16; ++d)
+                        *reinterpret_cast<f32x4 *>(results + wave * (kKeyBytes / 4) + c * kJoinStride + 16 * d + 4 * g) =
+                            out[round * (kJoinDims / 16) + d];
+                }
                 __syncthreads();
+                if (round == 0) {
 #pragma unroll
-                for (int k = 0; k < kJoinDims / (4 * kColThreads); ++k) {
-                    const int at = 4 * (t % kColThreads) + 4 * kColThreads * k, d = round * kJoinDims + at;
+                    for (int x = 0; x < kWaves; ++x) col_top = fmaxf(col_top, tops[col][x]);
+#pragma unroll
+                    for (int x = 0; x < kWaves; ++x) {
+                        by[x] = __builtin_amdgcn_exp2f(tops[col][x] - (col_top == -INFINITY ? 0.0f : col_top));
+                        col_sum += by[x] * sums[col][x];
+                    }
+                    over = whole ? col_sum == 0.0f ? 0.0f : 1.0f / col_sum : 1.0f;
+                }
+                f32x4 v[kPasses];
+#pragma unroll
+                for (int k = 0; k < kPasses; ++k) v[k] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int x = 0; x < kWaves; ++x) {
+                    if (x >= busy) break;
+#pragma unroll
+                    for (int k = 0; k < kPasses; ++k)
+                        v[k] += by[x] * load_f4(results + x * (kKeyBytes / 4) + col * kJoinStride + at + 4 * kColThreads * k);
+                }
+#pragma unroll
+                for (int k = 0; k < kPasses; ++k) {
+                    const int d = round * kJoinDims + at + 4 * kColThreads * k;
                     if (!FULL && d >= latent) break;
-                    f32x4 v = load_f4(results + col * kJoinStride + at);
-#pragma unroll
-                    for (int x = 1; x < kWaves; ++x) v += load_f4(results + (x * kCols + col) * kJoinStride + at);
                     if (!whole)
-                        *reinterpret_cast<f32x4 *>(p.parts.sums + ((long)part * kCols + col) * kLatentMax + d) = v;
+                        *reinterpret_cast<f32x4 *>(p.parts.sums + (part * kCols + col) * kLatentMax + d) = v[k];
                     else if (col < used)
-                        store4<BF16>(p.out, (base + col) * latent + d, v * over);
+                        store4<BF16>(p.out, (base + col) * latent + d, v[k] * over);
                 }
             }
             if (!whole && t % kColThreads == 0) {
-                p.parts.stats[(long)part * 2 * kCols + col] = col_top;
-                p.parts.stats[((long)part * 2 + 1) * kCols + col] = col_sum;
+                p.parts.stats[part * 2 * kCols + col] = col_top;
+                p.parts.stats[(part * 2 + 1) * kCols + col] = col_sum;
             }
-            if (t == 0 && from > 0 && upto == w.per) {
-                // the workgroup whose run holds the tile's first unit
-                record[1] = tile;
-                record[2] = run.owner(run.begin - from);
-                record[0] = s;
+            if (t == 0 && last == w.per && (first > 0 || p.parts.tiles)) {
+                // (owner: of the tile's first unit)
+                const Record record = {s, tile, first > 0 ? run.owner(run.begin - first) : -1, group};
+                p.parts.records[p.parts.tiles ? (int)(base / kCols) + s : group] = record;
             }
-            __syncthreads();
         }
     }
 }
 
-// Joins the tile that workgroup blockIdx.x finished but did not begin: its sums are in part
-// 2 first + 1 and in parts 2w of the workgroups w after the first.  A workgroup of this
-// launch takes kJoinCols columns, 128 threads each.
-constexpr int kJoinCols = 2, kColThreads = kLatentMax / 4;
-template <bool BF16> __global__ __launch_bounds__(kJoinCols *kColThreads) void latent_join_kernel(Params p) {
-    __shared__ float weights[kJoinCols][kMaxGroups];
-    __shared__ float reds[kJoinCols][2][kColThreads / kWave];
-    const int group = blockIdx.x, x = threadIdx.x / kColThreads, t = threadIdx.x % kColThreads;
-    const int col = blockIdx.y * kJoinCols + x;
-    const int *record = p.parts.records + kRecord * group;
-    const int s = record[0], tile = record[1], first = record[2];
-    if (s < 0) return;
+// Joins the tile of record blockIdx.x: its sums are in part 2 first + 1 and in parts 2w of
+// the workgroups w after the first.  128 threads take a column's values, and blockDim.x /
+// 128 such teams share its parts: a round of loads from what other workgroups wrote takes
+// about a microsecond, so as many as can are under way at once.
+constexpr int kTeam = kLatentMax / 4;
+constexpr int kJoinLoads = 16;  // parts that a thread has on their way
+constexpr int kMaxTeams = 4;
+template <bool BF16> __global__ __launch_bounds__(kTeam *kMaxTeams) void latent_join_kernel(Params p) {
+    __shared__ float tops[2 * kMaxGroups], sums[2 * kMaxGroups];
+    __shared__ float reds[2][kTeam * kMaxTeams / kWave];
+    __shared__ f32x4 shares[kMaxTeams - 1][kTeam];
+    const Record record = p.parts.records[blockIdx.x];
+    if (record.first < 0) return;
+    const int col = blockIdx.y, team = threadIdx.x / kTeam, t = threadIdx.x % kTeam, teams = blockDim.x / kTeam;
+    // (a record without a tile holds anything)
+    const int first = record.first < p.groups ? record.first : 0;
+    const int last = record.last < first ? first : record.last < p.groups ? record.last : p.groups - 1;
+    const int count = last - first + 1;
+    const auto part_of = [&](int i) { return 2 * (first + i) + (i == 0 ? 1 : 0); };
+    const int s = (unsigned)record.seq < (unsigned)p.b.seqs ? record.seq : 0;
     const LatentSeq seq = latent_seq(p.b, s, p.rows);
-    const int count = group - first + 1;
-    const auto part_of = [&](int i) { return i == 0 ? 2L * first + 1 : 2L * (first + i); };
-    float top = -INFINITY;
-    for (int i = t; i < count; i += kColThreads) {
-        const float its = p.parts.stats[part_of(i) * 2 * kCols + col];
-        weights[x][i] = its;
-        top = fmaxf(top, its);
+    const int pairs = seq.count * p.heads, pair = record.tile * kCols + col;
+    const long base = (long)seq.begin * p.heads;
+    const float *from = p.parts.sums + col * kLatentMax + 4 * t;
+    float top = -INFINITY, sum = 0.0f;
+    f32x4 v[kJoinLoads], result = {0.f, 0.f, 0.f, 0.f};
+    // (entered a step early, for the loads; parts i0 + team + k teams)
+    const int stride = kJoinLoads * teams;
+    for (int i0 = team - stride; i0 < count; i0 += stride) {
+        if (i0 >= 0) {
+#pragma unroll
+            for (int k = 0; k < kJoinLoads; ++k)
+                if (i0 + k * teams < count) result += tops[i0 + k * teams] * v[k];
+        }
+#pragma unroll
+        for (int k = 0; k < kJoinLoads; ++k) {
+            const int i = i0 + stride + k * teams;
+            v[k] = load_f4(from + part_of(i < count ? i : count - 1) * (kCols * kLatentMax));
+        }
+        if (i0 >= 0) continue;
+        // (what a record without a tile says of one is not true)
+        if (p.parts.tiles && ((unsigned)record.tile > (unsigned)pairs / kCols ||
+                              (int)((base + record.tile * kCols) / kCols) + s != (int)blockIdx.x))
+            return;
+        for (int i = threadIdx.x; i < count; i += blockDim.x) {
+            const float *stats = p.parts.stats + part_of(i) * (2 * kCols) + col;
+            tops[i] = stats[0];
+            sums[i] = stats[kCols];
+            top = fmaxf(top, stats[0]);
+        }
+        top = dpp_wave_max(top);
+        if (threadIdx.x % kWave == 0) reds[0][threadIdx.x / kWave] = top;
+        __syncthreads();
+        for (int k = 0; k < teams * kTeam / kWave; ++k) top = fmaxf(top, reds[0][k]);
+        if (top == -INFINITY) top = 0.0f;
+        for (int i = threadIdx.x; i < count; i += blockDim.x) {
+            const float by = __builtin_amdgcn_exp2f(tops[i] - top);
+            tops[i] = by;
+            sum += by * sums[i];
+        }
+        sum = dpp_wave_sum(sum);
+        if (threadIdx.x % kWave == 0) reds[1][threadIdx.x / kWave] = sum;
+        __syncthreads();
+        sum = 0.0f;
+        for (int k = 0; k < teams * kTeam / kWave; ++k) sum += reds[1][k];
     }
-    top = wave_max(top);
-    if (t % kWave == 0) reds[x][0][t / kWave] = top;
-    __syncthreads();
-    top = fmaxf(reds[x][0][0], reds[x][0][1]);
-    float sum = 0.0f;
-    for (int i = t; i < count; i += kColThreads) {
-        const float its = weights[x][i];
-        const float by = its == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(its - top);
-        sum += by * p.parts.stats[(part_of(i) * 2 + 1) * kCols + col];
-        weights[x][i] = by;
+    if (teams > 1) {
+        if (team) shares[team - 1][t] = result;
+        __syncthreads();
+        if (team) return;
+        for (int k = 1; k < teams; ++k) result += shares[k - 1][t];
     }
-    sum = wave_sum(sum);
-    if (t % kWave == 0) reds[x][1][t / kWave] = sum;
-    __syncthreads();
-    sum = reds[x][1][0] + reds[x][1][1];
-    const unsigned pair = (unsigned)tile * kCols + col;
-    if (pair >= (unsigned)seq.count * (unsigned)p.heads || 4 * t >= p.b.latent) return;
-    const float *from = p.parts.sums + (long)col * kLatentMax + 4 * t;
-    f32x4 v = weights[x][0] * load_f4(from + part_of(0) * kCols * kLatentMax);
-    from += part_of(1) * kCols * kLatentMax;
-#pragma unroll 8
-    for (int i = 1; i < count; ++i) v += weights[x][i] * load_f4(from + (long)(i - 1) * 2 * kCols * kLatentMax);
-    v *= top == -INFINITY && !(sum != sum) ? 0.0f : 1.0f / sum;
-    store4<BF16>(p.out, ((long)seq.begin * p.heads + pair) * p.b.latent + 4 * t, v);
+    if (pair >= pairs || 4 * t >= p.b.latent) return;
+    store4<BF16>(p.out, (base + pair) * p.b.latent + 4 * t, result * (sum == 0.0f ? 0.0f : 1.0f / sum));
 }
 
 template <bool FP4, bool BF16, bool FULL> int launch(const Params &p, hipStream_t stream) {
@@ -643,7 +745,10 @@ template <bool FP4, bool BF16, bool FULL> int launch(const Params &p, hipStream_
     kernel<<<p.groups, threads, bytes, stream>>>(p);
     if (hipGetLastError() != hipSuccess) return kErrLaunch;
     if (p.groups == 1) return kOk;
-    latent_join_kernel<BF16><<<dim3(p.groups, kCols / kJoinCols), kJoinCols * kColThreads, 0, stream>>>(p);
+    // four teams where all records' workgroups are resident at once that way
+    const int records = p.parts.tiles ? p.parts.tiles : p.groups;
+    const int teams = records * kCols * kTeam * kMaxTeams <= p.groups * 2048 ? kMaxTeams : 1;
+    latent_join_kernel<BF16><<<dim3(records, kCols), kTeam * teams, 0, stream>>>(p);
     return hipGetLastError() == hipSuccess ? kOk : kErrLaunch;
 }
 
@@ -660,10 +765,18 @@ int latent_attend(const MlkLatentBatch &b, const LatentAttend &p, int cu_count, 
     a.heads = p.heads;
     a.scale = p.scale * 1.44269504f;
     a.groups = cu_count < kMaxGroups ? cu_count : kMaxGroups;
+    const long room = (long)b.table_width * b.page_size;
+    a.keys = room < 0x7FFFFFFF ? (int)room : 0x7FFFFFFF;
+    // units of more keys where there could be 2^31 of them (a tile has at least a column)
+    const long tiles = (long)p.rows * p.heads / kCols + b.seqs;
+    a.parts.tiles = tiles <= kMaxTileRecords ? (int)tiles : 0;
+    for (a.shift = 0; tiles * ((a.keys - 1) / (kStepKeys << a.shift) + 1) >= 0x7FFFFFFF; ++a.shift) {}
+    a.page = Divisor::of((unsigned)b.page_size);
+    a.head = Divisor::of((unsigned)p.heads);
     uint8_t *at = static_cast<uint8_t *>(p.workspace);
     a.parts.sums = reinterpret_cast<float *>(at);
     a.parts.stats = reinterpret_cast<float *>(at + kSumsBytes);
-    a.parts.records = reinterpret_cast<int *>(at + kSumsBytes + kStatsBytes);
+    a.parts.records = reinterpret_cast<Record *>(at + kSumsBytes + kStatsBytes);
     const bool full = b.latent == kLatentMax && b.rope == kLatentRopeMax;
     if (b.type == MLK_FP4)
         return p.bf16 ? (full ? launch<true, true, true>(a, stream) : launch<true, true, false>(a, stream))
