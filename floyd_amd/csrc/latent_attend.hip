@@ -48,8 +48,8 @@ constexpr int kMaxGroups = 512;                  // workgroups of a launch
 // Waves of a workgroup, one workgroup a CU: with bf16 queries in LDS (18 KB) beside 17 KB of
 // keys for each wave there is room for two waves on a SIMD, one's loads under the other's
 // products; f32 queries take three bf16 parts (55 KB).
-template <bool BF16> constexpr int kWavesOf = BF16 ? 8 : 4;
-template <bool BF16> constexpr int kAheadOf = BF16 ? 2 : 3;  // steps that queries are read ahead
+template <bool FP4, bool BF16> constexpr int kWavesOf = FP4 && BF16 ? 8 : 4;
+template <int WAVES> constexpr int kAheadOf = WAVES == 8 ? 2 : 3;  // steps that queries are read ahead
 
 // A wave's keys in LDS: rows 32 bytes apart from a multiple of the banks, so that neither
 // the rows of a transposed read nor those of a write share them.
@@ -341,8 +341,8 @@ template <bool BF16> __device__ __forceinline__ void store4(void *out, long at, 
 constexpr float kSlack = 8.0f;
 
 template <bool FP4, bool BF16, bool FULL>
-__global__ __launch_bounds__(kWavesOf<BF16> *kWave, 1) void latent_attend_kernel(Params p) {
-    constexpr int kWaves = kWavesOf<BF16>, kThreads = kWaves * kWave;
+__global__ __launch_bounds__((kWavesOf<FP4, BF16> * kWave), 1) void latent_attend_kernel(Params p) {
+    constexpr int kWaves = kWavesOf<FP4, BF16>, kThreads = kWaves * kWave;
     constexpr int kParts = BF16 ? 1 : 3;  // bf16 parts of a query value and of a probability
     extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
     __shared__ __attribute__((aligned(16))) float tops[kCols][kWaves], sums[kCols][kWaves];
@@ -362,6 +362,9 @@ __global__ __launch_bounds__(kWavesOf<BF16> *kWave, 1) void latent_attend_kernel
     for (int s = run.seq; left > 0 && s < p.b.seqs; ++s, offset = 0) {
         const Work w = work_of(p, p.b.seqs <= kThreads ? held[s] : latent_seq(p.b, s, p.rows));
         while (left > 0 && offset < w.per * w.tiles) {
+            // (what follows from it is not worth a register from one tile to the next)
+            int tid = t;
+            asm volatile("" : "+v"(tid));
             const int tile = (int)((unsigned)offset / (unsigned)w.per), first = offset - tile * w.per;
             const int last = left < w.per - first ? first + left : w.per;
             left -= last - first;
@@ -395,13 +398,13 @@ __global__ __launch_bounds__(kWavesOf<BF16> *kWave, 1) void latent_attend_kernel
             unsigned in_page = 0, next_in_page;
             int page = 0, next_page = page_of(from + wave, &next_in_page);
 
-            // the queries into LDS, 8 values a thread and pass
+            // the queries, 8 values a thread and pass
             constexpr int kPieces = (kLatentMax + kLatentRopeMax) / 8;
             constexpr int kLoads = (kCols * kPieces + kThreads - 1) / kThreads;
             u32x4 pieces[kLoads][BF16 ? 1 : 2];
 #pragma unroll
             for (int y = 0; y < kLoads; ++y) {
-                const int i = t + y * kThreads, col = i / kPieces, d = 8 * (i % kPieces);
+                const int i = tid + y * kThreads, col = i / kPieces, d = 8 * (i % kPieces);
                 const bool in = col < used && (FULL || (d < kLatentMax ? d < latent : d - kLatentMax < rope));
                 const long at = (base + col) * width + (FULL || d < kLatentMax ? d : latent + d - kLatentMax);
 #pragma unroll
@@ -412,36 +415,10 @@ __global__ __launch_bounds__(kWavesOf<BF16> *kWave, 1) void latent_attend_kernel
                     else __builtin_memcpy(&pieces[y][h], static_cast<const float *>(p.q) + at + 4 * h, 16);
                 }
             }
-            __syncthreads();  // (the tile before is done with them)
-#pragma unroll
-            for (int y = 0; y < kLoads; ++y) {
-                const int i = t + y * kThreads, col = i / kPieces, d = 8 * (i % kPieces);
-                if (kCols * kPieces % kThreads && i >= kCols * kPieces) break;
-                uint16_t *to = query_lds + col * kQueryStride + d;
-                if constexpr (BF16) {
-                    *reinterpret_cast<u32x4 *>(to) = pieces[y][0];
-                } else {
-                    u32x4 v[3];
-#pragma unroll
-                    for (int k = 0; k < 4; ++k) {
-                        unsigned lo[3], hi[3];
-                        split3(__uint_as_float(pieces[y][k / 2][2 * (k % 2)]), lo);
-                        split3(__uint_as_float(pieces[y][k / 2][2 * (k % 2) + 1]), hi);
-#pragma unroll
-                        for (int x = 0; x < 3; ++x) v[x][k] = lo[x] | hi[x] << 16;
-                    }
-#pragma unroll
-                    for (int x = 0; x < 3; ++x) *reinterpret_cast<u32x4 *>(to + x * kCols * kQueryStride) = v[x];
-                }
-            }
-            __syncthreads();
-
             // Running softmax: lane (c, g) holds column c, its sum over keys 4 g .. 4 g + 3 of
             // every step; a row that sees keys behind its table is NaN.
             float top = -INFINITY, sum = c < used && sees > w.keys ? NAN : 0.0f;
             f32x4 out[kDims];
-#pragma unroll
-            for (int d = 0; d < kDims; ++d) out[d] = f32x4{0.f, 0.f, 0.f, 0.f};
 
             Raw<FP4> raw;
             for (int step = from + wave - kWaves;; step += kWaves) {
@@ -453,7 +430,7 @@ __global__ __launch_bounds__(kWavesOf<BF16> *kWave, 1) void latent_attend_kernel
                 if (live) {
                     // (queries come from LDS a few steps ahead of their product, and no more:
                     // registers are what limits a wave here)
-                    constexpr int kAhead = kAheadOf<BF16>;
+                    constexpr int kAhead = kAheadOf<kWaves>;
                     u32x4 ahead[2][kAhead][kParts];
                     const auto fetch = [&](int j0) {
 #pragma unroll
@@ -494,8 +471,34 @@ __global__ __launch_bounds__(kWavesOf<BF16> *kWave, 1) void latent_attend_kernel
                     load_key<FP4, FULL>(raw, static_cast<const uint8_t *>(p.b.data) + slot * row_bytes, g, latent, rope);
                 }
                 if (!live) {
-                    if (step < from) continue;
-                    break;
+                    if (step >= from) break;
+                    // once, the first keys on their way
+                    __syncthreads();  // (the tile before is done with them)
+#pragma unroll
+                    for (int y = 0; y < kLoads; ++y) {
+                        const int i = tid + y * kThreads, col = i / kPieces, d = 8 * (i % kPieces);
+                        if (kCols * kPieces % kThreads && i >= kCols * kPieces) break;
+                        uint16_t *to = query_lds + col * kQueryStride + d;
+                        if constexpr (BF16) {
+                            *reinterpret_cast<u32x4 *>(to) = pieces[y][0];
+                        } else {
+                            u32x4 v[3];
+#pragma unroll
+                            for (int k = 0; k < 4; ++k) {
+                                unsigned lo[3], hi[3];
+                                split3(__uint_as_float(pieces[y][k / 2][2 * (k % 2)]), lo);
+                                split3(__uint_as_float(pieces[y][k / 2][2 * (k % 2) + 1]), hi);
+#pragma unroll
+                                for (int x = 0; x < 3; ++x) v[x][k] = lo[x] | hi[x] << 16;
+                            }
+#pragma unroll
+                            for (int x = 0; x < 3; ++x) *reinterpret_cast<u32x4 *>(to + x * kCols * kQueryStride) = v[x];
+                        }
+                    }
+                    __syncthreads();
+#pragma unroll
+                    for (int d = 0; d < kDims; ++d) out[d] = f32x4{0.f, 0.f, 0.f, 0.f};
+                    continue;
                 }
                 f32x4 sc = score[0];
                 if constexpr (!BF16) sc += score[1] + score[2];
@@ -564,7 +567,7 @@ __global__ __launch_bounds__(kWavesOf<BF16> *kWave, 1) void latent_attend_kernel
                 }
                 __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
                 const uint8_t *from_lds = keys_lds + (4 * g + c / 4) * kKeyStride + 8 * (c % 4);
-                constexpr int kRead = BF16 ? 4 : 8;
+                constexpr int kRead = kWaves == 8 ? 4 : 8;
                 s16x4 turned[2][kRead];
                 const auto read = [&](int d0) {
 #pragma unroll
@@ -602,7 +605,7 @@ __global__ __launch_bounds__(kWavesOf<BF16> *kWave, 1) void latent_attend_kernel
             const int part = 2 * group + (first == 0 ? 1 : 0);
             // a thread's column of the results, 4 values at a time
             constexpr int kColThreads = kThreads / kCols, kPasses = kJoinDims / (4 * kColThreads);
-            const int col = t / kColThreads, at = 4 * (t % kColThreads);
+            const int col = tid / kColThreads, at = 4 * (tid % kColThreads);
             float col_top = -INFINITY, col_sum = 0.0f, by[kWaves], over = 0.0f;
             float *results = reinterpret_cast<float *>(lds);
 #pragma unroll
@@ -646,7 +649,7 @@ __global__ __launch_bounds__(kWavesOf<BF16> *kWave, 1) void latent_attend_kernel
                         store4<BF16>(p.out, (base + col) * latent + d, v[k] * over);
                 }
             }
-            if (!whole && t % kColThreads == 0) {
+            if (!whole && at == 0) {
                 p.parts.stats[part * 2 * kCols + col] = col_top;
                 p.parts.stats[(part * 2 + 1) * kCols + col] = col_sum;
             }
@@ -736,8 +739,8 @@ template <bool BF16> __global__ __launch_bounds__(kTeam *kMaxTeams) void latent_
 }
 
 template <bool FP4, bool BF16, bool FULL> int launch(const Params &p, hipStream_t stream) {
-    constexpr int threads = kWavesOf<BF16> * kWave;
-    constexpr int bytes = kWavesOf<BF16> * kKeyBytes + kQueryBytes<BF16>;
+    constexpr int threads = kWavesOf<FP4, BF16> * kWave;
+    constexpr int bytes = kWavesOf<FP4, BF16> * kKeyBytes + kQueryBytes<BF16>;
     const auto kernel = latent_attend_kernel<FP4, BF16, FULL>;
     static const bool ok = hipFuncSetAttribute(reinterpret_cast<const void *>(kernel),
                                                hipFuncAttributeMaxDynamicSharedMemorySize, bytes) == hipSuccess;
