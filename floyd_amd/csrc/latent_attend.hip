@@ -4,8 +4,8 @@
 //   s_j = scale * q . [latent_j | rope_j],  out = sum_j exp(s_j - m) latent_j / sum_j exp(s_j - m)
 //
 // for each (token row, head); a sequence's (row, head) pairs are taken 16 at a time
-// (a tile: the 16 columns of a matrix instruction), and a tile's keys 16 at a time (a
-// unit; more where units could not be counted in 32 bits).  The units of all tiles, in order, are dealt out in equal runs to as many
+// (a tile: the 16 columns of a matrix instruction), and a tile's keys 16 or 32 at a time
+// (a step, and a unit where those can be counted in 32 bits).  The units of all tiles, in order, are dealt out in equal runs to as many
 // workgroups as the chip holds, so ragged lengths leave none of them idle; a tile whose
 // units fell to several is joined by latent_join_kernel from their partial sums.
 //
@@ -13,7 +13,7 @@
 // their own, and meet at the end of a tile.  The keys are read straight into the matrix operand
 // (lane (k, g): 8 values of key k at a step), so the scores S[key][column] come from
 // v_mfma_f32_16x16x32_bf16; their registers hold 4 keys of a column, which is the operand
-// layout of the second product O[latent][column] += V^T P on v_mfma_f32_16x16x16_bf16.
+// layout of the second product O[latent][column] += V^T P (of two products for 32 keys).
 // V^T, the same keys with the latent index across lanes, goes through a piece of LDS of
 // the wave's own, written in rows and read transposed (ds_read_b64_tr_b16).  The next
 // keys are on their way from when the first product has taken the present ones, and the
@@ -37,29 +37,29 @@ typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef u32x4 u32x4_any __attribute__((aligned(2)));
 
 constexpr int kCols = 16;       // (row, head) pairs of a tile
-constexpr int kStepKeys = 16, kStepShift = 4;  // keys of a wave's step
-constexpr int kLeastUnits = 4;  // that a workgroup takes, where there are as many
+constexpr int kKeys = 16;       // keys of a product: its rows
+// Products of a wave's step: with two the queries are read once for 32 keys, and the second
+// product takes 32 keys an instruction.  (f32 queries leave the LDS no room for it.)
+template <bool BF16> constexpr int kTwo = BF16 ? 2 : 1;
+constexpr int kLeastShift = 6;  // log2 of the keys that a workgroup takes, where there are as many
 constexpr int kSteps = kLatentMax / 32;          // product steps over a latent row
 constexpr int kRopeSteps = kLatentRopeMax / 32;  // and over a rope row
 constexpr int kAllSteps = kSteps + kRopeSteps;
 constexpr int kDims = kLatentMax / 16;           // 16-value tiles of a latent row
 constexpr int kMaxGroups = 512;                  // workgroups of a launch
 
-// Waves of a workgroup, one workgroup a CU: with bf16 queries in LDS (18 KB) beside 17 KB of
-// keys for each wave there is room for two waves on a SIMD, one's loads under the other's
-// products; f32 queries take three bf16 parts (55 KB).
-template <bool FP4, bool BF16> constexpr int kWavesOf = FP4 && BF16 ? 8 : 4;
-template <int WAVES> constexpr int kAheadOf = WAVES == 8 ? 2 : 3;  // steps that queries are read ahead
+// One workgroup a CU, one wave a SIMD: 128 registers hold results, 144 keys on their way.
+constexpr int kWaves = 4, kThreads = kWaves * kWave;
 
 // A wave's keys in LDS: rows 32 bytes apart from a multiple of the banks, so that neither
 // the rows of a transposed read nor those of a write share them.
 constexpr int kKeyStride = 2 * kLatentMax + 32;
-constexpr int kKeyBytes = kStepKeys * kKeyStride;
+template <int TWO> constexpr int kKeyBytes = TWO * kKeys * kKeyStride;
 // The waves' results in LDS, kJoinDims latent values of each column at a time, each wave's
 // where its keys were (the others may still read theirs).
 constexpr int kJoinDims = 256;
 constexpr int kJoinStride = kJoinDims + 4;
-static_assert(kCols * kJoinStride * 4 <= kKeyBytes, "the results fit where the keys were");
+static_assert(kCols * kJoinStride * 4 <= kKeyBytes<1>, "the results fit where the keys were");
 constexpr int kQueryStride = kLatentMax + kLatentRopeMax + 8;
 template <bool BF16> constexpr int kQueryBytes = (BF16 ? 1 : 3) * kCols * kQueryStride * 2;
 
@@ -111,10 +111,14 @@ struct Params {
     float scale;  // times log2(e)
     int groups;
     int keys;     // that a table can hold
-    int shift;    // a unit is kStepKeys << shift keys
+    int step, shift;  // keys of a step, a unit is 2^shift steps: log2 of both
     Divisor page, head;
     Parts parts;
 };
+
+// A value that all lanes of a wave hold, known to be one: what depends on it is computed and
+// branched on once for the wave.
+__device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
 
 // A sequence's work.
 struct Work {
@@ -129,7 +133,7 @@ __device__ __forceinline__ Work work_of(const Params &p, const LatentSeq &seq) {
     w.seq = seq;
     const int length = seq.length < 0 ? 0 : seq.length;
     w.keys = length < p.keys ? length : p.keys;
-    w.per = w.keys > 0 ? ((w.keys - 1) >> (kStepShift + p.shift)) + 1 : 1;
+    w.per = w.keys > 0 ? ((w.keys - 1) >> (p.step + p.shift)) + 1 : 1;
     // (rows * heads is below 2^31 - 15)
     w.tiles = (int)(((unsigned)seq.count * (unsigned)p.heads + (kCols - 1)) / kCols);
     return w;
@@ -157,10 +161,10 @@ __device__ __forceinline__ int wave_scan(int v) {
 struct Run {
     int seq, offset, begin, length;
     int share, rest;  // workgroups have `share` units each, the first `rest` of them one more
-    // Of `total` units, dealt to no more workgroups than leaves each kLeastUnits: then no
-    // run between those of one tile is empty, and a tile has no more parts than pay.
-    __device__ __forceinline__ void deal(int total, int groups, int group) {
-        const int most = (total + kLeastUnits - 1) / kLeastUnits;
+    // Of `total` units, dealt to no more workgroups than leaves each 2^kLeastShift keys: then no run
+    // between those of one tile is empty, and a tile has no more parts than pay.
+    __device__ __forceinline__ void deal(int total, int groups, int group, int step) {
+        const int most = ((total - 1) >> (kLeastShift - step)) + 1;
         groups = most < groups ? most : groups;
         offset = begin = length = share = seq = rest = 0;
         if (group >= groups) return;
@@ -177,10 +181,9 @@ struct Run {
 };
 
 // The sequences are in LDS (`held`) where a workgroup has a thread for each.
-template <int WAVES> __device__ __forceinline__ Run find_run(const Params &p, int group, LatentSeq *held) {
-    constexpr int kThreads = WAVES * kWave;
-    __shared__ int sums[WAVES], at[2];
-    const int t = threadIdx.x, wave = t / kWave, lane = t % kWave;
+__device__ __forceinline__ Run find_run(const Params &p, int group, LatentSeq *held) {
+    __shared__ int sums[kWaves], at[2];
+    const int t = threadIdx.x, wave = uniform(t / kWave), lane = t % kWave;
     const auto seq_of = [&](int s) { return s < p.b.seqs ? latent_seq(p.b, s, p.rows) : LatentSeq{0, 0, 0}; };
     const auto units_of = [&](const LatentSeq &q) {
         const Work w = work_of(p, q);
@@ -196,8 +199,8 @@ template <int WAVES> __device__ __forceinline__ Run find_run(const Params &p, in
         all = wave_sum_int(all);
         if (lane == 0) sums[wave] = all;
         __syncthreads();
-        for (int w = 0; w < WAVES; ++w) total += sums[w];
-        r.deal(total, p.groups, group);
+        for (int w = 0; w < kWaves; ++w) total += uniform(sums[w]);
+        r.deal(total, p.groups, group, p.step);
     }
     int before = 0;
     for (int s0 = 0;; s0 += kThreads) {
@@ -208,11 +211,11 @@ template <int WAVES> __device__ __forceinline__ Run find_run(const Params &p, in
         __syncthreads();
         int first = before + upto - units;
 #pragma unroll
-        for (int w = 0; w < WAVES; ++w) {
+        for (int w = 0; w < kWaves; ++w) {
             if (w < wave) first += sums[w];
-            before += sums[w];
+            before += uniform(sums[w]);
         }
-        if (p.b.seqs <= kThreads) r.deal(before, p.groups, group);
+        if (p.b.seqs <= kThreads) r.deal(before, p.groups, group, p.step);
         if (r.begin >= first && r.begin < first + units) {
             at[0] = s0 + t;
             at[1] = r.begin - first;
@@ -221,8 +224,8 @@ template <int WAVES> __device__ __forceinline__ Run find_run(const Params &p, in
     }
     __syncthreads();
     if (r.length > 0) {
-        r.seq = at[0];
-        r.offset = at[1];
+        r.seq = uniform(at[0]);
+        r.offset = uniform(at[1]);
     }
     return r;
 }
@@ -335,32 +338,37 @@ template <bool BF16> __device__ __forceinline__ void store4(void *out, long at, 
     else *reinterpret_cast<f32x4_any *>(static_cast<float *>(out) + at) = v;
 }
 
+// A sum that is in an accumulation register here.  Where sums begin and where they are
+// scaled, on both sides: else the compiler has all 128 moved out and back at every step.
+__device__ __forceinline__ void keep(f32x4 &v) { asm volatile("" : "+a"(v)); }
+
 // The reference that exponents are taken to moves up only when a score is this far above
 // it (in powers of 2): p stays below 2^8 and sums lose nothing by that, and most steps need
 // neither the maximum over the lane groups nor to scale what is summed.
 constexpr float kSlack = 8.0f;
 
 template <bool FP4, bool BF16, bool FULL>
-__global__ __launch_bounds__((kWavesOf<FP4, BF16> * kWave), 1) void latent_attend_kernel(Params p) {
-    constexpr int kWaves = kWavesOf<FP4, BF16>, kThreads = kWaves * kWave;
+__global__ __launch_bounds__(kThreads, 1) void latent_attend_kernel(Params p) {
+    constexpr int kT = kTwo<BF16>, kStepKeys = kT * kKeys;
     constexpr int kParts = BF16 ? 1 : 3;  // bf16 parts of a query value and of a probability
     extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
     __shared__ __attribute__((aligned(16))) float tops[kCols][kWaves], sums[kCols][kWaves];
     __shared__ LatentSeq held[kThreads];
-    const int t = threadIdx.x, wave = t / kWave, lane = t % kWave;
+    const int t = threadIdx.x, wave = uniform(t / kWave), lane = t % kWave;
     const int g = lane / 16, c = lane % 16;
     const int latent = FULL ? kLatentMax : p.b.latent, rope = FULL ? kLatentRopeMax : p.b.rope;
     const int width = latent + rope, dims = latent / 16;
     const int row_bytes = latent_row_bytes(FP4, latent, rope);
-    uint8_t *keys_lds = lds + wave * kKeyBytes;
-    uint16_t *query_lds = reinterpret_cast<uint16_t *>(lds + kWaves * kKeyBytes);
+    uint8_t *keys_lds = lds + wave * kKeyBytes<kT>;
+    uint16_t *query_lds = reinterpret_cast<uint16_t *>(lds + kWaves * kKeyBytes<kT>);
 
     const int group = blockIdx.x;
-    const Run run = find_run<kWaves>(p, group, held);
+    const Run run = find_run(p, group, held);
     if (t == 0 && !p.parts.tiles) p.parts.records[group].first = -1;
     int left = run.length, offset = run.offset;
     for (int s = run.seq; left > 0 && s < p.b.seqs; ++s, offset = 0) {
-        const Work w = work_of(p, p.b.seqs <= kThreads ? held[s] : latent_seq(p.b, s, p.rows));
+        const LatentSeq seq = p.b.seqs <= kThreads ? held[s] : latent_seq(p.b, s, p.rows);
+        const Work w = work_of(p, {uniform(seq.begin), uniform(seq.count), uniform(seq.length)});
         while (left > 0 && offset < w.per * w.tiles) {
             // (what follows from it is not worth a register from one tile to the next)
             int tid = t;
@@ -381,22 +389,24 @@ __global__ __launch_bounds__((kWavesOf<FP4, BF16> * kWave), 1) void latent_atten
             const int limit = c < used ? within : 0;
             const int least = __builtin_amdgcn_readlane(within, 0);
             const int most = __builtin_amdgcn_readlane(within, used - 1);
-            // in steps of 16 keys
-            const int from = first << p.shift, seen_steps = (most + kStepKeys - 1) >> kStepShift;
+            // in steps
+            const int from = first << p.shift, seen_steps = (most + kStepKeys - 1) / kStepKeys;
             const int upto = (last << p.shift) < seen_steps ? last << p.shift : seen_steps;
 
-            // A key's page, loaded a step before the key; keys that nothing sees are taken from
+            // A key's page, asked for a step before the key; keys that nothing sees are taken from
             // page 0 (and out of the products).
             const int *table = p.b.tables + (long)s * p.b.table_width;
-            const auto page_of = [&](int step, unsigned *in_page) {
-                const unsigned j = (unsigned)step * kStepKeys + c, at = p.page.quotient(j);
+            const auto page_of = [&](int step, int x, unsigned *in_page) {
+                const unsigned j = (unsigned)step * kStepKeys + x * kKeys + c, at = p.page.quotient(j);
                 *in_page = j - at * (unsigned)p.b.page_size;
                 int page = 0;
                 if (step < upto && j < (unsigned)most) page = table[at];
                 return page;
             };
-            unsigned in_page = 0, next_in_page;
-            int page = 0, next_page = page_of(from + wave, &next_in_page);
+            unsigned in_page[kT];
+            int page[kT];
+#pragma unroll
+            for (int x = 0; x < kT; ++x) page[x] = page_of(from + wave, x, &in_page[x]);
 
             // the queries, 8 values a thread and pass
             constexpr int kPieces = (kLatentMax + kLatentRopeMax) / 8;
@@ -420,116 +430,135 @@ __global__ __launch_bounds__((kWavesOf<FP4, BF16> * kWave), 1) void latent_atten
             float top = -INFINITY, sum = c < used && sees > w.keys ? NAN : 0.0f;
             f32x4 out[kDims];
 
-            Raw<FP4> raw;
-            for (int step = from + wave - kWaves;; step += kWaves) {
-                const bool live = step >= from && step < upto;
-                const int key0 = step * kStepKeys;
-                f32x4 score[kParts];
+            const auto key_at = [&](int x, int j) {
+                return reinterpret_cast<u32x4 *>(keys_lds + (x * kKeys + c) * kKeyStride + 2 * dim_of<FP4>(j, g));
+            };
+            Raw<FP4> raw[kT];
+            unsigned bad_pages[kT];
+            // the keys of the step whose pages are there, and the pages of the step after it
+            const auto go_on = [&](int step) {
 #pragma unroll
-                for (int k = 0; k < kParts; ++k) score[k] = f32x4{0.f, 0.f, 0.f, 0.f};
-                if (live) {
-                    // (queries come from LDS a few steps ahead of their product, and no more:
-                    // registers are what limits a wave here)
-                    constexpr int kAhead = kAheadOf<kWaves>;
-                    u32x4 ahead[2][kAhead][kParts];
-                    const auto fetch = [&](int j0) {
+                for (int x = 0; x < kT; ++x) {
+                    const bool there = (unsigned)page[x] < (unsigned)p.b.pages;
+                    const long slot = there ? (long)page[x] * p.b.page_size + in_page[x] : 0;
+                    bad_pages[x] = (unsigned)__ballot(!there) & 0xFFFFu;
+                    page[x] = page_of(step + kWaves, x, &in_page[x]);
+                    load_key<FP4, FULL>(raw[x], static_cast<const uint8_t *>(p.b.data) + slot * row_bytes, g, latent, rope);
+                }
+            };
+            go_on(from + wave);
+            __syncthreads();  // (the tile before is done with them)
 #pragma unroll
-                        for (int x = 0; x < kAhead; ++x) {
-                            const int j = j0 + x;
-                            const int at = j < kSteps ? dim_of<FP4>(j, g) : kLatentMax + 32 * (j - kSteps) + 8 * g;
+            for (int y = 0; y < kLoads; ++y) {
+                const int i = tid + y * kThreads, col = i / kPieces, d = 8 * (i % kPieces);
+                if (kCols * kPieces % kThreads && i >= kCols * kPieces) break;
+                uint16_t *to = query_lds + col * kQueryStride + d;
+                if constexpr (BF16) {
+                    *reinterpret_cast<u32x4 *>(to) = pieces[y][0];
+                } else {
+                    u32x4 v[3];
 #pragma unroll
-                            for (int k = 0; k < kParts; ++k)
-                                ahead[j0 / kAhead % 2][x][k] =
-                                    *reinterpret_cast<const u32x4 *>(query_lds + (k * kCols + c) * kQueryStride + at);
-                        }
-                    };
-                    fetch(0);
+                    for (int k = 0; k < 4; ++k) {
+                        unsigned lo[3], hi[3];
+                        split3(__uint_as_float(pieces[y][k / 2][2 * (k % 2)]), lo);
+                        split3(__uint_as_float(pieces[y][k / 2][2 * (k % 2) + 1]), hi);
 #pragma unroll
-                    for (int j0 = 0; j0 < kAllSteps; j0 += kAhead) {
-                        __builtin_amdgcn_sched_barrier(0);
-                        if (j0 + kAhead < kAllSteps) fetch(j0 + kAhead);
-#pragma unroll
-                        for (int x = 0; x < kAhead; ++x) {
-                            const int j = j0 + x;
-                            const u32x4 v = operand<FP4, FULL>(raw, j, g, latent);
-                            if (j < kSteps)
-                                *reinterpret_cast<u32x4 *>(keys_lds + c * kKeyStride + 2 * dim_of<FP4>(j, g)) = v;
-#pragma unroll
-                            for (int k = 0; k < kParts; ++k)
-                                score[k] = mfma32(v, ahead[j0 / kAhead % 2][x][k], score[k]);
-                        }
+                        for (int x = 0; x < 3; ++x) v[x][k] = lo[x] | hi[x] << 16;
                     }
-                    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                    for (int x = 0; x < 3; ++x) *reinterpret_cast<u32x4 *>(to + x * kCols * kQueryStride) = v[x];
                 }
-                // the page of the step after the next, then the next step's keys
-                const unsigned bad_pages = (unsigned)__ballot((unsigned)page >= (unsigned)p.b.pages) & 0xFFFFu;
-                page = next_page;
-                in_page = next_in_page;
-                next_page = page_of(step + 2 * kWaves, &next_in_page);
-                if (step + kWaves < upto) {
-                    const long slot = (unsigned)page < (unsigned)p.b.pages ? (long)page * p.b.page_size + in_page : 0;
-                    load_key<FP4, FULL>(raw, static_cast<const uint8_t *>(p.b.data) + slot * row_bytes, g, latent, rope);
-                }
-                if (!live) {
-                    if (step >= from) break;
-                    // once, the first keys on their way
-                    __syncthreads();  // (the tile before is done with them)
+            }
+            __syncthreads();
 #pragma unroll
-                    for (int y = 0; y < kLoads; ++y) {
-                        const int i = tid + y * kThreads, col = i / kPieces, d = 8 * (i % kPieces);
-                        if (kCols * kPieces % kThreads && i >= kCols * kPieces) break;
-                        uint16_t *to = query_lds + col * kQueryStride + d;
-                        if constexpr (BF16) {
-                            *reinterpret_cast<u32x4 *>(to) = pieces[y][0];
-                        } else {
-                            u32x4 v[3];
-#pragma unroll
-                            for (int k = 0; k < 4; ++k) {
-                                unsigned lo[3], hi[3];
-                                split3(__uint_as_float(pieces[y][k / 2][2 * (k % 2)]), lo);
-                                split3(__uint_as_float(pieces[y][k / 2][2 * (k % 2) + 1]), hi);
-#pragma unroll
-                                for (int x = 0; x < 3; ++x) v[x][k] = lo[x] | hi[x] << 16;
-                            }
-#pragma unroll
-                            for (int x = 0; x < 3; ++x) *reinterpret_cast<u32x4 *>(to + x * kCols * kQueryStride) = v[x];
-                        }
-                    }
-                    __syncthreads();
-#pragma unroll
-                    for (int d = 0; d < kDims; ++d) out[d] = f32x4{0.f, 0.f, 0.f, 0.f};
-                    continue;
-                }
-                f32x4 sc = score[0];
-                if constexpr (!BF16) sc += score[1] + score[2];
+            for (int d = 0; d < kDims; ++d) {
+                out[d] = f32x4{0.f, 0.f, 0.f, 0.f};
+                keep(out[d]);
+            }
 
-                bool hidden[4] = {false, false, false, false};
-                if (bad_pages || key0 + kStepKeys > least) {
+            for (int step = from + wave; step < upto; step += kWaves) {
+                const int key0 = step * kStepKeys;
+                f32x4 score[kT][kParts];
+#pragma unroll
+                for (int x = 0; x < kT; ++x)
+#pragma unroll
+                    for (int k = 0; k < kParts; ++k) score[x][k] = f32x4{0.f, 0.f, 0.f, 0.f};
+                // (queries come from LDS a few steps ahead of their product)
+                constexpr int kAhead = 3;
+                u32x4 ahead[2][kAhead][kParts];
+                const auto fetch = [&](int j0) {
+#pragma unroll
+                    for (int y = 0; y < kAhead; ++y) {
+                        const int j = j0 + y;
+                        const int at = j < kSteps ? dim_of<FP4>(j, g) : kLatentMax + 32 * (j - kSteps) + 8 * g;
+#pragma unroll
+                        for (int k = 0; k < kParts; ++k)
+                            ahead[j0 / kAhead % 2][y][k] =
+                                *reinterpret_cast<const u32x4 *>(query_lds + (k * kCols + c) * kQueryStride + at);
+                    }
+                };
+                fetch(0);
+#pragma unroll
+                for (int j0 = 0; j0 < kAllSteps; j0 += kAhead) {
+                    __builtin_amdgcn_sched_barrier(0);
+                    if (j0 + kAhead < kAllSteps) fetch(j0 + kAhead);
+#pragma unroll
+                    for (int y = 0; y < kAhead; ++y) {
+                        const int j = j0 + y;
+#pragma unroll
+                        for (int x = 0; x < kT; ++x) {
+                            const u32x4 v = operand<FP4, FULL>(raw[x], j, g, latent);
+                            if (j < kSteps) *key_at(x, j) = v;
+#pragma unroll
+                            for (int k = 0; k < kParts; ++k)
+                                score[x][k] = mfma32(v, ahead[j0 / kAhead % 2][y][k], score[x][k]);
+                        }
+                    }
+                }
+                __builtin_amdgcn_sched_barrier(0);
+                unsigned bad_now[kT];
+#pragma unroll
+                for (int x = 0; x < kT; ++x) bad_now[x] = bad_pages[x];
+                if (step + kWaves < upto) go_on(step + kWaves);
+                bool hidden[kT][4], edge = key0 + kStepKeys > least;
+#pragma unroll
+                for (int x = 0; x < kT; ++x) {
+                    if constexpr (!BF16) score[x][0] += score[x][1] + score[x][2];
+                    edge |= bad_now[x] != 0;
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) hidden[x][i] = false;
+                }
+                if (edge) {
                     // Keys that not every column sees, or that have no place: those that a
                     // column does not see must not reach it by 0 * NaN either, so rows that
                     // are not finite (or not there) are taken out of the second product and
                     // make NaN of the scores of the columns that see them.
-                    const bool there = key0 + c < most;
-                    bool odd = false;
-#pragma unroll 1
-                    for (int j = 0; j < kSteps; ++j)
-                        odd |= not_finite(*reinterpret_cast<const u32x4 *>(keys_lds + c * kKeyStride + 2 * dim_of<FP4>(j, g)));
-                    const unsigned long long which = __ballot(odd && there);
-                    const unsigned bad = bad_pages | ((unsigned)(which | which >> 16 | which >> 32 | which >> 48) & 0xFFFFu);
-                    if (!there || (bad >> c & 1u)) {
-#pragma unroll 1
-                        for (int j = 0; j < kSteps; ++j)
-                            *reinterpret_cast<u32x4 *>(keys_lds + c * kKeyStride + 2 * dim_of<FP4>(j, g)) = u32x4{0, 0, 0, 0};
-                    }
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        if (bad >> (4 * g + i) & 1u) sc[i] = NAN;
-                        hidden[i] = key0 + 4 * g + i >= limit;
+                    for (int x = 0; x < kT; ++x) {
+                        const int mine = key0 + x * kKeys + c;
+                        bool odd = false;
+#pragma unroll 1
+                        for (int j = 0; j < kSteps; ++j) odd |= not_finite(*key_at(x, j));
+                        const unsigned long long which = __ballot(odd && mine < most);
+                        const unsigned bad =
+                            bad_now[x] | ((unsigned)(which | which >> 16 | which >> 32 | which >> 48) & 0xFFFFu);
+                        if (mine >= most || (bad >> c & 1u)) {
+#pragma unroll 1
+                            for (int j = 0; j < kSteps; ++j) *key_at(x, j) = u32x4{0, 0, 0, 0};
+                        }
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            if (bad >> (4 * g + i) & 1u) score[x][0][i] = NAN;
+                            hidden[x][i] = key0 + x * kKeys + 4 * g + i >= limit;
+                        }
                     }
                 }
                 float high = -INFINITY;
 #pragma unroll
-                for (int i = 0; i < 4; ++i) high = fmaxf(high, hidden[i] ? -INFINITY : sc[i] * p.scale);
+                for (int x = 0; x < kT; ++x)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        high = fmaxf(high, hidden[x][i] ? -INFINITY : score[x][0][i] * p.scale);
                 if (__any(high > top + kSlack)) {
                     const float next = fmaxf(top, groups_max(high));
                     const float by = top == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(top - next);
@@ -538,42 +567,55 @@ __global__ __launch_bounds__((kWavesOf<FP4, BF16> * kWave), 1) void latent_atten
                     top = next;
                     if (begun) {
 #pragma unroll
-                        for (int d = 0; d < kDims; ++d) out[d] *= by;
+                        for (int d = 0; d < kDims; ++d) {
+                            keep(out[d]);
+                            out[d] *= by;
+                            keep(out[d]);
+                        }
                     }
                 }
                 const float to = top == -INFINITY ? 0.0f : top;
-                s16x4 probs[kParts];
-                float prob[4];
+                // probabilities, as the second product's operand: keys 4 g .. 4 g + 3 of each
+                union Probs {
+                    s16x4 one[kT];
+                    u32x4 two;
+                } probs[kParts];
 #pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    prob[i] = hidden[i] ? 0.0f : __builtin_amdgcn_exp2f(fmaf(sc[i], p.scale, -to));
-                if constexpr (BF16) {
-                    bf16x4 r;
+                for (int x = 0; x < kT; ++x) {
+                    float prob[4];
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        r[i] = (__bf16)prob[i];
-                        sum += (float)r[i];
-                    }
-                    probs[0] = __builtin_bit_cast(s16x4, r);
-                } else {
+                    for (int i = 0; i < 4; ++i)
+                        prob[i] = hidden[x][i] ? 0.0f : __builtin_amdgcn_exp2f(fmaf(score[x][0][i], p.scale, -to));
+                    if constexpr (BF16) {
+                        bf16x4 r;
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        unsigned part[3];
-                        split3(prob[i], part);
+                        for (int i = 0; i < 4; ++i) {
+                            r[i] = (__bf16)prob[i];
+                            sum += (float)r[i];
+                        }
+                        probs[0].one[x] = __builtin_bit_cast(s16x4, r);
+                    } else {
 #pragma unroll
-                        for (int k = 0; k < kParts; ++k) probs[k][i] = (short)part[k];
-                        sum += prob[i];
+                        for (int i = 0; i < 4; ++i) {
+                            unsigned part[3];
+                            split3(prob[i], part);
+#pragma unroll
+                            for (int k = 0; k < kParts; ++k) probs[k].one[x][i] = (short)part[k];
+                            sum += prob[i];
+                        }
                     }
                 }
                 __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
                 const uint8_t *from_lds = keys_lds + (4 * g + c / 4) * kKeyStride + 8 * (c % 4);
-                constexpr int kRead = kWaves == 8 ? 4 : 8;
-                s16x4 turned[2][kRead];
+                constexpr int kRead = 8;
+                Probs turned[2][kRead];
                 const auto read = [&](int d0) {
 #pragma unroll
-                    for (int x = 0; x < kRead; ++x)
-                        turned[d0 / kRead % 2][x] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                            (__attribute__((address_space(3))) s16x4 *)(from_lds + 32 * (d0 + x)));
+                    for (int y = 0; y < kRead; ++y)
+#pragma unroll
+                        for (int x = 0; x < kT; ++x)
+                            turned[d0 / kRead % 2][y].one[x] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                                (__attribute__((address_space(3))) s16x4 *)(from_lds + x * kKeys * kKeyStride + 32 * (d0 + y)));
                 };
                 read(0);
 #pragma unroll
@@ -582,11 +624,15 @@ __global__ __launch_bounds__((kWavesOf<FP4, BF16> * kWave), 1) void latent_atten
                     __builtin_amdgcn_sched_barrier(0);
                     if (d0 + kRead < kDims) read(d0 + kRead);
 #pragma unroll
-                    for (int x = 0; x < kRead; ++x)
+                    for (int y = 0; y < kRead; ++y)
 #pragma unroll
-                        for (int k = 0; k < kParts; ++k)
-                            out[d0 + x] = __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(turned[d0 / kRead % 2][x], probs[k],
-                                                                                   out[d0 + x], 0, 0, 0);
+                        for (int k = 0; k < kParts; ++k) {
+                            if constexpr (kT == 2)
+                                out[d0 + y] = mfma32(turned[d0 / kRead % 2][y].two, probs[k].two, out[d0 + y]);
+                            else
+                                out[d0 + y] = __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(
+                                    turned[d0 / kRead % 2][y].one[0], probs[k].one[0], out[d0 + y], 0, 0, 0);
+                        }
                 }
                 __builtin_amdgcn_sched_barrier(0);
                 __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
@@ -615,7 +661,7 @@ __global__ __launch_bounds__((kWavesOf<FP4, BF16> * kWave), 1) void latent_atten
                 if (wave < busy) {
 #pragma unroll
                     for (int d = 0; d < kJoinDims / 16; ++d)
-                        *reinterpret_cast<f32x4 *>(results + wave * (kKeyBytes / 4) + c * kJoinStride + 16 * d + 4 * g) =
+                        *reinterpret_cast<f32x4 *>(results + wave * (kKeyBytes<kT> / 4) + c * kJoinStride + 16 * d + 4 * g) =
                             out[round * (kJoinDims / 16) + d];
                 }
                 __syncthreads();
@@ -637,7 +683,7 @@ __global__ __launch_bounds__((kWavesOf<FP4, BF16> * kWave), 1) void latent_atten
                     if (x >= busy) break;
 #pragma unroll
                     for (int k = 0; k < kPasses; ++k)
-                        v[k] += by[x] * load_f4(results + x * (kKeyBytes / 4) + col * kJoinStride + at + 4 * kColThreads * k);
+                        v[k] += by[x] * load_f4(results + x * (kKeyBytes<kT> / 4) + col * kJoinStride + at + 4 * kColThreads * k);
                 }
 #pragma unroll
                 for (int k = 0; k < kPasses; ++k) {
@@ -739,13 +785,12 @@ template <bool BF16> __global__ __launch_bounds__(kTeam *kMaxTeams) void latent_
 }
 
 template <bool FP4, bool BF16, bool FULL> int launch(const Params &p, hipStream_t stream) {
-    constexpr int threads = kWavesOf<FP4, BF16> * kWave;
-    constexpr int bytes = kWavesOf<FP4, BF16> * kKeyBytes + kQueryBytes<BF16>;
+    constexpr int bytes = kWaves * kKeyBytes<kTwo<BF16>> + kQueryBytes<BF16>;
     const auto kernel = latent_attend_kernel<FP4, BF16, FULL>;
     static const bool ok = hipFuncSetAttribute(reinterpret_cast<const void *>(kernel),
                                                hipFuncAttributeMaxDynamicSharedMemorySize, bytes) == hipSuccess;
     if (!ok) return kErrLaunch;
-    kernel<<<p.groups, threads, bytes, stream>>>(p);
+    kernel<<<p.groups, kThreads, bytes, stream>>>(p);
     if (hipGetLastError() != hipSuccess) return kErrLaunch;
     if (p.groups == 1) return kOk;
     // four teams where all records' workgroups are resident at once that way
@@ -773,7 +818,9 @@ int latent_attend(const MlkLatentBatch &b, const LatentAttend &p, int cu_count, 
     // units of more keys where there could be 2^31 of them (a tile has at least a column)
     const long tiles = (long)p.rows * p.heads / kCols + b.seqs;
     a.parts.tiles = tiles <= kMaxTileRecords ? (int)tiles : 0;
-    for (a.shift = 0; tiles * ((a.keys - 1) / (kStepKeys << a.shift) + 1) >= 0x7FFFFFFF; ++a.shift) {}
+    a.step = p.bf16 ? 5 : 4;
+    static_assert(kTwo<true> * kKeys == 32 && kTwo<false> * kKeys == 16, "a step's keys");
+    for (a.shift = 0; tiles * (((a.keys - 1) >> (a.step + a.shift)) + 1) >= 0x7FFFFFFF; ++a.shift) {}
     a.page = Divisor::of((unsigned)b.page_size);
     a.head = Divisor::of((unsigned)p.heads);
     uint8_t *at = static_cast<uint8_t *>(p.workspace);
