@@ -4,20 +4,24 @@
 //   s_j = scale * q . [latent_j | rope_j],  out = sum_j exp(s_j - m) latent_j / sum_j exp(s_j - m)
 //
 // for each (token row, head); a sequence's (row, head) pairs are taken 16 at a time
-// (a tile: the 16 columns of a matrix instruction), and a tile's keys 16 or 32 at a time
-// (a step, and a unit where those can be counted in 32 bits).  The units of all tiles, in order, are dealt out in equal runs to as many
+// (a tile: the 16 columns of a matrix instruction), and a tile's keys 16 at a time (a
+// step, and a unit where those can be counted in 32 bits).  The units of all tiles, in order, are dealt out in equal runs to as many
 // workgroups as the chip holds, so ragged lengths leave none of them idle; a tile whose
 // units fell to several is joined by latent_join_kernel from their partial sums.
 //
-// The waves of a workgroup take its units in turn, with a running maximum and sum of
-// their own, and meet at the end of a tile.  The keys are read straight into the matrix operand
-// (lane (k, g): 8 values of key k at a step), so the scores S[key][column] come from
+// The waves of a workgroup take its steps in turn, with a running maximum and sum of their
+// own, and meet at the end of a tile.  The keys are read straight into the matrix operand
+// (lane (k, g): 8 values of key k at a product step), so the scores S[key][column] come from
 // v_mfma_f32_16x16x32_bf16; their registers hold 4 keys of a column, which is the operand
-// layout of the second product O[latent][column] += V^T P (of two products for 32 keys).
-// V^T, the same keys with the latent index across lanes, goes through a piece of LDS of
-// the wave's own, written in rows and read transposed (ds_read_b64_tr_b16).  The next
-// keys are on their way from when the first product has taken the present ones, and the
-// page numbers of those after them.
+// layout of the second product O[latent][column] += V^T P on v_mfma_f32_16x16x16_bf16.
+// V^T, the same keys with the latent index across lanes, is a product too: with the
+// identity, whose result registers hold 4 keys of a latent value, exact and to be packed.
+// (Through LDS, written in rows and read transposed, it is 16 KB of writes and as much of
+// reads a step: 4-bit keys took the same, bf16 ones 3 % less, and f32 queries, for which the
+// LDS then has room for four waves only, 13 % more.)
+//
+// The next keys are on their way from when the first product has taken the present ones, and
+// the page numbers of those after them.
 //
 // What runs once costs its instructions' way from memory, about 4 cycles a byte: loops are
 // entered a step early rather than with a copy of their loads before them, and unrolled
@@ -37,10 +41,7 @@ typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef u32x4 u32x4_any __attribute__((aligned(2)));
 
 constexpr int kCols = 16;       // (row, head) pairs of a tile
-constexpr int kKeys = 16;       // keys of a product: its rows
-// Products of a wave's step: with two the queries are read once for 32 keys, and the second
-// product takes 32 keys an instruction.  (f32 queries leave the LDS no room for it.)
-template <bool BF16> constexpr int kTwo = BF16 ? 2 : 1;
+constexpr int kStepKeys = 16, kStepShift = 4;  // keys of a wave's step
 constexpr int kLeastShift = 6;  // log2 of the keys that a workgroup takes, where there are as many
 constexpr int kSteps = kLatentMax / 32;          // product steps over a latent row
 constexpr int kRopeSteps = kLatentRopeMax / 32;  // and over a rope row
@@ -48,20 +49,19 @@ constexpr int kAllSteps = kSteps + kRopeSteps;
 constexpr int kDims = kLatentMax / 16;           // 16-value tiles of a latent row
 constexpr int kMaxGroups = 512;                  // workgroups of a launch
 
-// One workgroup a CU, one wave a SIMD: 128 registers hold results, 144 keys on their way.
-constexpr int kWaves = 4, kThreads = kWaves * kWave;
+// Waves of a workgroup, one workgroup a CU.  4-bit keys leave a wave in 256 registers, for two
+// waves on a SIMD; of bf16 keys, 72 registers a step, two steps are held by one.
+template <bool FP4> constexpr int kWavesOf = FP4 ? 8 : 4;
 
-// A wave's keys in LDS: rows 32 bytes apart from a multiple of the banks, so that neither
-// the rows of a transposed read nor those of a write share them.
-constexpr int kKeyStride = 2 * kLatentMax + 32;
-template <int TWO> constexpr int kKeyBytes = TWO * kKeys * kKeyStride;
-// The waves' results in LDS, kJoinDims latent values of each column at a time, each wave's
-// where its keys were (the others may still read theirs).
-constexpr int kJoinDims = 256;
-constexpr int kJoinStride = kJoinDims + 4;
-static_assert(kCols * kJoinStride * 4 <= kKeyBytes<1>, "the results fit where the keys were");
+// LDS: the queries (three bf16 parts of f32 ones); then, over them, the waves' results,
+// kJoinDims latent values of each column at a time, piece q (16 bytes) of column c at q ^ c:
+// the 16 lanes that write a piece of each column find them in different banks.
 constexpr int kQueryStride = kLatentMax + kLatentRopeMax + 8;
 template <bool BF16> constexpr int kQueryBytes = (BF16 ? 1 : 3) * kCols * kQueryStride * 2;
+constexpr int kJoinDims = 256;
+constexpr int kJoinBytes = kCols * kJoinDims * 4;  // of a wave
+template <bool FP4, bool BF16> constexpr int kLdsBytes =
+    kQueryBytes<BF16> > kWavesOf<FP4> * kJoinBytes ? kQueryBytes<BF16> : kWavesOf<FP4> * kJoinBytes;
 
 // What latent_join_kernel has to know of a tile, told by the workgroup that ends it: its
 // sequence and number in it, and the workgroups that its units fell to (-1: to one, there is
@@ -111,7 +111,7 @@ struct Params {
     float scale;  // times log2(e)
     int groups;
     int keys;     // that a table can hold
-    int step, shift;  // keys of a step, a unit is 2^shift steps: log2 of both
+    int shift;    // a unit is 2^shift steps
     Divisor page, head;
     Parts parts;
 };
@@ -133,7 +133,7 @@ __device__ __forceinline__ Work work_of(const Params &p, const LatentSeq &seq) {
     w.seq = seq;
     const int length = seq.length < 0 ? 0 : seq.length;
     w.keys = length < p.keys ? length : p.keys;
-    w.per = w.keys > 0 ? ((w.keys - 1) >> (p.step + p.shift)) + 1 : 1;
+    w.per = w.keys > 0 ? ((w.keys - 1) >> (kStepShift + p.shift)) + 1 : 1;
     // (rows * heads is below 2^31 - 15)
     w.tiles = (int)(((unsigned)seq.count * (unsigned)p.heads + (kCols - 1)) / kCols);
     return w;
@@ -163,8 +163,8 @@ struct Run {
     int share, rest;  // workgroups have `share` units each, the first `rest` of them one more
     // Of `total` units, dealt to no more workgroups than leaves each 2^kLeastShift keys: then no run
     // between those of one tile is empty, and a tile has no more parts than pay.
-    __device__ __forceinline__ void deal(int total, int groups, int group, int step) {
-        const int most = ((total - 1) >> (kLeastShift - step)) + 1;
+    __device__ __forceinline__ void deal(int total, int groups, int group) {
+        const int most = ((total - 1) >> (kLeastShift - kStepShift)) + 1;
         groups = most < groups ? most : groups;
         offset = begin = length = share = seq = rest = 0;
         if (group >= groups) return;
@@ -181,7 +181,8 @@ struct Run {
 };
 
 // The sequences are in LDS (`held`) where a workgroup has a thread for each.
-__device__ __forceinline__ Run find_run(const Params &p, int group, LatentSeq *held) {
+template <int WAVES> __device__ __forceinline__ Run find_run(const Params &p, int group, LatentSeq *held) {
+    constexpr int kWaves = WAVES, kThreads = kWaves * kWave;
     __shared__ int sums[kWaves], at[2];
     const int t = threadIdx.x, wave = uniform(t / kWave), lane = t % kWave;
     const auto seq_of = [&](int s) { return s < p.b.seqs ? latent_seq(p.b, s, p.rows) : LatentSeq{0, 0, 0}; };
@@ -200,7 +201,7 @@ __device__ __forceinline__ Run find_run(const Params &p, int group, LatentSeq *h
         if (lane == 0) sums[wave] = all;
         __syncthreads();
         for (int w = 0; w < kWaves; ++w) total += uniform(sums[w]);
-        r.deal(total, p.groups, group, p.step);
+        r.deal(total, p.groups, group);
     }
     int before = 0;
     for (int s0 = 0;; s0 += kThreads) {
@@ -215,7 +216,7 @@ __device__ __forceinline__ Run find_run(const Params &p, int group, LatentSeq *h
             if (w < wave) first += sums[w];
             before += uniform(sums[w]);
         }
-        if (p.b.seqs <= kThreads) r.deal(before, p.groups, group, p.step);
+        if (p.b.seqs <= kThreads) r.deal(before, p.groups, group);
         if (r.begin >= first && r.begin < first + units) {
             at[0] = s0 + t;
             at[1] = r.begin - first;
@@ -247,6 +248,33 @@ template <> struct Raw<true> {
     unsigned scales;
     u32x4 rope[kRopeSteps];
 };
+
+// Whether one of its latent values is not finite, and the key without its latent values.
+__device__ __forceinline__ bool not_finite(const Raw<true> &raw, int g, int latent) {
+    bool bad = false;
+#pragma unroll
+    for (int j = 0; j < kSteps / 4; ++j)  // (scales that a narrower row has not are any bytes)
+        bad |= 128 * j + 32 * g < latent && (raw.scales >> (8 * j) & 0xFFu) == 0xFFu;
+    return bad;
+}
+__device__ __forceinline__ bool not_finite(const Raw<false> &raw, int, int) {
+    bool bad = false;
+#pragma unroll
+    for (int j = 0; j < kSteps; ++j)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            bad |= (raw.v[j][i] & 0x7F80u) == 0x7F80u || (raw.v[j][i] & 0x7F800000u) == 0x7F800000u;
+    return bad;
+}
+__device__ __forceinline__ void drop(Raw<true> &raw) {
+    raw.scales = 0x7F7F7F7Fu;
+#pragma unroll
+    for (int j = 0; j < kSteps / 4; ++j) raw.codes[j] = u32x4{0, 0, 0, 0};
+}
+__device__ __forceinline__ void drop(Raw<false> &raw) {
+#pragma unroll
+    for (int j = 0; j < kSteps; ++j) raw.v[j] = u32x4{0, 0, 0, 0};
+}
 
 template <bool FP4, bool FULL>
 __device__ __forceinline__ void load_key(Raw<FP4> &raw, const uint8_t *row, int g, int latent, int rope) {
@@ -294,14 +322,6 @@ __device__ __forceinline__ u32x4 operand(const Raw<FP4> &raw, int j, int g, int 
     }
 }
 
-__device__ __forceinline__ bool not_finite(const u32x4 &v) {
-    bool bad = false;
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-        bad |= (v[i] & 0x7F80u) == 0x7F80u || (v[i] & 0x7F800000u) == 0x7F800000u;
-    return bad;
-}
-
 // x as three bf16 parts that add up to it, cut off one after the other.
 __device__ __forceinline__ void split3(float x, unsigned (&part)[3]) {
     const unsigned a = __float_as_uint(x) & 0xFFFF0000u;
@@ -338,8 +358,9 @@ template <bool BF16> __device__ __forceinline__ void store4(void *out, long at, 
     else *reinterpret_cast<f32x4_any *>(static_cast<float *>(out) + at) = v;
 }
 
-// A sum that is in an accumulation register here.  Where sums begin and where they are
-// scaled, on both sides: else the compiler has all 128 moved out and back at every step.
+// A sum that is in an accumulation register here.  With 512 registers, where sums begin and
+// where they are scaled, on both sides: else the compiler has all 128 moved out and back at
+// every step.  (Of 256 all are alike.)
 __device__ __forceinline__ void keep(f32x4 &v) { asm volatile("" : "+a"(v)); }
 
 // The reference that exponents are taken to moves up only when a score is this far above
@@ -348,22 +369,31 @@ __device__ __forceinline__ void keep(f32x4 &v) { asm volatile("" : "+a"(v)); }
 constexpr float kSlack = 8.0f;
 
 template <bool FP4, bool BF16, bool FULL>
-__global__ __launch_bounds__(kThreads, 1) void latent_attend_kernel(Params p) {
-    constexpr int kT = kTwo<BF16>, kStepKeys = kT * kKeys;
+__global__ __launch_bounds__((kWavesOf<FP4> * kWave), 1) void latent_attend_kernel(Params p) {
+    constexpr int kWaves = kWavesOf<FP4>, kThreads = kWaves * kWave;
     constexpr int kParts = BF16 ? 1 : 3;  // bf16 parts of a query value and of a probability
+    constexpr int kGroup = 4;  // product steps that may be mixed: more of them takes more registers
     extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
     __shared__ __attribute__((aligned(16))) float tops[kCols][kWaves], sums[kCols][kWaves];
     __shared__ LatentSeq held[kThreads];
     const int t = threadIdx.x, wave = uniform(t / kWave), lane = t % kWave;
     const int g = lane / 16, c = lane % 16;
     const int latent = FULL ? kLatentMax : p.b.latent, rope = FULL ? kLatentRopeMax : p.b.rope;
-    const int width = latent + rope, dims = latent / 16;
+    const int width = latent + rope;
     const int row_bytes = latent_row_bytes(FP4, latent, rope);
-    uint8_t *keys_lds = lds + wave * kKeyBytes<kT>;
-    uint16_t *query_lds = reinterpret_cast<uint16_t *>(lds + kWaves * kKeyBytes<kT>);
+    uint16_t *query_lds = reinterpret_cast<uint16_t *>(lds);
+
+    // Column c of the identity's two halves: with 32 values of each key as the other operand,
+    // out comes value c, or 16 + c, of every key.
+    u32x4 identity[2];
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            identity[h][i] = g == 2 * h + c / 8 && i == c % 8 / 2 ? c % 2 ? 0x3F800000u : 0x3F80u : 0u;
 
     const int group = blockIdx.x;
-    const Run run = find_run(p, group, held);
+    const Run run = find_run<kWaves>(p, group, held);
     if (t == 0 && !p.parts.tiles) p.parts.records[group].first = -1;
     int left = run.length, offset = run.offset;
     for (int s = run.seq; left > 0 && s < p.b.seqs; ++s, offset = 0) {
@@ -396,17 +426,15 @@ __global__ __launch_bounds__(kThreads, 1) void latent_attend_kernel(Params p) {
             // A key's page, asked for a step before the key; keys that nothing sees are taken from
             // page 0 (and out of the products).
             const int *table = p.b.tables + (long)s * p.b.table_width;
-            const auto page_of = [&](int step, int x, unsigned *in_page) {
-                const unsigned j = (unsigned)step * kStepKeys + x * kKeys + c, at = p.page.quotient(j);
+            const auto page_of = [&](int step, unsigned *in_page) {
+                const unsigned j = (unsigned)step * kStepKeys + c, at = p.page.quotient(j);
                 *in_page = j - at * (unsigned)p.b.page_size;
                 int page = 0;
                 if (step < upto && j < (unsigned)most) page = table[at];
                 return page;
             };
-            unsigned in_page[kT];
-            int page[kT];
-#pragma unroll
-            for (int x = 0; x < kT; ++x) page[x] = page_of(from + wave, x, &in_page[x]);
+            unsigned in_page;
+            int page = page_of(from + wave, &in_page);
 
             // the queries, 8 values a thread and pass
             constexpr int kPieces = (kLatentMax + kLatentRopeMax) / 8;
@@ -430,21 +458,15 @@ __global__ __launch_bounds__(kThreads, 1) void latent_attend_kernel(Params p) {
             float top = -INFINITY, sum = c < used && sees > w.keys ? NAN : 0.0f;
             f32x4 out[kDims];
 
-            const auto key_at = [&](int x, int j) {
-                return reinterpret_cast<u32x4 *>(keys_lds + (x * kKeys + c) * kKeyStride + 2 * dim_of<FP4>(j, g));
-            };
-            Raw<FP4> raw[kT];
-            unsigned bad_pages[kT];
+            Raw<FP4> raw, next;
+            unsigned bad_pages, next_bad;  // keys without a place
             // the keys of the step whose pages are there, and the pages of the step after it
             const auto go_on = [&](int step) {
-#pragma unroll
-                for (int x = 0; x < kT; ++x) {
-                    const bool there = (unsigned)page[x] < (unsigned)p.b.pages;
-                    const long slot = there ? (long)page[x] * p.b.page_size + in_page[x] : 0;
-                    bad_pages[x] = (unsigned)__ballot(!there) & 0xFFFFu;
-                    page[x] = page_of(step + kWaves, x, &in_page[x]);
-                    load_key<FP4, FULL>(raw[x], static_cast<const uint8_t *>(p.b.data) + slot * row_bytes, g, latent, rope);
-                }
+                const bool there = (unsigned)page < (unsigned)p.b.pages;
+                const long slot = there ? (long)page * p.b.page_size + in_page : 0;
+                next_bad = (unsigned)__ballot(!there) & 0xFFFFu;
+                page = page_of(step + kWaves, &in_page);
+                load_key<FP4, FULL>(next, static_cast<const uint8_t *>(p.b.data) + slot * row_bytes, g, latent, rope);
             };
             go_on(from + wave);
             __syncthreads();  // (the tile before is done with them)
@@ -473,92 +495,48 @@ __global__ __launch_bounds__(kThreads, 1) void latent_attend_kernel(Params p) {
 #pragma unroll
             for (int d = 0; d < kDims; ++d) {
                 out[d] = f32x4{0.f, 0.f, 0.f, 0.f};
-                keep(out[d]);
+                if constexpr (kWaves == 4) keep(out[d]);
             }
 
             for (int step = from + wave; step < upto; step += kWaves) {
                 const int key0 = step * kStepKeys;
-                f32x4 score[kT][kParts];
+                raw = next;
+                bad_pages = next_bad;
+                f32x4 score[kParts];
 #pragma unroll
-                for (int x = 0; x < kT; ++x)
+                for (int k = 0; k < kParts; ++k) score[k] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-                    for (int k = 0; k < kParts; ++k) score[x][k] = f32x4{0.f, 0.f, 0.f, 0.f};
-                // (queries come from LDS a few steps ahead of their product)
-                constexpr int kAhead = 3;
-                u32x4 ahead[2][kAhead][kParts];
-                const auto fetch = [&](int j0) {
+                for (int j = 0; j < kAllSteps; ++j) {
+                    const u32x4 v = operand<FP4, FULL>(raw, j, g, latent);
+                    const int at = j < kSteps ? dim_of<FP4>(j, g) : kLatentMax + 32 * (j - kSteps) + 8 * g;
 #pragma unroll
-                    for (int y = 0; y < kAhead; ++y) {
-                        const int j = j0 + y;
-                        const int at = j < kSteps ? dim_of<FP4>(j, g) : kLatentMax + 32 * (j - kSteps) + 8 * g;
-#pragma unroll
-                        for (int k = 0; k < kParts; ++k)
-                            ahead[j0 / kAhead % 2][y][k] =
-                                *reinterpret_cast<const u32x4 *>(query_lds + (k * kCols + c) * kQueryStride + at);
-                    }
-                };
-                fetch(0);
-#pragma unroll
-                for (int j0 = 0; j0 < kAllSteps; j0 += kAhead) {
-                    __builtin_amdgcn_sched_barrier(0);
-                    if (j0 + kAhead < kAllSteps) fetch(j0 + kAhead);
-#pragma unroll
-                    for (int y = 0; y < kAhead; ++y) {
-                        const int j = j0 + y;
-#pragma unroll
-                        for (int x = 0; x < kT; ++x) {
-                            const u32x4 v = operand<FP4, FULL>(raw[x], j, g, latent);
-                            if (j < kSteps) *key_at(x, j) = v;
-#pragma unroll
-                            for (int k = 0; k < kParts; ++k)
-                                score[x][k] = mfma32(v, ahead[j0 / kAhead % 2][y][k], score[x][k]);
-                        }
-                    }
+                    for (int k = 0; k < kParts; ++k)
+                        score[k] = mfma32(v, *reinterpret_cast<const u32x4 *>(query_lds + (k * kCols + c) * kQueryStride + at),
+                                          score[k]);
+                    if (j % kGroup == kGroup - 1) __builtin_amdgcn_sched_barrier(0);
                 }
-                __builtin_amdgcn_sched_barrier(0);
-                unsigned bad_now[kT];
-#pragma unroll
-                for (int x = 0; x < kT; ++x) bad_now[x] = bad_pages[x];
                 if (step + kWaves < upto) go_on(step + kWaves);
-                bool hidden[kT][4], edge = key0 + kStepKeys > least;
-#pragma unroll
-                for (int x = 0; x < kT; ++x) {
-                    if constexpr (!BF16) score[x][0] += score[x][1] + score[x][2];
-                    edge |= bad_now[x] != 0;
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) hidden[x][i] = false;
-                }
-                if (edge) {
+                f32x4 sc = score[0];
+                if constexpr (!BF16) sc += score[1] + score[2];
+                bool hidden[4] = {false, false, false, false};
+                if (bad_pages || key0 + kStepKeys > least) {
                     // Keys that not every column sees, or that have no place: those that a
                     // column does not see must not reach it by 0 * NaN either, so rows that
                     // are not finite (or not there) are taken out of the second product and
                     // make NaN of the scores of the columns that see them.
+                    const bool mine = key0 + c < most;
+                    const unsigned long long which = __ballot(mine && not_finite(raw, g, latent));
+                    const unsigned bad = bad_pages | ((unsigned)(which | which >> 16 | which >> 32 | which >> 48) & 0xFFFFu);
+                    if (!mine || (bad >> c & 1u)) drop(raw);
 #pragma unroll
-                    for (int x = 0; x < kT; ++x) {
-                        const int mine = key0 + x * kKeys + c;
-                        bool odd = false;
-#pragma unroll 1
-                        for (int j = 0; j < kSteps; ++j) odd |= not_finite(*key_at(x, j));
-                        const unsigned long long which = __ballot(odd && mine < most);
-                        const unsigned bad =
-                            bad_now[x] | ((unsigned)(which | which >> 16 | which >> 32 | which >> 48) & 0xFFFFu);
-                        if (mine >= most || (bad >> c & 1u)) {
-#pragma unroll 1
-                            for (int j = 0; j < kSteps; ++j) *key_at(x, j) = u32x4{0, 0, 0, 0};
-                        }
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            if (bad >> (4 * g + i) & 1u) score[x][0][i] = NAN;
-                            hidden[x][i] = key0 + x * kKeys + 4 * g + i >= limit;
-                        }
+                    for (int i = 0; i < 4; ++i) {
+                        if (bad >> (4 * g + i) & 1u) sc[i] = NAN;
+                        hidden[i] = key0 + 4 * g + i >= limit;
                     }
                 }
                 float high = -INFINITY;
 #pragma unroll
-                for (int x = 0; x < kT; ++x)
-#pragma unroll
-                    for (int i = 0; i < 4; ++i)
-                        high = fmaxf(high, hidden[x][i] ? -INFINITY : score[x][0][i] * p.scale);
+                for (int i = 0; i < 4; ++i) high = fmaxf(high, hidden[i] ? -INFINITY : sc[i] * p.scale);
                 if (__any(high > top + kSlack)) {
                     const float next = fmaxf(top, groups_max(high));
                     const float by = top == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(top - next);
@@ -568,74 +546,56 @@ __global__ __launch_bounds__(kThreads, 1) void latent_attend_kernel(Params p) {
                     if (begun) {
 #pragma unroll
                         for (int d = 0; d < kDims; ++d) {
-                            keep(out[d]);
+                            if constexpr (kWaves == 4) keep(out[d]);
                             out[d] *= by;
-                            keep(out[d]);
+                            if constexpr (kWaves == 4) keep(out[d]);
                         }
                     }
                 }
                 const float to = top == -INFINITY ? 0.0f : top;
-                // probabilities, as the second product's operand: keys 4 g .. 4 g + 3 of each
-                union Probs {
-                    s16x4 one[kT];
-                    u32x4 two;
-                } probs[kParts];
+                s16x4 probs[kParts];
+                float prob[4];
 #pragma unroll
-                for (int x = 0; x < kT; ++x) {
-                    float prob[4];
+                for (int i = 0; i < 4; ++i)
+                    prob[i] = hidden[i] ? 0.0f : __builtin_amdgcn_exp2f(fmaf(sc[i], p.scale, -to));
+                if constexpr (BF16) {
+                    bf16x4 r;
 #pragma unroll
-                    for (int i = 0; i < 4; ++i)
-                        prob[i] = hidden[x][i] ? 0.0f : __builtin_amdgcn_exp2f(fmaf(score[x][0][i], p.scale, -to));
-                    if constexpr (BF16) {
-                        bf16x4 r;
+                    for (int i = 0; i < 4; ++i) {
+                        r[i] = (__bf16)prob[i];
+                        sum += (float)r[i];
+                    }
+                    probs[0] = __builtin_bit_cast(s16x4, r);
+                } else {
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            r[i] = (__bf16)prob[i];
-                            sum += (float)r[i];
-                        }
-                        probs[0].one[x] = __builtin_bit_cast(s16x4, r);
-                    } else {
+                    for (int i = 0; i < 4; ++i) {
+                        unsigned part[3];
+                        split3(prob[i], part);
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            unsigned part[3];
-                            split3(prob[i], part);
-#pragma unroll
-                            for (int k = 0; k < kParts; ++k) probs[k].one[x][i] = (short)part[k];
-                            sum += prob[i];
-                        }
+                        for (int k = 0; k < kParts; ++k) probs[k][i] = (short)part[k];
+                        sum += prob[i];
                     }
                 }
-                __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-                const uint8_t *from_lds = keys_lds + (4 * g + c / 4) * kKeyStride + 8 * (c % 4);
-                constexpr int kRead = 8;
-                Probs turned[2][kRead];
-                const auto read = [&](int d0) {
 #pragma unroll
-                    for (int y = 0; y < kRead; ++y)
+                for (int j = 0; j < kSteps; ++j) {
+                    if (!FULL && !FP4 && 32 * j >= latent) continue;
+                    const u32x4 v = operand<FP4, FULL>(raw, j, g, latent);
+                    s16x4 turned[2];
 #pragma unroll
-                        for (int x = 0; x < kT; ++x)
-                            turned[d0 / kRead % 2][y].one[x] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                                (__attribute__((address_space(3))) s16x4 *)(from_lds + x * kKeys * kKeyStride + 32 * (d0 + y)));
-                };
-                read(0);
+                    for (int h = 0; h < 2; ++h) {
+                        const u32x4 x = __builtin_bit_cast(u32x4, mfma32(v, identity[h], f32x4{0.f, 0.f, 0.f, 0.f}));
+                        // (the upper halves: bf16 values are exact)
+                        const unsigned lo = __builtin_amdgcn_perm(x[1], x[0], 0x07060302u);
+                        const unsigned hi = __builtin_amdgcn_perm(x[3], x[2], 0x07060302u);
+                        turned[h] = __builtin_bit_cast(s16x4, (unsigned long)hi << 32 | lo);
+                    }
 #pragma unroll
-                for (int d0 = 0; d0 < kDims; d0 += kRead) {
-                    if (!FULL && d0 >= dims) break;
-                    __builtin_amdgcn_sched_barrier(0);
-                    if (d0 + kRead < kDims) read(d0 + kRead);
+                    for (int k = 0; k < kParts; ++k)
 #pragma unroll
-                    for (int y = 0; y < kRead; ++y)
-#pragma unroll
-                        for (int k = 0; k < kParts; ++k) {
-                            if constexpr (kT == 2)
-                                out[d0 + y] = mfma32(turned[d0 / kRead % 2][y].two, probs[k].two, out[d0 + y]);
-                            else
-                                out[d0 + y] = __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(
-                                    turned[d0 / kRead % 2][y].one[0], probs[k].one[0], out[d0 + y], 0, 0, 0);
-                        }
+                        for (int h = 0; h < 2; ++h)
+                            out[2 * j + h] = __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(turned[h], probs[k], out[2 * j + h], 0, 0, 0);
+                    if (j % kGroup == kGroup - 1) __builtin_amdgcn_sched_barrier(0);
                 }
-                __builtin_amdgcn_sched_barrier(0);
-                __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
             }
 
             // the waves' sums: each to the largest of their maxima, then added
@@ -657,12 +617,16 @@ __global__ __launch_bounds__(kThreads, 1) void latent_attend_kernel(Params p) {
 #pragma unroll
             for (int round = 0; round < kLatentMax / kJoinDims; ++round) {
                 if (!FULL && round * kJoinDims >= latent) break;
-                if (round) __syncthreads();
+                __syncthreads();  // (the queries, or the last round's results, are read)
                 if (wave < busy) {
 #pragma unroll
-                    for (int d = 0; d < kJoinDims / 16; ++d)
-                        *reinterpret_cast<f32x4 *>(results + wave * (kKeyBytes<kT> / 4) + c * kJoinStride + 16 * d + 4 * g) =
+                    for (int d = 0; d < kJoinDims / 16; ++d) {
+                        // rows 4 g .. 4 g + 3 of out[2 j + h] are 4 latent values of lane group
+                        // 2 h + g / 2 at step j
+                        const int at = dim_of<FP4>(d / 2, 2 * (d % 2) + g / 2) + 4 * (g % 2);
+                        *reinterpret_cast<f32x4 *>(results + wave * (kJoinBytes / 4) + c * kJoinDims + 4 * ((at / 4) ^ c)) =
                             out[round * (kJoinDims / 16) + d];
+                    }
                 }
                 __syncthreads();
                 if (round == 0) {
@@ -683,7 +647,8 @@ __global__ __launch_bounds__(kThreads, 1) void latent_attend_kernel(Params p) {
                     if (x >= busy) break;
 #pragma unroll
                     for (int k = 0; k < kPasses; ++k)
-                        v[k] += by[x] * load_f4(results + x * (kKeyBytes<kT> / 4) + col * kJoinStride + at + 4 * kColThreads * k);
+                        v[k] += by[x] * load_f4(results + x * (kJoinBytes / 4) + col * kJoinDims +
+                                                4 * ((at / 4 + kColThreads * k) ^ col));
                 }
 #pragma unroll
                 for (int k = 0; k < kPasses; ++k) {
@@ -785,7 +750,8 @@ template <bool BF16> __global__ __launch_bounds__(kTeam *kMaxTeams) void latent_
 }
 
 template <bool FP4, bool BF16, bool FULL> int launch(const Params &p, hipStream_t stream) {
-    constexpr int bytes = kWaves * kKeyBytes<kTwo<BF16>> + kQueryBytes<BF16>;
+    constexpr int kThreads = kWavesOf<FP4> * kWave;
+    constexpr int bytes = kLdsBytes<FP4, BF16>;
     const auto kernel = latent_attend_kernel<FP4, BF16, FULL>;
     static const bool ok = hipFuncSetAttribute(reinterpret_cast<const void *>(kernel),
                                                hipFuncAttributeMaxDynamicSharedMemorySize, bytes) == hipSuccess;
@@ -818,9 +784,7 @@ int latent_attend(const MlkLatentBatch &b, const LatentAttend &p, int cu_count, 
     // units of more keys where there could be 2^31 of them (a tile has at least a column)
     const long tiles = (long)p.rows * p.heads / kCols + b.seqs;
     a.parts.tiles = tiles <= kMaxTileRecords ? (int)tiles : 0;
-    a.step = p.bf16 ? 5 : 4;
-    static_assert(kTwo<true> * kKeys == 32 && kTwo<false> * kKeys == 16, "a step's keys");
-    for (a.shift = 0; tiles * (((a.keys - 1) >> (a.step + a.shift)) + 1) >= 0x7FFFFFFF; ++a.shift) {}
+    for (a.shift = 0; tiles * (((a.keys - 1) >> (kStepShift + a.shift)) + 1) >= 0x7FFFFFFF; ++a.shift) {}
     a.page = Divisor::of((unsigned)b.page_size);
     a.head = Divisor::of((unsigned)p.heads);
     uint8_t *at = static_cast<uint8_t *>(p.workspace);

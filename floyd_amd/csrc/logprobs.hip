@@ -9,9 +9,13 @@
 // bytes of logits at a time; those among which the piece's maximum may be are added one by
 // one, since next to its 1 what makes a likely token's log p would be lost.
 //
-// The top k: the k-th largest of the threads' own largest is a bound that at least k values
-// reach, and only values of k threads do, so what is left to be put in order is few however
+// The top k: the k-th largest of a wave's threads' own largest is a bound that at least k
+// values reach, and only k threads' values, so what is left to be put in order is few however
 // the values lie.  (value, index) are compared as one whole number, all different.
+//
+// exp(d) is the hardware's 2^(d log2 e): d and the product are rounded to f32, which puts a
+// term off by 2.1 |d| 2^-24 of itself.  That and the rest is 12 operations a value, what
+// the vector units do of bf16 logits in the time that the memory takes to bring them.
 #include "bf16.h"
 #include "latent.h"
 #include "mlh_device.h"
@@ -47,10 +51,24 @@ struct Stats {
     float pad;
 };
 
+// Reductions over a wave without LDS (a step through it takes 100 cycles and more): lane 63
+// has the sum over the wave, as an ordinary value in every lane.
+template <int CTRL, int ROWS> __device__ __forceinline__ double dpp_add(double v) {
+    const long long bits = __double_as_longlong(v);
+    const int lo = __builtin_amdgcn_update_dpp(0, (int)bits, CTRL, ROWS, 0xF, false);
+    const int hi = __builtin_amdgcn_update_dpp(0, (int)(bits >> 32), CTRL, ROWS, 0xF, false);
+    return v + __longlong_as_double((long long)hi << 32 | (unsigned)lo);
+}
 __device__ __forceinline__ double wave_sum64(double v) {
-#pragma unroll
-    for (int o = 32; o >= 1; o >>= 1) v += __shfl_xor(v, o, kWave);
-    return v;
+    v = dpp_add<0x111, 0xF>(v);  // row_shr:1, 2, 4, 8
+    v = dpp_add<0x112, 0xF>(v);
+    v = dpp_add<0x114, 0xF>(v);
+    v = dpp_add<0x118, 0xF>(v);
+    v = dpp_add<0x142, 0xA>(v);  // row_bcast:15, 31
+    v = dpp_add<0x143, 0xC>(v);
+    const long long bits = __double_as_longlong(v);
+    const unsigned lo = __builtin_amdgcn_readlane((int)bits, 63);
+    return __longlong_as_double((long long)__builtin_amdgcn_readlane((int)(bits >> 32), 63) << 32 | lo);
 }
 
 // The largest `top` ranks among `n` candidates in LDS, in order, into out[0 .. top).
@@ -64,17 +82,23 @@ __device__ __forceinline__ void put_in_order(const Rank *found, int n, int top, 
     for (int i = n + threadIdx.x; i < top; i += kThreads) out[i] = 0;
 }
 
-// The `top`-th largest of the threads' ranks (0 where fewer have one).
-__device__ __forceinline__ Rank bound_of(Rank mine, int top, Rank *all, Rank *bound) {
+// A bound that at least `top` of the workgroup's values reach, if it has as many, and values
+// of at most `top` threads of each wave: the largest of the waves' `top`-th largest threads
+// (0 where fewer than `top` threads of each have a rank).
+__device__ __forceinline__ Rank bound_of(Rank mine, int top, Rank *all, Rank *bounds) {
+    const int wave = threadIdx.x / kWave;
     all[threadIdx.x] = mine;
-    if (threadIdx.x == 0) *bound = 0;
-    __syncthreads();
+    if (threadIdx.x % kWave == 0) bounds[wave] = 0;
+    const Rank *its = all + wave * kWave;
     int above = 0;
 #pragma unroll 16
-    for (int j = 0; j < kThreads; ++j) above += all[j] > mine;
-    if (mine && above == top - 1) *bound = mine;
+    for (int j = 0; j < kWave; ++j) above += its[j] > mine;
+    if (mine && above == top - 1) bounds[wave] = mine;
     __syncthreads();
-    return *bound;
+    Rank bound = bounds[0];
+#pragma unroll
+    for (int w = 1; w < kWaves; ++w) bound = bounds[w] > bound ? bounds[w] : bound;
+    return bound;
 }
 
 __device__ __forceinline__ float from_bits(unsigned w, int half) {
@@ -107,8 +131,8 @@ __global__ __launch_bounds__(kThreads) void logprobs_piece_kernel(TokenLogprobs 
     constexpr int kVec = BF16 ? 8 : 4, kVecs = N / kVec;
     __shared__ float tops[kWaves];
     __shared__ double sums[kWaves][2];
-    __shared__ Rank all[TOP ? kThreads : 1], found[TOP ? kLogprobsMaxTop * N : 1], sorted[TOP ? kLogprobsMaxTop : 1];
-    __shared__ Rank bound;
+    __shared__ Rank all[TOP ? kThreads : 1], found[TOP ? kWaves * kLogprobsMaxTop * N : 1], sorted[TOP ? kLogprobsMaxTop : 1];
+    __shared__ Rank bounds[kWaves];
     __shared__ int count;
     const int t = threadIdx.x, wave = t / kWave, lane = t % kWave;
     const int r = blockIdx.x / pieces, piece = blockIdx.x - r * pieces;
@@ -147,22 +171,22 @@ __global__ __launch_bounds__(kThreads) void logprobs_piece_kernel(TokenLogprobs 
         for (int x = 0; x < kVec; ++x) vec_top[k] = fmaxf(vec_top[k], value(k, x));
         mine = fmaxf(mine, vec_top[k]);
     }
-    const float wave_top = wave_max(mine);
+    const float wave_top = dpp_wave_max(mine);
     if (lane == 0) tops[wave] = wave_top;
     if (TOP && t == 0) count = 0;
     __syncthreads();
     const float top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
+    const float base_top = top == -INFINITY ? 0.0f : top;  // (of a piece with nothing above)
     double sum = 0.0, mean = 0.0;
 #pragma unroll
     for (int k = 0; k < kVecs; ++k) {
         float e[kVec], s = 0.0f, m = 0.0f;
 #pragma unroll
         for (int x = 0; x < kVec; ++x) {
-            const float d = value(k, x) - top;
-            e[x] = expf(d);
-            // (-inf has no part; a piece of nothing else has top -inf and d NaN)
-            if (value(k, x) == -INFINITY) e[x] = 0.0f;
-            else m += e[x] * d;
+            // (a masked value's 0 times infinity is to be 0; NaN stays NaN, by e)
+            const float d = value(k, x) - base_top;
+            e[x] = __builtin_amdgcn_exp2f(d * 1.44269504f);
+            m = fmaf(e[x], fmaxf(d, -1000.0f), m);
             s += e[x];
         }
         if (vec_top[k] - top > -0.7f) {
@@ -187,7 +211,7 @@ __global__ __launch_bounds__(kThreads) void logprobs_piece_kernel(TokenLogprobs 
 #pragma unroll
             for (int x = kVec - 1; x >= 0; --x)
                 if (value(k, x) == mine && first(k) + x < p.vocab) at = first(k) + x, any = true;
-        const Rank least = bound_of(any ? rank_of(mine, at) : 0, p.top, all, &bound);
+        const Rank least = bound_of(any ? rank_of(mine, at) : 0, p.top, all, bounds);
 #pragma unroll
         for (int k = 0; k < kVecs; ++k) {
             if (rank_of(vec_top[k], first(k)) < least) continue;
@@ -219,13 +243,18 @@ __global__ __launch_bounds__(kThreads) void logprobs_join_kernel(TokenLogprobs p
     __shared__ double sums[kWaves][2];
     __shared__ Rank all[TOP ? kThreads : 1], sorted[TOP ? kLogprobsMaxTop : 1];
     extern __shared__ __attribute__((aligned(16))) Rank found[];
-    __shared__ Rank bound;
+    __shared__ Rank bounds[kWaves];
     __shared__ int count;
     const int t = threadIdx.x, wave = t / kWave, lane = t % kWave, r = blockIdx.x;
     const Stats *its = stats + (long)r * pieces;
+    const Rank *from = ranks + (long)r * pieces * p.top;
+    const int n = pieces * p.top;
+    Rank best = 0;
+    if constexpr (TOP)
+        for (int i = t; i < n; i += kThreads) best = from[i] > best ? from[i] : best;
     float mine = -INFINITY;
     for (int i = t; i < pieces; i += kThreads) mine = fmaxf(mine, its[i].top);
-    mine = wave_max(mine);
+    mine = dpp_wave_max(mine);
     if (lane == 0) tops[wave] = mine;
     if (TOP && t == 0) count = 0;
     __syncthreads();
@@ -251,11 +280,7 @@ __global__ __launch_bounds__(kThreads) void logprobs_join_kernel(TokenLogprobs p
     if (top == -INFINITY) sum = NAN;
     if (t == 0) finish(p, r, top, sum, mean);
     if constexpr (TOP) {
-        const Rank *from = ranks + (long)r * pieces * p.top;
-        const int n = pieces * p.top;
-        Rank best = 0;
-        for (int i = t; i < n; i += kThreads) best = from[i] > best ? from[i] : best;
-        const Rank least = bound_of(best, p.top, all, &bound);
+        const Rank least = bound_of(best, p.top, all, bounds);
         for (int i = t; i < n; i += kThreads) {
             const Rank rank = from[i];
             if (rank && rank >= least) found[atomicAdd(&count, 1)] = rank;
@@ -280,8 +305,9 @@ template <bool BF16, bool TOP, int N> int launch(const TokenLogprobs &p, hipStre
     logprobs_piece_kernel<BF16, TOP, N><<<(unsigned)blocks, kThreads, 0, stream>>>(p, pieces, stats, ranks);
     if (hipGetLastError() != hipSuccess) return kErrLaunch;
     if (pieces == 1) return kOk;
-    // ranks of the `top` threads that reach the bound
-    const size_t found = TOP ? sizeof(Rank) * p.top * (((size_t)pieces * p.top - 1) / kThreads + 1) : 0;
+    // ranks of the threads that reach the bound: at most `top` of a wave, and all of n
+    const size_t n = (size_t)pieces * p.top, reach = kWaves * p.top * ((n - 1) / kThreads + 1);
+    const size_t found = TOP ? sizeof(Rank) * (n < reach ? n : reach) : 0;
     logprobs_join_kernel<TOP><<<p.rows, kThreads, found, stream>>>(p, pieces, stats, ranks);
     return hipGetLastError() == hipSuccess ? kOk : kErrLaunch;
 }
