@@ -27,14 +27,24 @@ template <bool BF16> __device__ __forceinline__ double value(typename Elem<BF16>
     if constexpr (BF16) return (double)bf16_value(v);
     else return (double)v;
 }
+// By way of f32, which the compiler is not to skip: its conversion of that is one instruction
+// for two values (NaN stays NaN), of 64 bits a dozen.
+__device__ __forceinline__ uint16_t to_bf16(double v) {
+    float f = (float)v;
+    asm("" : "+v"(f));
+    return __builtin_bit_cast(uint16_t, (__bf16)f);
+}
 template <bool BF16> __device__ __forceinline__ void store(typename Elem<BF16>::type *p, double v) {
-    if constexpr (BF16) *p = (uint16_t)bf16_bits((float)v);
+    if constexpr (BF16) *p = to_bf16(v);
     else *p = (float)v;
 }
-
-__device__ __forceinline__ double wave_sum64(double v) {
-#pragma unroll
-    for (int o = 32; o >= 1; o >>= 1) v += __shfl_xor(v, o, kWave);
+// Two neighbours, at any address of their type.
+template <bool BF16> struct Pair {
+    typename Elem<BF16>::type x, y;
+};
+template <bool BF16> __device__ __forceinline__ Pair<BF16> load_pair(const typename Elem<BF16>::type *p) {
+    Pair<BF16> v;
+    __builtin_memcpy(&v, p, sizeof(v));
     return v;
 }
 
@@ -65,92 +75,159 @@ __device__ __forceinline__ bool place_of_row(const MlkLatentBatch &b, int r, int
     return true;
 }
 
+// sin and cos of an angle below 2^32 in magnitude, to a few last places of 1: the nearest
+// multiple of pi / 2 is taken off in two parts (products and differences exact by fma), and
+// what is left, at most pi / 4, goes into the power series up to x^17 and x^16.
+__device__ __forceinline__ void turn_of(double angle, double *sine, double *cosine) {
+    constexpr double kHalfPi = 0x1.921fb54442d18p+0, kHalfPiRest = 0x1.1a62633145c07p-54;
+    const double k = rint(angle * 0x1.45f306dc9c883p-1);
+    const double x = fma(-k, kHalfPiRest, fma(-k, kHalfPi, angle)), y = x * x;
+    double s = 1.0 / 355687428096000.0, c = 1.0 / 20922789888000.0;
+    s = fma(s, y, -1.0 / 1307674368000.0);
+    s = fma(s, y, 1.0 / 6227020800.0);
+    s = fma(s, y, -1.0 / 39916800.0);
+    s = fma(s, y, 1.0 / 362880.0);
+    s = fma(s, y, -1.0 / 5040.0);
+    s = fma(s, y, 1.0 / 120.0);
+    s = fma(s, y, -1.0 / 6.0);
+    s = fma(s * y, x, x);
+    c = fma(c, y, -1.0 / 87178291200.0);
+    c = fma(c, y, 1.0 / 479001600.0);
+    c = fma(c, y, -1.0 / 3628800.0);
+    c = fma(c, y, 1.0 / 40320.0);
+    c = fma(c, y, -1.0 / 720.0);
+    c = fma(c, y, 1.0 / 24.0);
+    c = fma(c, y, -0.5);
+    c = fma(c, y, 1.0);
+    const int quarter = (int)((long long)k & 3);
+    const double a = quarter & 1 ? c : s, b = quarter & 1 ? s : c;
+    *sine = quarter & 2 ? -a : a;
+    *cosine = (quarter + 1) & 2 ? -b : b;
+}
+
 // 2^e of a double, e in its normal range.
 __device__ __forceinline__ double power2(int e) {
     return __longlong_as_double((long long)(e + 1023) << 52);
 }
 
-// The e2m1 code nearest to v (|v| <= 6), ties to even.
-__device__ __forceinline__ unsigned fp4_code(double v) {
-    const double a = fabs(v);
-    const unsigned m = (a > 0.25) + (a >= 0.75) + (a > 1.25) + (a >= 1.75) + (a > 2.5) + (a >= 3.5) +
-                       (a > 5.0);
-    return m | (v < 0.0 ? 8u : 0u);
+// A value cut off to f32 with its last bit set where that left something out: rounded to fewer
+// bits it goes where the value goes.
+__device__ __forceinline__ float to_odd(double v) {
+    const float f = (float)v;
+    const double back = (double)f;
+    unsigned u = __float_as_uint(f);
+    if (fabs(back) > fabs(v)) --u;
+    return __uint_as_float(back != v ? u | 1u : u);
+}
+// The e2m1 codes nearest to two values of at most 6 in magnitude, ties to even.
+__device__ __forceinline__ uint8_t fp4_codes(double v0, double v1) {
+    return (uint8_t)__builtin_amdgcn_cvt_scalef32_pk_fp4_f32(0u, to_odd(v0), to_odd(v1), 1.0f, 0);
 }
 
-// One token row a workgroup.
+// The largest of a row of 16 lanes.
+template <int CTRL> __device__ __forceinline__ unsigned dpp_max(unsigned v) {
+    const unsigned other = __builtin_amdgcn_update_dpp(0, v, CTRL, 0xF, 0xF, true);
+    return other > v ? other : v;
+}
+__device__ __forceinline__ unsigned row_max(unsigned v) {
+    v = dpp_max<0xB1>(v);   // quad_perm [1,0,3,2]
+    v = dpp_max<0x4E>(v);   // quad_perm [2,3,0,1]
+    v = dpp_max<0x141>(v);  // row_half_mirror
+    return dpp_max<0x140>(v);  // row_mirror
+}
+
+// One token row a workgroup.  What it reads of the row is asked for at once, beside the way to
+// its place (starts, then length and table, a microsecond each).  Queries: 32 threads for the
+// pairs of a head, 8 heads a pass.
+constexpr int kPairLanes = kLatentRopeMax / 2, kPassHeads = kThreads / kPairLanes;
+constexpr int kTurns = 2;  // passes on their way at once
 template <bool BF16, bool FP4>
 __global__ __launch_bounds__(kThreads) void latent_append_kernel(MlkLatentBatch b, LatentAppend p) {
     using T = typename Elem<BF16>::type;
     __shared__ double part[kWaves];
     __shared__ double turn[kLatentRopeMax / 2][2];
     const int r = blockIdx.x, t = threadIdx.x;
-    const int latent = b.latent, half = b.rope / 2;
-    // thread t: latent values 2t and 2t + 1
+    const int latent = b.latent, half = b.rope / 2, width = latent + b.rope;
+    // thread t: latent values 2t and 2t + 1, rope pair t
     const T *kv = static_cast<const T *>(p.kv) + (long)r * p.kv_stride;
-    const bool has = 2 * t < latent;
-    double c0 = has ? value<BF16>(kv[2 * t]) : 0.0, c1 = has ? value<BF16>(kv[2 * t + 1]) : 0.0;
+    const bool has = 2 * t < latent, turns = t < half;
+    const auto latent_pair = load_pair<BF16>(kv + (has ? 2 * t : 0));
+    const auto rope_pair = load_pair<BF16>(kv + (turns ? latent + 2 * t : 0));
+    const float w0 = p.norm_w && has ? p.norm_w[2 * t] : 1.0f, w1 = p.norm_w && has ? p.norm_w[2 * t + 1] : 1.0f;
+    const float freq = p.inv_freq[turns ? t : 0];
+    const int lane_pair = t % kPairLanes, head0 = t / kPairLanes;
+    const int heads = p.query && lane_pair < half ? p.heads : 0;
+    const T *query = static_cast<const T *>(p.query) + (long)r * p.query_stride + p.head_width - b.rope + 2 * lane_pair;
+    Pair<BF16> asked[kTurns];
+#pragma unroll
+    for (int k = 0; k < kTurns; ++k) {
+        asked[k] = {};
+        const int h = head0 + k * kPassHeads;
+        if (h < heads) asked[k] = load_pair<BF16>(query + (long)h * p.head_width);
+    }
     int position;
     long slot;
     if (!place_of_row(b, r, p.rows, &position, &slot) || position < 0) return;
-    if (t < half) {
-        double sn, cs;
-        sincos((double)position * (double)p.inv_freq[t], &sn, &cs);
+    double cs = 1.0, sn = 0.0;
+    if (turns) {
+        turn_of((double)position * (double)freq, &sn, &cs);
         turn[t][0] = cs;
         turn[t][1] = sn;
     }
-    const double squares = wave_sum64(c0 * c0 + c1 * c1);
+    double c0 = has ? value<BF16>(latent_pair.x) : 0.0, c1 = has ? value<BF16>(latent_pair.y) : 0.0;
+    const double squares = dpp_wave_sum(c0 * c0 + c1 * c1);
     if (t % kWave == 0) part[t / kWave] = squares;
     __syncthreads();
-    if (p.query) {
-        const T *query = static_cast<const T *>(p.query) + (long)r * p.query_stride;
-        T *q = static_cast<T *>(p.q) + (long)r * p.heads * (latent + b.rope);
-        for (int j = t; j < p.heads * half; j += kThreads) {
-            const int h = j / half, i = j - h * half;
-            const T *in = query + (long)(h + 1) * p.head_width - b.rope + 2 * i;
-            const double x = value<BF16>(in[0]), y = value<BF16>(in[1]);
-            T *out = q + (long)h * (latent + b.rope) + latent + i;
-            store<BF16>(out, x * turn[i][0] - y * turn[i][1]);
-            store<BF16>(out + half, y * turn[i][0] + x * turn[i][1]);
-        }
+    if (heads) {
+        const double qc = turn[lane_pair][0], qs = turn[lane_pair][1];
+        T *out = static_cast<T *>(p.q) + (long)r * p.heads * width + latent + lane_pair;
+        const auto turn_query = [&](int h, Pair<BF16> q) {
+            const double x = value<BF16>(q.x), y = value<BF16>(q.y);
+            store<BF16>(out + (long)h * width, x * qc - y * qs);
+            store<BF16>(out + (long)h * width + half, y * qc + x * qs);
+        };
+#pragma unroll
+        for (int k = 0; k < kTurns; ++k)
+            if (head0 + k * kPassHeads < heads) turn_query(head0 + k * kPassHeads, asked[k]);
+        for (int h = head0 + kTurns * kPassHeads; h < heads; h += kPassHeads)
+            turn_query(h, load_pair<BF16>(query + (long)h * p.head_width));
     }
     if (slot < 0) return;
     uint8_t *row = static_cast<uint8_t *>(b.data) + slot * latent_row_bytes(FP4, latent, b.rope);
     if (p.norm_w && has) {
         const double total = (part[0] + part[1]) + (part[2] + part[3]);
-        const double inv = 1.0 / sqrt(total / latent + (double)p.eps);
-        c0 = c0 * inv * (double)p.norm_w[2 * t];
-        c1 = c1 * inv * (double)p.norm_w[2 * t + 1];
+        const double inv = rsqrt(total / latent + (double)p.eps);
+        c0 = c0 * inv * (double)w0;
+        c1 = c1 * inv * (double)w1;
     }
     if constexpr (FP4) {
-        // the 16 threads of 32 values; magnitudes in the order of their bits, NaN above all
-        const long long a0 = __double_as_longlong(fabs(c0)), a1 = __double_as_longlong(fabs(c1));
-        long long top = a0 > a1 ? a0 : a1;
-#pragma unroll
-        for (int o = 8; o >= 1; o >>= 1) {
-            const long long other = __shfl_xor(top, o, kWave);
-            top = other > top ? other : top;
-        }
-        const int exp = (int)(top >> 52) - 1023;  // top = 1.m * 2^exp <= 6 * 2^e = 1.5 * 2^(e + 2)
-        const bool above = (top & 0xFFFFFFFFFFFFFLL) > 0x8000000000000LL;
+        // the 16 threads of 32 values.  Of a magnitude the upper half of its bits is enough, the
+        // last one set if a lower one is: they are in the order of the magnitudes, NaN above
+        // all, and show a mantissa of 1.5 and more than that apart.
+        const auto upper = [](double v) {
+            const unsigned long long u = __double_as_longlong(fabs(v));
+            return (unsigned)(u >> 32) | ((unsigned)u != 0u ? 1u : 0u);
+        };
+        const unsigned u0 = upper(c0), u1 = upper(c1), top = row_max(u0 > u1 ? u0 : u1);
+        const int exp = (int)(top >> 20) - 1023;  // top = 1.m * 2^exp <= 6 * 2^e = 1.5 * 2^(e + 2)
         const bool bad = exp >= 127;
-        const int least = exp - (above ? 1 : 2);
+        const int least = exp - ((top & 0xFFFFFu) > 0x80000u ? 1 : 2);
         const int e = bad ? 0 : least < kFp4LeastExp ? kFp4LeastExp : least;
         const double inv = power2(-e);
         if (has) {
-            row[t] = bad ? (uint8_t)0 : (uint8_t)(fp4_code(c0 * inv) | (fp4_code(c1 * inv) << 4));
+            row[t] = bad ? (uint8_t)0 : fp4_codes(c0 * inv, c1 * inv);
             const int g = t / (kFp4Group / 2);
             if (t % (kFp4Group / 2) == 0)
                 row[latent / 2 + 4 * (g % 4) + g / 4] = (uint8_t)(bad ? 255 : e + kFp4Bias);
         }
     } else if (has) {
-        reinterpret_cast<unsigned *>(row)[t] = bf16_bits((float)c0) | (bf16_bits((float)c1) << 16);
+        reinterpret_cast<unsigned *>(row)[t] = to_bf16(c0) | (unsigned)to_bf16(c1) << 16;
     }
-    if (t < half) {
-        const double x = value<BF16>(kv[latent + 2 * t]), y = value<BF16>(kv[latent + 2 * t + 1]);
+    if (turns) {
+        const double x = value<BF16>(rope_pair.x), y = value<BF16>(rope_pair.y);
         uint16_t *rope = reinterpret_cast<uint16_t *>(row + latent_part_bytes(FP4, latent));
-        rope[t] = (uint16_t)bf16_bits((float)(x * turn[t][0] - y * turn[t][1]));
-        rope[half + t] = (uint16_t)bf16_bits((float)(y * turn[t][0] + x * turn[t][1]));
+        rope[t] = to_bf16(x * cs - y * sn);
+        rope[half + t] = to_bf16(y * cs + x * sn);
     }
 }
 

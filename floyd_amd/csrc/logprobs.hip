@@ -51,26 +51,6 @@ struct Stats {
     float pad;
 };
 
-// Reductions over a wave without LDS (a step through it takes 100 cycles and more): lane 63
-// has the sum over the wave, as an ordinary value in every lane.
-template <int CTRL, int ROWS> __device__ __forceinline__ double dpp_add(double v) {
-    const long long bits = __double_as_longlong(v);
-    const int lo = __builtin_amdgcn_update_dpp(0, (int)bits, CTRL, ROWS, 0xF, false);
-    const int hi = __builtin_amdgcn_update_dpp(0, (int)(bits >> 32), CTRL, ROWS, 0xF, false);
-    return v + __longlong_as_double((long long)hi << 32 | (unsigned)lo);
-}
-__device__ __forceinline__ double wave_sum64(double v) {
-    v = dpp_add<0x111, 0xF>(v);  // row_shr:1, 2, 4, 8
-    v = dpp_add<0x112, 0xF>(v);
-    v = dpp_add<0x114, 0xF>(v);
-    v = dpp_add<0x118, 0xF>(v);
-    v = dpp_add<0x142, 0xA>(v);  // row_bcast:15, 31
-    v = dpp_add<0x143, 0xC>(v);
-    const long long bits = __double_as_longlong(v);
-    const unsigned lo = __builtin_amdgcn_readlane((int)bits, 63);
-    return __longlong_as_double((long long)__builtin_amdgcn_readlane((int)(bits >> 32), 63) << 32 | lo);
-}
-
 // The largest `top` ranks among `n` candidates in LDS, in order, into out[0 .. top).
 __device__ __forceinline__ void put_in_order(const Rank *found, int n, int top, Rank *out) {
     for (int i = threadIdx.x; i < n; i += kThreads) {
@@ -197,8 +177,8 @@ __global__ __launch_bounds__(kThreads) void logprobs_piece_kernel(TokenLogprobs 
         }
         mean += (double)m;
     }
-    sum = wave_sum64(sum);
-    mean = wave_sum64(mean);
+    sum = dpp_wave_sum(sum);
+    mean = dpp_wave_sum(mean);
     if (lane == 0) sums[wave][0] = sum, sums[wave][1] = mean;
     __syncthreads();
     sum = (sums[0][0] + sums[1][0]) + (sums[2][0] + sums[3][0]);
@@ -271,8 +251,8 @@ __global__ __launch_bounds__(kThreads) void logprobs_join_kernel(TokenLogprobs p
         sum += by * s.sum;
         mean += by == 0.0 ? 0.0 : by * (s.mean + off * s.sum);
     }
-    sum = wave_sum64(sum);
-    mean = wave_sum64(mean);
+    sum = dpp_wave_sum(sum);
+    mean = dpp_wave_sum(mean);
     if (lane == 0) sums[wave][0] = sum, sums[wave][1] = mean;
     __syncthreads();
     sum = (sums[0][0] + sums[1][0]) + (sums[2][0] + sums[3][0]);

@@ -75,6 +75,25 @@ __device__ __forceinline__ float dpp_wave_max(float v) {
 }
 #undef MLH_DPP
 
+// The same sum in 64 bits.
+template <int CTRL, int ROWS> __device__ __forceinline__ double dpp_add(double v) {
+    const long long bits = __double_as_longlong(v);
+    const int lo = __builtin_amdgcn_update_dpp(0, (int)bits, CTRL, ROWS, 0xF, false);
+    const int hi = __builtin_amdgcn_update_dpp(0, (int)(bits >> 32), CTRL, ROWS, 0xF, false);
+    return v + __longlong_as_double((long long)hi << 32 | (unsigned)lo);
+}
+__device__ __forceinline__ double dpp_wave_sum(double v) {
+    v = dpp_add<0x111, 0xF>(v);  // row_shr:1, 2, 4, 8
+    v = dpp_add<0x112, 0xF>(v);
+    v = dpp_add<0x114, 0xF>(v);
+    v = dpp_add<0x118, 0xF>(v);
+    v = dpp_add<0x142, 0xA>(v);  // row_bcast:15, 31
+    v = dpp_add<0x143, 0xC>(v);
+    const long long bits = __double_as_longlong(v);
+    const unsigned lo = __builtin_amdgcn_readlane((int)bits, 63);
+    return __longlong_as_double((long long)__builtin_amdgcn_readlane((int)(bits >> 32), 63) << 32 | lo);
+}
+
 __device__ __forceinline__ float wave_max(float v) {
 #pragma unroll
     for (int o = 32; o >= 1; o >>= 1) v = fmaxf(v, __shfl_xor(v, o, kWave));

@@ -237,8 +237,9 @@ size_t mlk_latent_row_bytes(int type, int latent, int rope);
 /* Writes each token row's key: kv [rows, kv_stride] of `type` (MLK_F32 or
  * MLK_BF16) holds latent values, of which RMSNorm(...) * norm_w is cached (the
  * values themselves where norm_w is NULL), then rope values, rotated by the
- * key's position p: with a = p * inv_freq[i] pair (2i, 2i + 1) becomes values i and
- * i + rope / 2, x cos a - y sin a and y cos a + x sin a.  With `query` != NULL
+ * key's position p: with a = p * inv_freq[i] (below 2^32 in magnitude) pair
+ * (2i, 2i + 1) becomes values i and i + rope / 2, x cos a - y sin a and
+ * y cos a + x sin a.  With `query` != NULL
  * the last rope values of each head of query [rows, query_stride] (heads of
  * head_width values) are rotated likewise into the last rope values of each head
  * of q [rows, heads, latent + rope].  Strides are in values.
