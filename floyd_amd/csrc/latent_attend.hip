@@ -26,28 +26,21 @@
 // What runs once costs its instructions' way from memory, about 4 cycles a byte: loops are
 // entered a step early rather than with a copy of their loads before them, and unrolled
 // only where registers are counted.
-#include "bf16.h"
-#include "latent.h"
-#include "mlh_device.h"
-#include "mlh_host.h"
+#include "latent_attend.h"
 
 namespace mlh {
+
+using namespace latent_attention;
 
 namespace {
 
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));
-typedef u32x4 u32x4_any __attribute__((aligned(2)));
 
-constexpr int kCols = 16;       // (row, head) pairs of a tile
-constexpr int kStepKeys = 16, kStepShift = 4;  // keys of a wave's step
-constexpr int kLeastShift = 6;  // log2 of the keys that a workgroup takes, where there are as many
-constexpr int kSteps = kLatentMax / 32;          // product steps over a latent row
-constexpr int kRopeSteps = kLatentRopeMax / 32;  // and over a rope row
+constexpr int kCols = Narrow::kCols, kStepKeys = Narrow::kStepKeys;
 constexpr int kAllSteps = kSteps + kRopeSteps;
-constexpr int kDims = kLatentMax / 16;           // 16-value tiles of a latent row
-constexpr int kMaxGroups = 512;                  // workgroups of a launch
+constexpr int kDims = kLatentMax / 16;  // 16-value tiles of a latent row
 
 // Waves of a workgroup, one workgroup a CU.  4-bit keys leave a wave in 256 registers, for two
 // waves on a SIMD; of bf16 keys, 72 registers a step, two steps are held by one.
@@ -62,265 +55,6 @@ constexpr int kJoinDims = 256;
 constexpr int kJoinBytes = kCols * kJoinDims * 4;  // of a wave
 template <bool FP4, bool BF16> constexpr int kLdsBytes =
     kQueryBytes<BF16> > kWavesOf<FP4> * kJoinBytes ? kQueryBytes<BF16> : kWavesOf<FP4> * kJoinBytes;
-
-// What latent_join_kernel has to know of a tile, told by the workgroup that ends it: its
-// sequence and number in it, and the workgroups that its units fell to (-1: to one, there is
-// nothing to join).  Where a batch has few tiles a record belongs to the tile: of sequence s,
-// the tile that begins with pair b of all (row, head) pairs has record b / 16 + s.  Those
-// are different, but not every record has a tile, and one that has none tells of an
-// earlier call's.  Else a record belongs to the workgroup, which ends at most one tile that
-// another one began.
-struct __attribute__((aligned(16))) Record {
-    int seq, tile, first, last;
-};
-constexpr int kMaxTileRecords = 2048;
-
-// Partial sums of tiles: slot 2w holds the tile that workgroup w found begun, slot 2w + 1
-// the one that it left unfinished.
-struct Parts {
-    float *sums;    // [2 groups][kCols][kLatentMax]
-    float *stats;   // [2 groups][2][kCols] maxima, then sums
-    Record *records;
-    int tiles;      // records of tiles, else 0: of workgroups
-};
-constexpr size_t kSumsBytes = 2L * kMaxGroups * kCols * kLatentMax * 4;
-constexpr size_t kStatsBytes = 2L * kMaxGroups * 2 * kCols * 4;
-constexpr size_t kRecordBytes = (size_t)kMaxTileRecords * sizeof(Record);
-static_assert(kMaxGroups <= kMaxTileRecords, "records of workgroups");
-
-// n / d of n below 2^31 by a product: m is the whole number above 2^(31 + l) / d with l the
-// least for which 2^l >= d.
-struct Divisor {
-    unsigned m, shift;
-    __host__ static Divisor of(unsigned d) {
-        unsigned l = 0;
-        while ((1ull << l) < d) ++l;
-        return {(unsigned)((1ull << (31 + l)) / d + 1), l};
-    }
-    // ((2^32 / 2) / d would not fit for d = 1)
-    __device__ __forceinline__ unsigned quotient(unsigned n) const {
-        return shift ? __umulhi(n, m) >> (shift - 1) : n;
-    }
-};
-
-struct Params {
-    MlkLatentBatch b;
-    const void *q;
-    void *out;
-    int rows, heads;
-    float scale;  // times log2(e)
-    int groups;
-    int keys;     // that a table can hold
-    int shift;    // a unit is 2^shift steps
-    Divisor page, head;
-    Parts parts;
-};
-
-// A value that all lanes of a wave hold, known to be one: what depends on it is computed and
-// branched on once for the wave.
-__device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
-
-// A sequence's work.
-struct Work {
-    LatentSeq seq;
-    int keys;    // that its table can hold
-    int per;     // units of a tile
-    int tiles;
-};
-
-__device__ __forceinline__ Work work_of(const Params &p, const LatentSeq &seq) {
-    Work w;
-    w.seq = seq;
-    const int length = seq.length < 0 ? 0 : seq.length;
-    w.keys = length < p.keys ? length : p.keys;
-    w.per = w.keys > 0 ? ((w.keys - 1) >> (kStepShift + p.shift)) + 1 : 1;
-    // (rows * heads is below 2^31 - 15)
-    w.tiles = (int)(((unsigned)seq.count * (unsigned)p.heads + (kCols - 1)) / kCols);
-    return w;
-}
-
-__device__ __forceinline__ int wave_sum_int(int v) {
-#pragma unroll
-    for (int o = 32; o >= 1; o >>= 1) v += __shfl_xor(v, o, kWave);
-    return v;
-}
-
-// The sum of a value over this lane and those before it.
-__device__ __forceinline__ int wave_scan(int v) {
-    v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xF, 0xF, false);  // row_shr:1
-    v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xF, 0xF, false);
-    v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xF, 0xF, false);
-    v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xF, 0xF, false);
-    v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xA, 0xF, false);  // row_bcast:15
-    v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xC, 0xF, false);  // row_bcast:31
-    return v;
-}
-
-// A workgroup's run of units: `length` of them from the one that is `offset` after the first
-// of sequence `seq`; `begin` is that one's place among all.
-struct Run {
-    int seq, offset, begin, length;
-    int share, rest;  // workgroups have `share` units each, the first `rest` of them one more
-    // Of `total` units, dealt to no more workgroups than leaves each 2^kLeastShift keys: then no run
-    // between those of one tile is empty, and a tile has no more parts than pay.
-    __device__ __forceinline__ void deal(int total, int groups, int group) {
-        const int most = ((total - 1) >> (kLeastShift - kStepShift)) + 1;
-        groups = most < groups ? most : groups;
-        offset = begin = length = share = seq = rest = 0;
-        if (group >= groups) return;
-        share = (int)((unsigned)total / (unsigned)groups);
-        rest = total - share * groups;
-        begin = share * group + (group < rest ? group : rest);
-        length = share + (group < rest ? 1 : 0);
-    }
-    __device__ __forceinline__ int owner(int unit) const {
-        const int longer = (share + 1) * rest;
-        return (int)(unit < longer ? (unsigned)unit / (unsigned)(share + 1)
-                                   : rest + (unsigned)(unit - longer) / (unsigned)share);
-    }
-};
-
-// The sequences are in LDS (`held`) where a workgroup has a thread for each.
-template <int WAVES> __device__ __forceinline__ Run find_run(const Params &p, int group, LatentSeq *held) {
-    constexpr int kWaves = WAVES, kThreads = kWaves * kWave;
-    __shared__ int sums[kWaves], at[2];
-    const int t = threadIdx.x, wave = uniform(t / kWave), lane = t % kWave;
-    const auto seq_of = [&](int s) { return s < p.b.seqs ? latent_seq(p.b, s, p.rows) : LatentSeq{0, 0, 0}; };
-    const auto units_of = [&](const LatentSeq &q) {
-        const Work w = work_of(p, q);
-        return w.per * w.tiles;
-    };
-    Run r;
-    const LatentSeq mine = seq_of(t);
-    int units = units_of(mine), all = units, total = 0;
-    if (p.b.seqs <= kThreads) {
-        held[t] = mine;
-    } else {
-        for (int s = t + kThreads; s < p.b.seqs; s += kThreads) all += units_of(seq_of(s));
-        all = wave_sum_int(all);
-        if (lane == 0) sums[wave] = all;
-        __syncthreads();
-        for (int w = 0; w < kWaves; ++w) total += uniform(sums[w]);
-        r.deal(total, p.groups, group);
-    }
-    int before = 0;
-    for (int s0 = 0;; s0 += kThreads) {
-        if (s0) units = units_of(seq_of(s0 + t));
-        const int upto = wave_scan(units);
-        __syncthreads();
-        if (lane == kWave - 1) sums[wave] = upto;
-        __syncthreads();
-        int first = before + upto - units;
-#pragma unroll
-        for (int w = 0; w < kWaves; ++w) {
-            if (w < wave) first += sums[w];
-            before += uniform(sums[w]);
-        }
-        if (p.b.seqs <= kThreads) r.deal(before, p.groups, group);
-        if (r.begin >= first && r.begin < first + units) {
-            at[0] = s0 + t;
-            at[1] = r.begin - first;
-        }
-        if (r.begin < before || s0 + kThreads >= p.b.seqs) break;
-    }
-    __syncthreads();
-    if (r.length > 0) {
-        r.seq = uniform(at[0]);
-        r.offset = uniform(at[1]);
-    }
-    return r;
-}
-
-// Product step st, lane group g: the first of the 8 values that a lane holds.  Codes are
-// taken 32 at a time, one scale, so four steps go over 128 values.
-template <bool FP4> __device__ __forceinline__ int dim_of(int st, int g) {
-    if (FP4 && st < kSteps) return 128 * (st / 4) + 32 * g + 8 * (st % 4);
-    return 32 * st + 8 * g;
-}
-
-// A lane's share of a key as it is read.
-template <bool FP4> struct Raw;
-template <> struct Raw<false> {
-    u32x4 v[kAllSteps];
-};
-template <> struct Raw<true> {
-    u32x4 codes[kSteps / 4];
-    unsigned scales;
-    u32x4 rope[kRopeSteps];
-};
-
-// Whether one of its latent values is not finite, and the key without its latent values.
-__device__ __forceinline__ bool not_finite(const Raw<true> &raw, int g, int latent) {
-    bool bad = false;
-#pragma unroll
-    for (int j = 0; j < kSteps / 4; ++j)  // (scales that a narrower row has not are any bytes)
-        bad |= 128 * j + 32 * g < latent && (raw.scales >> (8 * j) & 0xFFu) == 0xFFu;
-    return bad;
-}
-__device__ __forceinline__ bool not_finite(const Raw<false> &raw, int, int) {
-    bool bad = false;
-#pragma unroll
-    for (int j = 0; j < kSteps; ++j)
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-            bad |= (raw.v[j][i] & 0x7F80u) == 0x7F80u || (raw.v[j][i] & 0x7F800000u) == 0x7F800000u;
-    return bad;
-}
-__device__ __forceinline__ void drop(Raw<true> &raw) {
-    raw.scales = 0x7F7F7F7Fu;
-#pragma unroll
-    for (int j = 0; j < kSteps / 4; ++j) raw.codes[j] = u32x4{0, 0, 0, 0};
-}
-__device__ __forceinline__ void drop(Raw<false> &raw) {
-#pragma unroll
-    for (int j = 0; j < kSteps; ++j) raw.v[j] = u32x4{0, 0, 0, 0};
-}
-
-template <bool FP4, bool FULL>
-__device__ __forceinline__ void load_key(Raw<FP4> &raw, const uint8_t *row, int g, int latent, int rope) {
-    const u32x4 none = {0, 0, 0, 0};
-    if constexpr (FP4) {
-#pragma unroll
-        for (int j = 0; j < kSteps / 4; ++j) {
-            const bool in = FULL || 128 * j + 32 * g < latent;
-            raw.codes[j] = in ? load_global16(row + 64 * j + 16 * g) : none;
-        }
-        raw.scales = *(const __attribute__((address_space(1))) unsigned *)(row + latent / 2 + 4 * g);
-        const uint8_t *tail = row + latent_part_bytes(true, latent);
-#pragma unroll
-        for (int j = 0; j < kRopeSteps; ++j) {
-            const bool in = FULL || 32 * j + 8 * g < rope;
-            raw.rope[j] = in ? load_global16(tail + 64 * j + 16 * g) : none;
-        }
-    } else {
-#pragma unroll
-        for (int j = 0; j < kAllSteps; ++j) {
-            // (steps past the latent row are the rope's)
-            const int at = j < kSteps ? 32 * j + 8 * g : 32 * (j - kSteps) + 8 * g;
-            const bool in = FULL || at < (j < kSteps ? latent : rope);
-            raw.v[j] = in ? load_global16(row + 2 * (j < kSteps ? at : latent + at)) : none;
-        }
-    }
-}
-
-// Its 8 values at step j.
-template <bool FP4, bool FULL>
-__device__ __forceinline__ u32x4 operand(const Raw<FP4> &raw, int j, int g, int latent) {
-    if constexpr (FP4) {
-        if (j >= kSteps) return raw.rope[j - kSteps];
-        const bool in = FULL || 128 * (j / 4) + 32 * g < latent;
-        const float scale = __uint_as_float(in ? (raw.scales >> (8 * (j / 4)) & 0xFFu) << 23 : 0x3F800000u);
-        const unsigned codes = raw.codes[j / 4][j % 4];
-        u32x4 v;
-        v[0] = __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes, scale, 0));
-        v[1] = __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes, scale, 1));
-        v[2] = __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes, scale, 2));
-        v[3] = __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes, scale, 3));
-        return v;
-    } else {
-        return raw.v[j];
-    }
-}
 
 // x as three bf16 parts that add up to it, cut off one after the other.
 __device__ __forceinline__ void split3(float x, unsigned (&part)[3]) {
@@ -348,25 +82,10 @@ __device__ __forceinline__ float groups_max(float v) {
     return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
 }
 
-// Results of one column, 4 values of it.
-template <bool BF16> __device__ __forceinline__ void store4(void *out, long at, f32x4 v) {
-    typedef unsigned u32x2_any __attribute__((ext_vector_type(2), aligned(2)));
-    typedef f32x4 f32x4_any __attribute__((aligned(4)));
-    if constexpr (BF16)
-        *reinterpret_cast<u32x2_any *>(static_cast<uint16_t *>(out) + at) =
-            u32x2_any{bf16_bits(v[0]) | bf16_bits(v[1]) << 16, bf16_bits(v[2]) | bf16_bits(v[3]) << 16};
-    else *reinterpret_cast<f32x4_any *>(static_cast<float *>(out) + at) = v;
-}
-
 // A sum that is in an accumulation register here.  With 512 registers, where sums begin and
 // where they are scaled, on both sides: else the compiler has all 128 moved out and back at
 // every step.  (Of 256 all are alike.)
 __device__ __forceinline__ void keep(f32x4 &v) { asm volatile("" : "+a"(v)); }
-
-// The reference that exponents are taken to moves up only when a score is this far above
-// it (in powers of 2): p stays below 2^8 and sums lose nothing by that, and most steps need
-// neither the maximum over the lane groups nor to scale what is summed.
-constexpr float kSlack = 8.0f;
 
 template <bool FP4, bool BF16, bool FULL>
 __global__ __launch_bounds__((kWavesOf<FP4> * kWave), 1) void latent_attend_kernel(Params p) {
@@ -393,12 +112,12 @@ __global__ __launch_bounds__((kWavesOf<FP4> * kWave), 1) void latent_attend_kern
             identity[h][i] = g == 2 * h + c / 8 && i == c % 8 / 2 ? c % 2 ? 0x3F800000u : 0x3F80u : 0u;
 
     const int group = blockIdx.x;
-    const Run run = find_run<kWaves>(p, group, held);
+    const Run run = find_run<Narrow, kWaves>(p, group, held);
     if (t == 0 && !p.parts.tiles) p.parts.records[group].first = -1;
     int left = run.length, offset = run.offset;
     for (int s = run.seq; left > 0 && s < p.b.seqs; ++s, offset = 0) {
         const LatentSeq seq = p.b.seqs <= kThreads ? held[s] : latent_seq(p.b, s, p.rows);
-        const Work w = work_of(p, {uniform(seq.begin), uniform(seq.count), uniform(seq.length)});
+        const Work w = work_of<Narrow>(p, {uniform(seq.begin), uniform(seq.count), uniform(seq.length)});
         while (left > 0 && offset < w.per * w.tiles) {
             // (what follows from it is not worth a register from one tile to the next)
             int tid = t;
@@ -673,100 +392,21 @@ __global__ __launch_bounds__((kWavesOf<FP4> * kWave), 1) void latent_attend_kern
     }
 }
 
-// Joins the tile of record blockIdx.x: its sums are in part 2 first + 1 and in parts 2w of
-// the workgroups w after the first.  128 threads take a column's values, and blockDim.x /
-// 128 such teams share its parts: a round of loads from what other workgroups wrote takes
-// about a microsecond, so as many as can are under way at once.
-constexpr int kTeam = kLatentMax / 4;
-constexpr int kJoinLoads = 16;  // parts that a thread has on their way
-constexpr int kMaxTeams = 4;
-template <bool BF16> __global__ __launch_bounds__(kTeam *kMaxTeams) void latent_join_kernel(Params p) {
-    __shared__ float tops[2 * kMaxGroups], sums[2 * kMaxGroups];
-    __shared__ float reds[2][kTeam * kMaxTeams / kWave];
-    __shared__ f32x4 shares[kMaxTeams - 1][kTeam];
-    const Record record = p.parts.records[blockIdx.x];
-    if (record.first < 0) return;
-    const int col = blockIdx.y, team = threadIdx.x / kTeam, t = threadIdx.x % kTeam, teams = blockDim.x / kTeam;
-    // (a record without a tile holds anything)
-    const int first = record.first < p.groups ? record.first : 0;
-    const int last = record.last < first ? first : record.last < p.groups ? record.last : p.groups - 1;
-    const int count = last - first + 1;
-    const auto part_of = [&](int i) { return 2 * (first + i) + (i == 0 ? 1 : 0); };
-    const int s = (unsigned)record.seq < (unsigned)p.b.seqs ? record.seq : 0;
-    const LatentSeq seq = latent_seq(p.b, s, p.rows);
-    const int pairs = seq.count * p.heads, pair = record.tile * kCols + col;
-    const long base = (long)seq.begin * p.heads;
-    const float *from = p.parts.sums + col * kLatentMax + 4 * t;
-    float top = -INFINITY, sum = 0.0f;
-    f32x4 v[kJoinLoads], result = {0.f, 0.f, 0.f, 0.f};
-    // (entered a step early, for the loads; parts i0 + team + k teams)
-    const int stride = kJoinLoads * teams;
-    for (int i0 = team - stride; i0 < count; i0 += stride) {
-        if (i0 >= 0) {
-#pragma unroll
-            for (int k = 0; k < kJoinLoads; ++k)
-                if (i0 + k * teams < count) result += tops[i0 + k * teams] * v[k];
-        }
-#pragma unroll
-        for (int k = 0; k < kJoinLoads; ++k) {
-            const int i = i0 + stride + k * teams;
-            v[k] = load_f4(from + part_of(i < count ? i : count - 1) * (kCols * kLatentMax));
-        }
-        if (i0 >= 0) continue;
-        // (what a record without a tile says of one is not true)
-        if (p.parts.tiles && ((unsigned)record.tile > (unsigned)pairs / kCols ||
-                              (int)((base + record.tile * kCols) / kCols) + s != (int)blockIdx.x))
-            return;
-        for (int i = threadIdx.x; i < count; i += blockDim.x) {
-            const float *stats = p.parts.stats + part_of(i) * (2 * kCols) + col;
-            tops[i] = stats[0];
-            sums[i] = stats[kCols];
-            top = fmaxf(top, stats[0]);
-        }
-        top = dpp_wave_max(top);
-        if (threadIdx.x % kWave == 0) reds[0][threadIdx.x / kWave] = top;
-        __syncthreads();
-        for (int k = 0; k < teams * kTeam / kWave; ++k) top = fmaxf(top, reds[0][k]);
-        if (top == -INFINITY) top = 0.0f;
-        for (int i = threadIdx.x; i < count; i += blockDim.x) {
-            const float by = __builtin_amdgcn_exp2f(tops[i] - top);
-            tops[i] = by;
-            sum += by * sums[i];
-        }
-        sum = dpp_wave_sum(sum);
-        if (threadIdx.x % kWave == 0) reds[1][threadIdx.x / kWave] = sum;
-        __syncthreads();
-        sum = 0.0f;
-        for (int k = 0; k < teams * kTeam / kWave; ++k) sum += reds[1][k];
-    }
-    if (teams > 1) {
-        if (team) shares[team - 1][t] = result;
-        __syncthreads();
-        if (team) return;
-        for (int k = 1; k < teams; ++k) result += shares[k - 1][t];
-    }
-    if (pair >= pairs || 4 * t >= p.b.latent) return;
-    store4<BF16>(p.out, (base + pair) * p.b.latent + 4 * t, result * (sum == 0.0f ? 0.0f : 1.0f / sum));
-}
-
 template <bool FP4, bool BF16, bool FULL> int launch(const Params &p, hipStream_t stream) {
     constexpr int kThreads = kWavesOf<FP4> * kWave;
     constexpr int bytes = kLdsBytes<FP4, BF16>;
     const auto kernel = latent_attend_kernel<FP4, BF16, FULL>;
-    static const bool ok = hipFuncSetAttribute(reinterpret_cast<const void *>(kernel),
-                                               hipFuncAttributeMaxDynamicSharedMemorySize, bytes) == hipSuccess;
+    static const bool ok = allow_lds(kernel, bytes);
     if (!ok) return kErrLaunch;
     kernel<<<p.groups, kThreads, bytes, stream>>>(p);
     if (hipGetLastError() != hipSuccess) return kErrLaunch;
-    if (p.groups == 1) return kOk;
-    // four teams where all records' workgroups are resident at once that way
-    const int records = p.parts.tiles ? p.parts.tiles : p.groups;
-    const int teams = records * kCols * kTeam * kMaxTeams <= p.groups * 2048 ? kMaxTeams : 1;
-    latent_join_kernel<BF16><<<dim3(records, kCols), kTeam * teams, 0, stream>>>(p);
-    return hipGetLastError() == hipSuccess ? kOk : kErrLaunch;
+    return launch_join<Narrow, BF16>(p, stream);
 }
 
 }  // namespace
+
+// Pairs a sequence from which the wide kernel is taken.
+constexpr int kWideFrom = 64;
 
 size_t latent_attend_workspace() { return kSumsBytes + kStatsBytes + kRecordBytes; }
 
@@ -778,20 +418,25 @@ int latent_attend(const MlkLatentBatch &b, const LatentAttend &p, int cu_count, 
     a.rows = p.rows;
     a.heads = p.heads;
     a.scale = p.scale * 1.44269504f;
-    a.groups = cu_count < kMaxGroups ? cu_count : kMaxGroups;
+    const bool full = b.latent == kLatentMax && b.rope == kLatentRopeMax;
+    const bool wide = full && p.bf16 && (reinterpret_cast<uintptr_t>(p.q) & 15) == 0 &&
+                      (long)p.rows * p.heads >= (long)kWideFrom * b.seqs;
+    const int most_groups = wide ? kMaxWideGroups : kMaxGroups;
+    a.groups = cu_count < most_groups ? cu_count : most_groups;
     const long room = (long)b.table_width * b.page_size;
     a.keys = room < 0x7FFFFFFF ? (int)room : 0x7FFFFFFF;
     // units of more keys where there could be 2^31 of them (a tile has at least a column)
-    const long tiles = (long)p.rows * p.heads / kCols + b.seqs;
+    const long tiles = (long)p.rows * p.heads / (wide ? Wide::kCols : Narrow::kCols) + b.seqs;
+    const int step_shift = wide ? Wide::kStepShift : Narrow::kStepShift;
     a.parts.tiles = tiles <= kMaxTileRecords ? (int)tiles : 0;
-    for (a.shift = 0; tiles * (((a.keys - 1) >> (kStepShift + a.shift)) + 1) >= 0x7FFFFFFF; ++a.shift) {}
+    for (a.shift = 0; tiles * (((a.keys - 1) >> (step_shift + a.shift)) + 1) >= 0x7FFFFFFF; ++a.shift) {}
     a.page = Divisor::of((unsigned)b.page_size);
     a.head = Divisor::of((unsigned)p.heads);
     uint8_t *at = static_cast<uint8_t *>(p.workspace);
     a.parts.sums = reinterpret_cast<float *>(at);
     a.parts.stats = reinterpret_cast<float *>(at + kSumsBytes);
     a.parts.records = reinterpret_cast<Record *>(at + kSumsBytes + kStatsBytes);
-    const bool full = b.latent == kLatentMax && b.rope == kLatentRopeMax;
+    if (wide) return launch_wide(b.type == MLK_FP4, a, stream);
     if (b.type == MLK_FP4)
         return p.bf16 ? (full ? launch<true, true, true>(a, stream) : launch<true, true, false>(a, stream))
                       : (full ? launch<true, false, true>(a, stream) : launch<true, false, false>(a, stream));

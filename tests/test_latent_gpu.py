@@ -279,6 +279,24 @@ def test_attend(device, workspace, dtype, cache_type, latent, rope, page, heads,
     check_attend(rng, cache, dtype, heads, workspace)
 
 
+@pytest.mark.parametrize("cache_type", [MLK_BF16, MLK_FP4])
+@pytest.mark.parametrize("page,heads,pairs,lead", [
+    (16, 16, [(64, 64)], 0),
+    (16, 16, [(4, 4)], 0),
+    (64, 16, [(127, 5), (128, 4), (129, 8), (0, 0), (1, 1), (63, 20)], 0),
+    (100, 5, [(300, 33), (40, 40)], 0),
+    (1, 128, [(65, 1), (200, 1)], 0),
+    (7, 40, [(2, 3), (90, 2), (0, 4)], 0),
+    (128, 16, [(1500, 40), (700, 8), (30, 30), (1100, 1)], 0),
+    (16, 1, [(150, 150)], 0),
+    (16, 16, [(90, 9)], 2)])
+def test_attend_many_pairs_a_sequence(device, workspace, cache_type, page, heads, pairs, lead):
+    """Prompts in chunks, many heads; beside single rows and empty sequences."""
+    rng = np.random.default_rng(page + heads + len(pairs))
+    cache = L.Cache(rng, cache_type, pairs, page_size=page, rows_behind=1).fill(rng)
+    check_attend(rng, cache, MLK_BF16, heads, workspace, lead=lead)
+
+
 @pytest.mark.parametrize("dtype", [MLK_F32, MLK_BF16])
 @pytest.mark.parametrize("cache_type", [MLK_BF16, MLK_FP4])
 def test_attend_joined_over_workgroups(device, workspace, dtype, cache_type):
@@ -307,6 +325,10 @@ def test_attend_sharp_and_flat_scores(device, workspace, dtype):
     check_attend(rng, cache, dtype, 16, workspace, scale=0.5)
     check_attend(rng, cache, dtype, 16, workspace, scale=-0.3)
     check_attend(rng, cache, dtype, 16, workspace, scale=0.0)
+    cache.starts = np.array([0, 6], np.int32)
+    cache.rows = 6
+    for scale in (0.5, -0.3, 0.0):
+        check_attend(rng, cache, dtype, 16, workspace, scale=scale)
 
 
 @pytest.mark.parametrize("cache_type", [MLK_BF16, MLK_FP4])
@@ -320,11 +342,11 @@ def test_attend_unaligned_rows(device, workspace, dtype, cache_type):
 @pytest.mark.parametrize("cache_type", [MLK_BF16, MLK_FP4])
 @pytest.mark.parametrize("dtype", [MLK_F32, MLK_BF16])
 @pytest.mark.parametrize("bad", [np.nan, np.inf, -np.inf])
-def test_attend_values_that_are_not_finite(device, workspace, dtype, cache_type, bad):
+@pytest.mark.parametrize("heads", [3, 40])
+def test_attend_values_that_are_not_finite(device, workspace, dtype, cache_type, bad, heads):
     """A key with such a value reaches the rows that see it, and those alone, in the
     latent row or in the rope row; so does a query."""
     rng = np.random.default_rng(24)
-    heads = 3
     for column in (100, 540):
         for at in (0, 20, 93, 99):
             cache = L.Cache(rng, cache_type, [(100, 12), (40, 1)]).fill(rng)
@@ -353,7 +375,8 @@ def test_attend_values_that_are_not_finite(device, workspace, dtype, cache_type,
 
 @pytest.mark.parametrize("cache_type", [MLK_BF16, MLK_FP4])
 @pytest.mark.parametrize("dtype", [MLK_F32, MLK_BF16])
-def test_attend_pages_out_of_range(device, workspace, dtype, cache_type):
+@pytest.mark.parametrize("heads", [3, 40])
+def test_attend_pages_out_of_range(device, workspace, dtype, cache_type, heads):
     """Rows that read a key without a page are NaN, the others as they were; so with keys
     behind the table."""
     rng = np.random.default_rng(25)
@@ -361,9 +384,9 @@ def test_attend_pages_out_of_range(device, workspace, dtype, cache_type):
     good = cache.tables.copy()
     cache.tables[0, 5] = cache.pages       # keys 80 .. 95
     cache.tables[1, 3] = -1
-    got, q, scale = run_attend(rng, cache, dtype, 3, workspace)
+    got, q, scale = run_attend(rng, cache, dtype, heads, workspace)
     cache.tables = good
-    want, mass, score = L.attend(cache, q, 3, scale)
+    want, mass, score = L.attend(cache, q, heads, scale)
     room = L.attend_tolerance(cache, want, mass, score, dtype)
     sees = np.array([s == 1 or (s == 0 and j >= 80) for _, s, j in cache.each_row()])
     assert np.isnan(got[sees]).all()
@@ -371,10 +394,10 @@ def test_attend_pages_out_of_range(device, workspace, dtype, cache_type):
     # the table of sequence 2 ends after 48 keys: its first row, key 48, sees one more
     cache = L.Cache(rng, cache_type, [(48, 2)], page_size=16, table_extra=0).fill(rng)
     cache.lengths[0] = 49
-    got, q, scale = run_attend(rng, cache, dtype, 3, workspace)
+    got, q, scale = run_attend(rng, cache, dtype, heads, workspace)
     cache.lengths[0] = 48
     cache.starts = np.array([0, 1], np.int32)
-    want, mass, score = L.attend(cache, q, 3, scale)
+    want, mass, score = L.attend(cache, q, heads, scale)
     room = L.attend_tolerance(cache, want, mass, score, dtype)
     assert np.all(np.abs(got - want[:2])[0] <= room[0]) and np.isnan(got[1]).all()
 
