@@ -15,17 +15,16 @@ typedef u32x4 u32x4_any __attribute__((aligned(2)));
 
 constexpr int kSteps = kLatentMax / 32;          // 32-value steps over a latent row
 constexpr int kRopeSteps = kLatentRopeMax / 32;  // and over a rope row
-constexpr int kMaxGroups = 512;                  // workgroups of a launch
-constexpr int kMaxWideGroups = 254;              // of the wide kernel: its parts, in 64 MiB of workspace
 
 // A tile is kCols (row, head) pairs of a sequence; its keys are taken 2^kStepShift at a time (a
 // step), and a workgroup has at least 2^kLeastShift keys, where there are as many.
-template <int COLS, int STEP_SHIFT, int LEAST_SHIFT> struct Tiling {
+template <int COLS, int STEP_SHIFT, int LEAST_SHIFT, int GROUPS> struct Tiling {
     static constexpr int kCols = COLS, kStepShift = STEP_SHIFT, kStepKeys = 1 << STEP_SHIFT;
     static constexpr int kLeastShift = LEAST_SHIFT;
+    static constexpr int kGroups = GROUPS;  // workgroups of a launch, at most
 };
-typedef Tiling<16, 4, 6> Narrow;
-typedef Tiling<64, 6, 7> Wide;
+typedef Tiling<16, 4, 6, 512> Narrow;
+typedef Tiling<64, 6, 7, 254> Wide;  // (its parts: in 64 MiB of workspace)
 
 // What latent_join_kernel has to know of a tile, told by the workgroup that ends it: its
 // sequence and number in it, and the workgroups that its units fell to (-1: to one, there is
@@ -47,13 +46,13 @@ struct Parts {
     Record *records;
     int tiles;      // records of tiles, else 0: of workgroups
 };
-constexpr long kMaxPartCols = kMaxGroups * Narrow::kCols > kMaxWideGroups * Wide::kCols ? 2 * kMaxGroups * Narrow::kCols
-                                                                                        : 2 * kMaxWideGroups * Wide::kCols;
+constexpr long kMaxPartCols = Narrow::kGroups * Narrow::kCols > Wide::kGroups * Wide::kCols ? 2 * Narrow::kGroups * Narrow::kCols
+                                                                                        : 2 * Wide::kGroups * Wide::kCols;
 constexpr size_t kSumsBytes = kMaxPartCols * kLatentMax * 4;
 constexpr size_t kStatsBytes = kMaxPartCols * 2 * 4;
 constexpr size_t kRecordBytes = (size_t)kMaxTileRecords * sizeof(Record);
 static_assert(kSumsBytes + kStatsBytes + kRecordBytes <= 64 << 20, "the workspace");
-static_assert(kMaxGroups <= kMaxTileRecords, "records of workgroups");
+static_assert(Narrow::kGroups <= kMaxTileRecords, "records of workgroups");
 
 // n / d of n below 2^31 by a product: m is the whole number above 2^(31 + l) / d with l the
 // least for which 2^l >= d.
@@ -303,20 +302,22 @@ template <bool BF16> __device__ __forceinline__ void store4(void *out, long at, 
 constexpr float kSlack = 24.0f;
 
 // Joins the tile of record blockIdx.x: its sums are in part 2 first + 1 and in parts 2w of
-// the workgroups w after the first.  128 threads take a column's values, and blockDim.x /
-// 128 such teams share its parts: a round of loads from what other workgroups wrote takes
-// about a microsecond, so as many as can are under way at once.
+// the workgroups w after the first.  128 threads take a column's values, and TEAMS such teams
+// share its parts: a round of loads from what other workgroups wrote takes about a
+// microsecond, so as many as can are under way at once, 16 a thread.  Where there are so many
+// records that not all of them are resident with four teams each, a tile has few parts, and a
+// thread asks for 4 at a time: what it asks for beyond the last part is read again for nothing
+// (128 tiles of 64 columns of two or three parts: 11.6 us, with 16 a thread 16.3).
 constexpr int kTeam = kLatentMax / 4;
-constexpr int kJoinLoads = 16;  // parts that a thread has on their way
 constexpr int kMaxTeams = 4;
-template <class Til, bool BF16> __global__ __launch_bounds__((kTeam * kMaxTeams)) void latent_join_kernel(Params p) {
-    constexpr int kCols = Til::kCols;
-    __shared__ float tops[2 * kMaxGroups], sums[2 * kMaxGroups];
-    __shared__ float reds[2][kTeam * kMaxTeams / kWave];
-    __shared__ f32x4 shares[kMaxTeams - 1][kTeam];
+template <class Til, bool BF16, int TEAMS> __global__ __launch_bounds__((kTeam * TEAMS)) void latent_join_kernel(Params p) {
+    constexpr int kCols = Til::kCols, kThreads = kTeam * TEAMS, kLoads = TEAMS == 1 ? 4 : 16, kStride = kLoads * TEAMS;
+    __shared__ float tops[Til::kGroups], sums[Til::kGroups];
+    __shared__ float reds[2][kThreads / kWave];
+    __shared__ f32x4 shares[TEAMS][kTeam];
     const Record record = p.parts.records[blockIdx.x];
     if (record.first < 0) return;
-    const int col = blockIdx.y, team = threadIdx.x / kTeam, t = threadIdx.x % kTeam, teams = blockDim.x / kTeam;
+    const int col = blockIdx.y, team = threadIdx.x / kTeam, t = threadIdx.x % kTeam;
     // (a record without a tile holds anything)
     const int first = record.first < p.groups ? record.first : 0;
     const int last = record.last < first ? first : record.last < p.groups ? record.last : p.groups - 1;
@@ -328,26 +329,25 @@ template <class Til, bool BF16> __global__ __launch_bounds__((kTeam * kMaxTeams)
     const long base = (long)seq.begin * p.heads;
     const float *from = p.parts.sums + col * kLatentMax + 4 * t;
     float top = -INFINITY, sum = 0.0f;
-    f32x4 v[kJoinLoads], result = {0.f, 0.f, 0.f, 0.f};
-    // (entered a step early, for the loads; parts i0 + team + k teams)
-    const int stride = kJoinLoads * teams;
-    for (int i0 = team - stride; i0 < count; i0 += stride) {
+    f32x4 v[kLoads], result = {0.f, 0.f, 0.f, 0.f};
+    // (entered a step early, for the loads; parts i0 + team + k TEAMS)
+    for (int i0 = team - kStride; i0 < count; i0 += kStride) {
         if (i0 >= 0) {
 #pragma unroll
-            for (int k = 0; k < kJoinLoads; ++k)
-                if (i0 + k * teams < count) result += tops[i0 + k * teams] * v[k];
+            for (int k = 0; k < kLoads; ++k)
+                if (i0 + k * TEAMS < count) result += tops[i0 + k * TEAMS] * v[k];
         }
 #pragma unroll
-        for (int k = 0; k < kJoinLoads; ++k) {
-            const int i = i0 + stride + k * teams;
-            v[k] = load_f4(from + part_of(i < count ? i : count - 1) * (kCols * kLatentMax));
+        for (int k = 0; k < kLoads; ++k) {
+            const int i = i0 + kStride + k * TEAMS;
+            v[k] = load_f4(from + (long)part_of(i < count ? i : count - 1) * (kCols * kLatentMax));
         }
         if (i0 >= 0) continue;
         // (what a record without a tile says of one is not true)
         if (p.parts.tiles && ((unsigned)record.tile > (unsigned)pairs / kCols ||
                               (int)((base + record.tile * kCols) / kCols) + s != (int)blockIdx.x))
             return;
-        for (int i = threadIdx.x; i < count; i += blockDim.x) {
+        for (int i = threadIdx.x; i < count; i += kThreads) {
             const float *stats = p.parts.stats + part_of(i) * (2 * kCols) + col;
             tops[i] = stats[0];
             sums[i] = stats[kCols];
@@ -356,9 +356,10 @@ template <class Til, bool BF16> __global__ __launch_bounds__((kTeam * kMaxTeams)
         top = dpp_wave_max(top);
         if (threadIdx.x % kWave == 0) reds[0][threadIdx.x / kWave] = top;
         __syncthreads();
-        for (int k = 0; k < teams * kTeam / kWave; ++k) top = fmaxf(top, reds[0][k]);
+#pragma unroll
+        for (int k = 0; k < kThreads / kWave; ++k) top = fmaxf(top, reds[0][k]);
         if (top == -INFINITY) top = 0.0f;
-        for (int i = threadIdx.x; i < count; i += blockDim.x) {
+        for (int i = threadIdx.x; i < count; i += kThreads) {
             const float by = __builtin_amdgcn_exp2f(tops[i] - top);
             tops[i] = by;
             sum += by * sums[i];
@@ -367,13 +368,15 @@ template <class Til, bool BF16> __global__ __launch_bounds__((kTeam * kMaxTeams)
         if (threadIdx.x % kWave == 0) reds[1][threadIdx.x / kWave] = sum;
         __syncthreads();
         sum = 0.0f;
-        for (int k = 0; k < teams * kTeam / kWave; ++k) sum += reds[1][k];
+#pragma unroll
+        for (int k = 0; k < kThreads / kWave; ++k) sum += reds[1][k];
     }
-    if (teams > 1) {
+    if (TEAMS > 1) {
         if (team) shares[team - 1][t] = result;
         __syncthreads();
         if (team) return;
-        for (int k = 1; k < teams; ++k) result += shares[k - 1][t];
+#pragma unroll
+        for (int k = 1; k < TEAMS; ++k) result += shares[k - 1][t];
     }
     if (pair >= pairs || 4 * t >= p.b.latent) return;
     store4<BF16>(p.out, (base + pair) * p.b.latent + 4 * t, result * (sum == 0.0f ? 0.0f : 1.0f / sum));
@@ -382,10 +385,11 @@ template <class Til, bool BF16> __global__ __launch_bounds__((kTeam * kMaxTeams)
 // Behind the attention kernel's launch.
 template <class Til, bool BF16> int launch_join(const Params &p, hipStream_t stream) {
     if (p.groups == 1) return kOk;
-    // four teams where all records' workgroups are resident at once that way
     const int records = p.parts.tiles ? p.parts.tiles : p.groups;
-    const int teams = records * Til::kCols * kTeam * kMaxTeams <= p.groups * 2048 ? kMaxTeams : 1;
-    latent_join_kernel<Til, BF16><<<dim3(records, Til::kCols), kTeam * teams, 0, stream>>>(p);
+    if ((long)records * Til::kCols * kTeam * kMaxTeams <= (long)p.groups * 2048)
+        latent_join_kernel<Til, BF16, kMaxTeams><<<dim3(records, Til::kCols), kTeam * kMaxTeams, 0, stream>>>(p);
+    else
+        latent_join_kernel<Til, BF16, 1><<<dim3(records, Til::kCols), kTeam, 0, stream>>>(p);
     return hipGetLastError() == hipSuccess ? kOk : kErrLaunch;
 }
 

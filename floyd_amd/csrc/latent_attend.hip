@@ -421,7 +421,7 @@ int latent_attend(const MlkLatentBatch &b, const LatentAttend &p, int cu_count, 
     const bool full = b.latent == kLatentMax && b.rope == kLatentRopeMax;
     const bool wide = full && p.bf16 && (reinterpret_cast<uintptr_t>(p.q) & 15) == 0 &&
                       (long)p.rows * p.heads >= (long)kWideFrom * b.seqs;
-    const int most_groups = wide ? kMaxWideGroups : kMaxGroups;
+    const int most_groups = wide ? Wide::kGroups : Narrow::kGroups;
     a.groups = cu_count < most_groups ? cu_count : most_groups;
     const long room = (long)b.table_width * b.page_size;
     a.keys = room < 0x7FFFFFFF ? (int)room : 0x7FFFFFFF;

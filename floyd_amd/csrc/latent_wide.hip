@@ -24,6 +24,7 @@ namespace {
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 
 constexpr int kCols = Wide::kCols, kStepKeys = Wide::kStepKeys;
@@ -141,32 +142,31 @@ template <bool FP4> __global__ __launch_bounds__(kThreads, 1) void latent_wide_k
             const int from = first << p.shift, seen_steps = (most + kStepKeys - 1) >> Wide::kStepShift;
             const int upto = (last << p.shift) < seen_steps ? last << p.shift : seen_steps;
 
-            // the pages of the keys that a wave brings in, asked for a step before those; keys that nothing
-            // sees are taken from page 0
+            // The keys that a wave brings in: their pages, asked for two steps before those, and then
+            // their addresses and whether they have one.  Keys that nothing sees are taken from page 0.
             const int *table = p.b.tables + (long)s * p.b.table_width;
             unsigned in_page;
-            const auto page_of = [&](int step) {
+            bool any_page;
+            int page;
+            const auto ask = [&](int step) {
                 const unsigned j = (unsigned)step * kStepKeys + own_key, at = p.page.quotient(j);
                 in_page = j - at * (unsigned)p.b.page_size;
-                int page = 0;
-                if (step < upto && j < (unsigned)most) page = table[at];
-                return page;
+                any_page = step >= upto || j >= (unsigned)most;
+                page = table[any_page ? 0 : at];
             };
-            int page = page_of(from);
-
-            // Of the step whose pages are there: kPieces loads, from `row` on, and the pages of the next
-            // step.  4-bit keys go through registers, to be written as bf16 ones, 16 bytes of a
-            // lane at a time.
             const uint8_t *row = nullptr;
-            Raw<true> codes;
-            constexpr int kPieces = (FP4 ? 0 : kStageKeys) + 2;
             const auto find = [&](int step) {
-                const bool there = (unsigned)page < (unsigned)p.b.pages;
-                const unsigned long long bad = __ballot(!there);
-                if (lane == 0) bads[step & 1][wave] = (unsigned)bad & 0xFFFFu;
-                const long slot = there ? (long)page * p.b.page_size + in_page : 0;
+                const int place = any_page ? 0 : page;
+                const bool there = (unsigned)place < (unsigned)p.b.pages;
+                bads[step & 1][wave] = (unsigned)__ballot(!there) & 0xFFFFu;
+                const unsigned long slot = (unsigned long)(there ? (unsigned)place : 0u) * (unsigned)p.b.page_size +
+                                           (there ? in_page : 0u);
                 row = static_cast<const uint8_t *>(p.b.data) + slot * row_bytes;
-                page = page_of(step + 1);
+            };
+            ask(from);
+            // 4-bit keys go through registers, to be written as bf16 ones, 16 bytes of a lane at a time.
+            Raw<true> codes;
+            const auto load_codes = [&] {
                 if constexpr (FP4) {
 #pragma unroll
                     for (int j = 0; j < kSteps / 4; ++j) codes.codes[j] = load_global16(row + 64 * j + 16 * g);
@@ -176,21 +176,23 @@ template <bool FP4> __global__ __launch_bounds__(kThreads, 1) void latent_wide_k
             // row k of a wave's, from the lane that has its address
             const auto bring_row = [&](LdsByte *to, const uint8_t *row, int k) {
                 const unsigned lo = (unsigned)(unsigned long long)row, hi = (unsigned)((unsigned long long)row >> 32);
-                const uint8_t *from = (const uint8_t *)((unsigned long long)__builtin_amdgcn_readlane(hi, k) << 32 |
-                                                        (unsigned)__builtin_amdgcn_readlane(lo, k));
+                void *from = (void *)((unsigned long long)__builtin_amdgcn_readlane(hi, k) << 32 |
+                                      (unsigned)__builtin_amdgcn_readlane(lo, k));
                 unsigned at = 16 * lane;
                 asm volatile("" : "+v"(at));
-                __builtin_amdgcn_global_load_lds((GlobalPtr)(from + (at ^ 16 * turn(k))),
-                                                 to + (kStageKeys * wave + k) * (kLatentMax * 2), 16, 0, 0);
+                __builtin_amdgcn_raw_ptr_buffer_load_lds(
+                    __builtin_amdgcn_make_buffer_rsrc(from, 0, kLatentMax * 2, 0x00027000),
+                    to + (kStageKeys * wave + k) * (kLatentMax * 2), 16, at ^ 16 * turn(k), 0, 0, 0);
             };
             const auto bring_rope = [&](LdsByte *to, const uint8_t *rope, int k) {
                 __builtin_amdgcn_global_load_lds((GlobalPtr)(rope + 16 * g + 64 * k),
                                                  to + kLatentBytes + wave * kRopeRows + 1024 * k, 16, 0, 0);
             };
+            constexpr int kPieces = (FP4 ? 0 : kStageKeys) + 2;
             const auto bring = [&](int step, int k) {
                 LdsByte *to = base_lds + (step & 1) * kStepBytes;
-                if (k < 2) bring_rope(to, row + latent_part_bytes(FP4, kLatentMax), k);
-                else bring_row(to, row, k - 2);
+                if (k < kPieces - 2) bring_row(to, row, k);
+                else bring_rope(to, row + latent_part_bytes(FP4, kLatentMax), k - (kPieces - 2));
             };
             const auto put = [&](int step, int j) {
                 if constexpr (FP4) {
@@ -221,10 +223,14 @@ template <bool FP4> __global__ __launch_bounds__(kThreads, 1) void latent_wide_k
 #pragma unroll
                 for (int k = 0; k < 2; ++k) bring_rope(to, at + kLatentMax * 2, k);
                 find(from);
+                ask(from + 1);
+                load_codes();
 #pragma unroll
                 for (int k = 0; k < kPieces; ++k) bring(from, k);
 #pragma unroll
                 for (int j = 0; j < kSteps; ++j) put(from, j);
+                find(from + 1);
+                ask(from + 2);
                 meet();
                 int straight = row_turn + col0 * (kLatentMax * 2) + (~from & 1) * kStepBytes;
                 asm volatile("" : "+v"(straight));
@@ -253,32 +259,35 @@ template <bool FP4> __global__ __launch_bounds__(kThreads, 1) void latent_wide_k
                 asm volatile("" : "+v"(straight), "+v"(turned));
                 straight &= 0x3FFFF, turned &= 0x3FFFF;
 
-                // S; a group of reads is ahead of its products by one
-                u32x4 part[2][kGroup];
+                // S; reads are two groups ahead of their products
+                u32x4 part[3][kGroup];
                 const auto read = [&](int n) {
 #pragma unroll
                     for (int x = 0; x < kGroup; ++x) {
                         const int j = n * kGroup + x;
-                        part[n % 2][x] = *(const LdsPiece *)(base_lds +
+                        part[n % 3][x] = *(const LdsPiece *)(base_lds +
                                                              (j < kRowSteps ? (straight ^ 2 * j % 16 * 16) + 256 * (j / 8)
                                                                             : rope_turn + 2 * half * kRopeRows +
                                                                                   buf * kStepBytes + 512 * (j - kRowSteps)));
                     }
                 };
                 read(0);
-                find(step + 1);  // (behind the last step: keys from page 0, that nothing uses)
+                read(1);
+                load_codes();  // (behind the last step: keys from page 0, that nothing uses)
                 f32x16 score = {0.f};
                 asm volatile("" : "+v"(score));
+                __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
                 for (int n = 0; n < kQuerySteps / kGroup; ++n) {
-                    if (n + 1 < kQuerySteps / kGroup) read(n + 1);
-#pragma unroll
-                    for (int k = 2 * n; k < 2 * n + 2; ++k)
-                        if (k < kPieces) bring(step + 1, k);
+                    if (n + 2 < kQuerySteps / kGroup) read(n + 2);
                     __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-                    for (int x = 0; x < kGroup; ++x) score = mfma(part[n % 2][x], query[n * kGroup + x], score);
-                    __builtin_amdgcn_sched_barrier(0);
+                    for (int x = 0; x < kGroup; ++x) {
+                        score = mfma(part[n % 3][x], query[n * kGroup + x], score);
+                        const int k = 2 * n + x / 2 - (2 * kQuerySteps / kGroup - kPieces);
+                        if (x % 2 && k >= 0) bring(step + 1, k);
+                        if (x % 2) __builtin_amdgcn_sched_barrier(0);
+                    }
                 }
 
                 float scale = p.scale;
@@ -290,20 +299,25 @@ template <bool FP4> __global__ __launch_bounds__(kThreads, 1) void latent_wide_k
                     // see them.
                     int row_at = buf * kStepBytes + (kWaveKeys * half + c) * (kLatentMax * 2);
                     asm volatile("" : "+v"(row_at));
-                    bool finite = true;
-                    for (int j = h; j < kLatentMax / 8; j += 2) {
-                        const u32x4 v = *(const LdsPiece *)(base_lds + row_at + 16 * j);
+                    u16x2 largest = {0, 0};
+#pragma unroll 8
+                    for (int j = 0; j < kLatentMax / 16; ++j) {  // (in an order that has lanes on all banks)
+                        const u32x4 v = *(const LdsPiece *)(base_lds + row_at + 16 * ((2 * j + h) ^ c % 16));
 #pragma unroll
                         for (int i = 0; i < 4; ++i)
-                            finite &= (v[i] & 0x7F80u) != 0x7F80u && (v[i] & 0x7F800000u) != 0x7F800000u;
+                            largest = __builtin_elementwise_max(largest, __builtin_bit_cast(u16x2, v[i] & 0x7FFF7FFFu));
                     }
+                    const bool finite = largest[0] < 0x7F80u && largest[1] < 0x7F80u;
                     const bool seen = key0 + kWaveKeys * half + c < most;
                     const unsigned long long which = __ballot(seen && !finite);
                     const unsigned wrong = (unsigned)(which | which >> 32) | bads[buf][2 * half] | bads[buf][2 * half + 1] << 16;
                     meet_lds();  // (both waves of a row have looked at it)
                     if (!seen || (wrong >> c & 1u)) {
-                        for (int j = h; j < kLatentMax / 8; j += 2) *(LdsPiece *)(base_lds + row_at + 16 * j) = u32x4{0, 0, 0, 0};
+#pragma unroll 8
+                        for (int j = 0; j < kLatentMax / 16; ++j)
+                            *(LdsPiece *)(base_lds + row_at + 16 * ((2 * j + h) ^ c % 16)) = u32x4{0, 0, 0, 0};
                     }
+                    meet_lds();
                     const unsigned bits = wrong >> 4 * h;
                     const int end = limit - (key0 + kWaveKeys * half + 4 * h);
 #pragma unroll
@@ -314,14 +328,20 @@ template <bool FP4> __global__ __launch_bounds__(kThreads, 1) void latent_wide_k
                     }
                     scale = 1.0f;
                 }
-                float high = -INFINITY;
+                float high = score[0];
+                if (scale >= 0) {
 #pragma unroll
-                for (int i = 0; i < 16; ++i) high = fmaxf(high, score[i] * scale);
+                    for (int i = 1; i < 16; ++i) high = fmaxf(high, score[i]);
+                } else {
+#pragma unroll
+                    for (int i = 1; i < 16; ++i) high = fminf(high, score[i]);
+                }
+                high *= scale;
                 high = halves_max(high);
-                if (h == 0) highs[half][col0 + c] = high;
-                if (t == 0) flags[~step & 1] = 0;
+                highs[half][col0 + c] = high;
+                flags[~step & 1] = 0;
                 const float own_top = col0 ? top[1] : top[0];
-                if (__any(high > own_top + kSlack) && lane == 0) flags[step & 1] = 1;
+                if (__any(high > own_top + kSlack)) flags[step & 1] = 1;
                 float added;
                 const auto exponentials = [&](float to) {
                     added = 0.0f;
@@ -331,7 +351,7 @@ template <bool FP4> __global__ __launch_bounds__(kThreads, 1) void latent_wide_k
                         const float a = __builtin_amdgcn_exp2f(fmaf(score[2 * i], scale, -to));
                         const float b = __builtin_amdgcn_exp2f(fmaf(score[2 * i + 1], scale, -to));
                         const bf16x2 r = {(__bf16)a, (__bf16)b};
-                        added += (float)r[0] + (float)r[1];
+                        added = __builtin_amdgcn_fdot2_f32_bf16(r, bf16x2{(__bf16)1.0f, (__bf16)1.0f}, added, false);
                         probs[i / 4][i % 4] = __builtin_bit_cast(unsigned, r);
                     }
 #pragma unroll
@@ -339,8 +359,32 @@ template <bool FP4> __global__ __launch_bounds__(kThreads, 1) void latent_wide_k
                         *(LdsPiece *)(base_lds + prob_at + col0 * kProbStride + 32 * (2 * half + m)) = probs[m];
                 };
                 exponentials(own_top == -INFINITY ? 0.0f : own_top);
+
+                // O; reads are a group ahead, the first values before all waves' P are there
+                u32x4 values[2][kTiles], probs[2][kColTiles];
+                const auto read_values = [&](int k) {
+#pragma unroll
+                    for (int j = 0; j < kTiles; ++j)
+#pragma unroll
+                        for (int u = 0; u < 2; ++u) {
+                            LdsByte *at = base_lds + (turned ^ (j * 64 | u * 32)) + (16 * k + 8 * u) * (kLatentMax * 2);
+                            const auto y = __builtin_bit_cast(unsigned long long, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                                                                                      (__attribute__((address_space(3))) s16x4 *)at));
+                            values[k % 2][j][2 * u] = (unsigned)y;
+                            values[k % 2][j][2 * u + 1] = (unsigned)(y >> 32);
+                        }
+                };
+                const auto read_probs = [&](int k) {
+#pragma unroll
+                    for (int x = 0; x < kColTiles; ++x)
+                        probs[k % 2][x] = *(const LdsPiece *)(base_lds + prob_at + 32 * x * kProbStride + 32 * k);
+                };
+                read_values(0);
                 meet_lds();
-                if (uniform(flags[step & 1])) {
+                const int flag = flags[step & 1];
+                read_probs(0);
+                asm volatile("" : "+v"(probs[0][0]), "+v"(probs[0][1]));  // (read with the flag, not after it)
+                if (uniform(flag)) {
                     const bool begun = __any(top[0] != -INFINITY || top[1] != -INFINITY);  // (else there is nothing yet, or NaN)
                     float by[2];
 #pragma unroll
@@ -363,39 +407,27 @@ template <bool FP4> __global__ __launch_bounds__(kThreads, 1) void latent_wide_k
                     const float to = col0 ? top[1] : top[0];
                     exponentials(to == -INFINITY ? 0.0f : to);
                     meet_lds();
+                    read_probs(0);
                 }
                 sum += added;
 
-                // O; again a group ahead
-                u32x4 values[2][kTiles], probs[2][kColTiles];
-                const auto read_values = [&](int k) {
-#pragma unroll
-                    for (int x = 0; x < kColTiles; ++x)
-                        probs[k % 2][x] = *(const LdsPiece *)(base_lds + prob_at + 32 * x * kProbStride + 32 * k);
-#pragma unroll
-                    for (int j = 0; j < kTiles; ++j)
-#pragma unroll
-                        for (int u = 0; u < 2; ++u) {
-                            LdsByte *at = base_lds + (turned ^ (j * 64 | u * 32)) + (16 * k + 8 * u) * (kLatentMax * 2);
-                            const auto y = __builtin_bit_cast(unsigned long long, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                                                                                      (__attribute__((address_space(3))) s16x4 *)at));
-                            values[k % 2][j][2 * u] = (unsigned)y;
-                            values[k % 2][j][2 * u + 1] = (unsigned)(y >> 32);
-                        }
-                };
-                read_values(0);
 #pragma unroll
                 for (int k = 0; k < kStepKeys / 16; ++k) {
-                    if (k + 1 < kStepKeys / 16) read_values(k + 1);
-#pragma unroll
-                    for (int j = 4 * k; j < 4 * k + 4; ++j) put(step + 1, j);
+                    if (k + 1 < kStepKeys / 16) {
+                        read_probs(k + 1);
+                        read_values(k + 1);
+                    }
                     __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-                    for (int j = 0; j < kTiles; ++j)
+                    for (int j = 0; j < kTiles; ++j) {
+                        if (k == 0 && j == 2) find(step + 2);
+                        if (k == 1 && j == 0) ask(step + 3);
 #pragma unroll
                         for (int x = 0; x < kColTiles; ++x)
                             out[j][x] = mfma(values[k % 2][j], probs[k % 2][x], out[j][x]);
-                    __builtin_amdgcn_sched_barrier(0);
+                        put(step + 1, 4 * k + j);
+                        __builtin_amdgcn_sched_barrier(0);
+                    }
                 }
             }
 
