@@ -159,6 +159,7 @@ template <class Til, int WAVES> __device__ __forceinline__ Run find_run(const Pa
     Run r;
     const LatentSeq mine = seq_of(t);
     int units = units_of(mine), all = units, total = 0;
+    if (t == 0) at[0] = p.b.seqs;  // (no sequence: starts that overlap could make more units than are counted)
     if (p.b.seqs <= kThreads) {
         held[t] = mine;
     } else {

@@ -405,8 +405,20 @@ template <bool FP4, bool BF16, bool FULL> int launch(const Params &p, hipStream_
 
 }  // namespace
 
-// Pairs a sequence from which the wide kernel is taken.
-constexpr int kWideFrom = 64;
+// Whether the wide kernel is taken, for bf16 queries: it reads keys once for 64 columns and not for
+// 16, and takes 25 us where there is next to nothing to do, the narrow one 15.  What the host
+// knows are the pairs, the sequences and the keys that a table holds.  Measured, wide and narrow,
+// in us, 3000 .. 4096 keys a sequence: bf16 keys, 4 sequences of 128 pairs 40 and 35, of 256 46 and
+// 49, of 512 45 and 62, of 2048 92 and 181; 16 of 48 44 and 41, of 64 44 and 45; 64 of 64 94 and
+// 101; 4-bit keys, 4 of 256 45 and 38, of 512 44 and 43, of 1024 56 and 65, of 2048 88 and 126; 32 of
+// 128 59 and 58; 64 of 64 72 and 58.  One sequence of 4096 pairs over 256 keys: bf16 27 and 22, 4
+// bits 27 and 17; one of 8192 pairs over 512 bf16 keys 39 and 55.  The queries come by copies of
+// 16 bytes.
+static bool wide_pays(const MlkLatentBatch &b, const LatentAttend &p) {
+    const long pairs = (long)p.rows * p.heads, few = b.type == MLK_FP4 ? 2 : 1;
+    return p.bf16 && b.latent == kLatentMax && b.rope == kLatentRopeMax && (reinterpret_cast<uintptr_t>(p.q) & 15) == 0 &&
+           pairs >= 64 * few * b.seqs && pairs >= 1024 * few && (long)b.table_width * b.page_size >= 512;
+}
 
 size_t latent_attend_workspace() { return kSumsBytes + kStatsBytes + kRecordBytes; }
 
@@ -418,9 +430,7 @@ int latent_attend(const MlkLatentBatch &b, const LatentAttend &p, int cu_count, 
     a.rows = p.rows;
     a.heads = p.heads;
     a.scale = p.scale * 1.44269504f;
-    const bool full = b.latent == kLatentMax && b.rope == kLatentRopeMax;
-    const bool wide = full && p.bf16 && (reinterpret_cast<uintptr_t>(p.q) & 15) == 0 &&
-                      (long)p.rows * p.heads >= (long)kWideFrom * b.seqs;
+    const bool wide = wide_pays(b, p);
     const int most_groups = wide ? Wide::kGroups : Narrow::kGroups;
     a.groups = cu_count < most_groups ? cu_count : most_groups;
     const long room = (long)b.table_width * b.page_size;
@@ -437,6 +447,7 @@ int latent_attend(const MlkLatentBatch &b, const LatentAttend &p, int cu_count, 
     a.parts.stats = reinterpret_cast<float *>(at + kSumsBytes);
     a.parts.records = reinterpret_cast<Record *>(at + kSumsBytes + kStatsBytes);
     if (wide) return launch_wide(b.type == MLK_FP4, a, stream);
+    const bool full = b.latent == kLatentMax && b.rope == kLatentRopeMax;
     if (b.type == MLK_FP4)
         return p.bf16 ? (full ? launch<true, true, true>(a, stream) : launch<true, true, false>(a, stream))
                       : (full ? launch<true, false, true>(a, stream) : launch<true, false, false>(a, stream));

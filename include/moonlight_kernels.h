@@ -212,7 +212,8 @@ int mlk_matmul_fp8_grouped(int out_type, const uint8_t *w, const float *ws,
  * Nothing out of range is read or written whatever they hold: a key whose page is
  * outside [0, pages), or behind the table's last page, is not written and makes
  * the rows that read it NaN; a sequence whose row_starts decrease or leave
- * [0, rows] has no rows.  Rows of no sequence are left as they were.
+ * [0, rows] has no rows.  Rows of no sequence are left as they were; what rows and
+ * slots hold that several sequences or rows claim is any of theirs.
  *
  * Limits: latent a multiple of 64 up to 512, rope a multiple of 16 up to 64;
  * data 16-byte aligned, other pointers to their values.  Calls queue on the library

@@ -281,20 +281,53 @@ def test_attend(device, workspace, dtype, cache_type, latent, rope, page, heads,
 
 @pytest.mark.parametrize("cache_type", [MLK_BF16, MLK_FP4])
 @pytest.mark.parametrize("page,heads,pairs,lead", [
-    (16, 16, [(64, 64)], 0),
-    (16, 16, [(4, 4)], 0),
-    (64, 16, [(127, 5), (128, 4), (129, 8), (0, 0), (1, 1), (63, 20)], 0),
-    (100, 5, [(300, 33), (40, 40)], 0),
-    (1, 128, [(65, 1), (200, 1)], 0),
-    (7, 40, [(2, 3), (90, 2), (0, 4)], 0),
-    (128, 16, [(1500, 40), (700, 8), (30, 30), (1100, 1)], 0),
-    (16, 1, [(150, 150)], 0),
-    (16, 16, [(90, 9)], 2)])
+    (16, 16, [(64, 64), (130, 66)], 0),
+    (16, 128, [(4, 4), (9, 9), (700, 5)], 16),
+    (64, 16, [(127, 45), (128, 40), (129, 38), (0, 0), (1, 1), (63, 20)], 0),
+    (100, 5, [(300, 293), (140, 140)], 0),
+    (1, 128, [(65, 1), (600, 16)], 0),
+    (7, 40, [(2, 3), (90, 52), (0, 4)], 0),
+    (128, 16, [(1500, 90), (700, 38), (30, 30), (1100, 1)], 0),
+    (16, 1, [(650, 650), (1600, 1450)], 0),
+    (16, 128, [(4000, 16)], 0),
+    (16, 16, [(140, 130)], 2)])
 def test_attend_many_pairs_a_sequence(device, workspace, cache_type, page, heads, pairs, lead):
     """Prompts in chunks, many heads; beside single rows and empty sequences."""
     rng = np.random.default_rng(page + heads + len(pairs))
-    cache = L.Cache(rng, cache_type, pairs, page_size=page, rows_behind=1).fill(rng)
+    cache = L.Cache(rng, cache_type, pairs, page_size=page, rows_behind=1, table_extra=512 // page + 1).fill(rng)
     check_attend(rng, cache, MLK_BF16, heads, workspace, lead=lead)
+
+
+@pytest.mark.parametrize("dtype,cache_type,latent,rope,heads,pairs", [
+    (MLK_F32, MLK_FP4, 64, 16, 128, [(300, 290), (20, 10)]),
+    (MLK_BF16, MLK_BF16, 64, 16, 128, [(300, 290), (20, 10)]),
+    (MLK_BF16, MLK_BF16, 512, 64, 128, [(70, 600), (90, 500)])])
+def test_attend_more_tiles_than_records(device, workspace, dtype, cache_type, latent, rope, heads, pairs):
+    rng = np.random.default_rng(28)
+    cache = L.Cache(rng, cache_type, pairs, latent, rope, table_extra=40).fill(rng)
+    q = rng.standard_normal((cache.rows, heads, latent + rope), dtype=F32)
+    check_attend(rng, cache, dtype, heads, workspace, q=q)
+
+
+@pytest.mark.parametrize("dtype,cache_type,latent,rope,rows", [
+    (MLK_F32, MLK_FP4, 64, 16, 4), (MLK_BF16, MLK_BF16, 512, 64, 40)])
+def test_attend_tables_of_2_to_the_31_keys(device, workspace, dtype, cache_type, latent, rope, rows):
+    """Steps of all keys that such tables hold are more than 32 bits count."""
+    rng = np.random.default_rng(29)
+    cache = L.Cache(rng, cache_type, [(100, rows), (70, 1)], latent, rope, 1 << 15, spare=0,
+                    table_extra=(1 << 16) - 1).fill(rng)
+    check_attend(rng, cache, dtype, 128, workspace)
+
+
+@pytest.mark.parametrize("cache_type", [MLK_BF16, MLK_FP4])
+def test_attend_sequences_that_share_pages(device, workspace, cache_type):
+    """A prefix that three sequences have in common, and a page twice in a table."""
+    rng = np.random.default_rng(33)
+    for heads, rows in ((16, 1), (16, 70)):
+        cache = L.Cache(rng, cache_type, [(96, rows)] * 3, table_extra=32).fill(rng)
+        cache.tables[1, :3] = cache.tables[2, :3] = cache.tables[0, :3]
+        cache.tables[1, 4] = cache.tables[1, 3]
+        check_attend(rng, cache, MLK_BF16, heads, workspace)
 
 
 @pytest.mark.parametrize("dtype", [MLK_F32, MLK_BF16])
@@ -319,14 +352,14 @@ def test_attend_many_short_sequences(device, workspace):
 def test_attend_sharp_and_flat_scores(device, workspace, dtype):
     """Scores in the hundreds, whose maximum moves late; all scores equal; a negative scale."""
     rng = np.random.default_rng(22)
-    cache = L.Cache(rng, MLK_BF16, [(400, 1)]).fill(rng)
+    cache = L.Cache(rng, MLK_BF16, [(400, 1)], table_extra=32).fill(rng)
     for j in range(400):  # ever larger rows
         cache.put(0, j, cache.get(0, j) * (0.2 + j / 200))
     check_attend(rng, cache, dtype, 16, workspace, scale=0.5)
     check_attend(rng, cache, dtype, 16, workspace, scale=-0.3)
     check_attend(rng, cache, dtype, 16, workspace, scale=0.0)
-    cache.starts = np.array([0, 6], np.int32)
-    cache.rows = 6
+    cache.starts = np.array([0, 70], np.int32)
+    cache.rows = 70
     for scale in (0.5, -0.3, 0.0):
         check_attend(rng, cache, dtype, 16, workspace, scale=scale)
 
@@ -342,14 +375,14 @@ def test_attend_unaligned_rows(device, workspace, dtype, cache_type):
 @pytest.mark.parametrize("cache_type", [MLK_BF16, MLK_FP4])
 @pytest.mark.parametrize("dtype", [MLK_F32, MLK_BF16])
 @pytest.mark.parametrize("bad", [np.nan, np.inf, -np.inf])
-@pytest.mark.parametrize("heads", [3, 40])
+@pytest.mark.parametrize("heads", [3, 160])
 def test_attend_values_that_are_not_finite(device, workspace, dtype, cache_type, bad, heads):
     """A key with such a value reaches the rows that see it, and those alone, in the
     latent row or in the rope row; so does a query."""
     rng = np.random.default_rng(24)
     for column in (100, 540):
         for at in (0, 20, 93, 99):
-            cache = L.Cache(rng, cache_type, [(100, 12), (40, 1)]).fill(rng)
+            cache = L.Cache(rng, cache_type, [(100, 12), (40, 1)], table_extra=32).fill(rng)
             clean = cache.get(0, at)
             v = clean.copy()
             v[column] = bad
@@ -364,7 +397,7 @@ def test_attend_values_that_are_not_finite(device, workspace, dtype, cache_type,
             told = ~np.isfinite(got[sees]).all((1, 2))
             # (an infinity in the rope row may make a score of -inf: the key has no weight)
             assert told.all() or (column == 540 and np.isinf(bad))
-    cache = L.Cache(rng, cache_type, [(100, 12), (40, 1)]).fill(rng)
+    cache = L.Cache(rng, cache_type, [(100, 12), (40, 1)], table_extra=32).fill(rng)
     q = rng.standard_normal((13, heads, 576))
     q[4, 1, 7] = bad
     got, _, _ = run_attend(rng, cache, dtype, heads, workspace, q=q)
@@ -375,12 +408,12 @@ def test_attend_values_that_are_not_finite(device, workspace, dtype, cache_type,
 
 @pytest.mark.parametrize("cache_type", [MLK_BF16, MLK_FP4])
 @pytest.mark.parametrize("dtype", [MLK_F32, MLK_BF16])
-@pytest.mark.parametrize("heads", [3, 40])
+@pytest.mark.parametrize("heads", [3, 160])
 def test_attend_pages_out_of_range(device, workspace, dtype, cache_type, heads):
     """Rows that read a key without a page are NaN, the others as they were; so with keys
     behind the table."""
     rng = np.random.default_rng(25)
-    cache = L.Cache(rng, cache_type, [(100, 30), (200, 1), (50, 2)], page_size=16).fill(rng)
+    cache = L.Cache(rng, cache_type, [(100, 30), (200, 1), (50, 2)], page_size=16, table_extra=32).fill(rng)
     good = cache.tables.copy()
     cache.tables[0, 5] = cache.pages       # keys 80 .. 95
     cache.tables[1, 3] = -1
@@ -391,26 +424,28 @@ def test_attend_pages_out_of_range(device, workspace, dtype, cache_type, heads):
     sees = np.array([s == 1 or (s == 0 and j >= 80) for _, s, j in cache.each_row()])
     assert np.isnan(got[sees]).all()
     assert np.all(np.abs(got - want)[~sees] <= room[~sees])
-    # the table of sequence 2 ends after 48 keys: its first row, key 48, sees one more
-    cache = L.Cache(rng, cache_type, [(48, 2)], page_size=16, table_extra=0).fill(rng)
-    cache.lengths[0] = 49
+    # a table that ends after 512 keys: the last row, key 512, sees one more
+    cache = L.Cache(rng, cache_type, [(512, 13)], page_size=16, table_extra=0).fill(rng)
+    cache.lengths[0] = 513
     got, q, scale = run_attend(rng, cache, dtype, heads, workspace)
-    cache.lengths[0] = 48
-    cache.starts = np.array([0, 1], np.int32)
+    cache.lengths[0] = 512
+    cache.starts = np.array([0, 12], np.int32)
     want, mass, score = L.attend(cache, q, heads, scale)
     room = L.attend_tolerance(cache, want, mass, score, dtype)
-    assert np.all(np.abs(got - want[:2])[0] <= room[0]) and np.isnan(got[1]).all()
+    assert np.all(np.abs(got - want)[:12] <= room[:12]) and np.isnan(got[12]).all()
 
 
-def test_attend_repeats_itself(device, workspace):
+@pytest.mark.parametrize("dtype,pairs", [(MLK_F32, [(900, 1), (3, 1), (400, 2)]),
+                                         (MLK_BF16, [(900, 100), (3, 1), (400, 60)])])
+def test_attend_repeats_itself(device, workspace, dtype, pairs):
     """The same call gives the same bits, whatever the workspace holds."""
     rng = np.random.default_rng(26)
-    cache = L.Cache(rng, MLK_FP4, [(900, 1), (3, 1), (400, 2)]).fill(rng)
-    q = rng.standard_normal((4, 16, 576))
-    first, _, _ = run_attend(rng, cache, MLK_F32, 16, workspace, q=q)
+    cache = L.Cache(rng, MLK_FP4, pairs).fill(rng)
+    q = rng.standard_normal((cache.rows, 16, 576))
+    first, _, _ = run_attend(rng, cache, dtype, 16, workspace, q=q)
     for fill in (0xFF, 0x00, 0x7F):
         workspace.upload(np.full(workspace.nbytes, fill, np.uint8))
-        again, _, _ = run_attend(rng, cache, MLK_F32, 16, workspace, q=q)
+        again, _, _ = run_attend(rng, cache, dtype, 16, workspace, q=q)
         assert np.array_equal(first, again)
 
 
