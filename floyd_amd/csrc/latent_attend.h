@@ -305,14 +305,15 @@ constexpr float kSlack = 24.0f;
 // Joins the tile of record blockIdx.x: its sums are in part 2 first + 1 and in parts 2w of
 // the workgroups w after the first.  128 threads take a column's values, and TEAMS such teams
 // share its parts: a round of loads from what other workgroups wrote takes about a
-// microsecond, so as many as can are under way at once, 16 a thread.  Where there are so many
-// records that not all of them are resident with four teams each, a tile has few parts, and a
-// thread asks for 4 at a time: what it asks for beyond the last part is read again for nothing
-// (128 tiles of 64 columns of two or three parts: 11.6 us, with 16 a thread 16.3).
+// microsecond, so as many as can are under way at once: four teams where all workgroups are
+// resident that way, and 16 loads a thread for the few tiles of small batches, whose parts are
+// many; else 4 loads, for what a thread asks for beyond the last part is read again for nothing
+// (17 tiles of about 15 parts 9.6 us with 16 loads, 6.1 with 4; 128 tiles of 64 columns and of two
+// or three parts 16.3 and 11.6).
 constexpr int kTeam = kLatentMax / 4;
 constexpr int kMaxTeams = 4;
-template <class Til, bool BF16, int TEAMS> __global__ __launch_bounds__((kTeam * TEAMS)) void latent_join_kernel(Params p) {
-    constexpr int kCols = Til::kCols, kThreads = kTeam * TEAMS, kLoads = TEAMS == 1 ? 4 : 16, kStride = kLoads * TEAMS;
+template <class Til, bool BF16, int TEAMS, int LOADS> __global__ __launch_bounds__((kTeam * TEAMS)) void latent_join_kernel(Params p) {
+    constexpr int kCols = Til::kCols, kThreads = kTeam * TEAMS, kLoads = LOADS, kStride = kLoads * TEAMS;
     __shared__ float tops[Til::kGroups], sums[Til::kGroups];
     __shared__ float reds[2][kThreads / kWave];
     __shared__ f32x4 shares[TEAMS][kTeam];
@@ -387,10 +388,13 @@ template <class Til, bool BF16, int TEAMS> __global__ __launch_bounds__((kTeam *
 template <class Til, bool BF16> int launch_join(const Params &p, hipStream_t stream) {
     if (p.groups == 1) return kOk;
     const int records = p.parts.tiles ? p.parts.tiles : p.groups;
-    if ((long)records * Til::kCols * kTeam * kMaxTeams <= (long)p.groups * 2048)
-        latent_join_kernel<Til, BF16, kMaxTeams><<<dim3(records, Til::kCols), kTeam * kMaxTeams, 0, stream>>>(p);
+    const dim3 grid(records, Til::kCols);
+    if ((long)records * Til::kCols * kTeam * kMaxTeams > (long)p.groups * 2048)
+        latent_join_kernel<Til, BF16, 1, 4><<<grid, kTeam, 0, stream>>>(p);
+    else if (records >= 16)
+        latent_join_kernel<Til, BF16, kMaxTeams, 4><<<grid, kTeam * kMaxTeams, 0, stream>>>(p);
     else
-        latent_join_kernel<Til, BF16, 1><<<dim3(records, Til::kCols), kTeam, 0, stream>>>(p);
+        latent_join_kernel<Til, BF16, kMaxTeams, 16><<<grid, kTeam * kMaxTeams, 0, stream>>>(p);
     return hipGetLastError() == hipSuccess ? kOk : kErrLaunch;
 }
 

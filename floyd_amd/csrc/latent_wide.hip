@@ -297,28 +297,30 @@ template <bool FP4> __global__ __launch_bounds__(kThreads, 1) void latent_wide_k
                     // does not see must not reach it by 0 * NaN either, so rows that are not finite
                     // (or not there) become zeros and make NaN of the scores of the columns that
                     // see them.
-                    int row_at = buf * kStepBytes + (kWaveKeys * half + c) * (kLatentMax * 2);
-                    asm volatile("" : "+v"(row_at));
+                    // (Each wave those that it brought; a row that others may still be reading for S
+                    // counts for nothing there.)
+                    int own_at = buf * kStepBytes + own_key * (kLatentMax * 2);
+                    asm volatile("" : "+v"(own_at));
                     u16x2 largest = {0, 0};
 #pragma unroll 8
-                    for (int j = 0; j < kLatentMax / 16; ++j) {  // (in an order that has lanes on all banks)
-                        const u32x4 v = *(const LdsPiece *)(base_lds + row_at + 16 * ((2 * j + h) ^ c % 16));
+                    for (int j = 0; j < kLatentMax / 32; ++j) {  // (in an order that has lanes on all banks)
+                        const u32x4 v = *(const LdsPiece *)(base_lds + own_at + 16 * ((4 * j + g) ^ c16));
 #pragma unroll
                         for (int i = 0; i < 4; ++i)
                             largest = __builtin_elementwise_max(largest, __builtin_bit_cast(u16x2, v[i] & 0x7FFF7FFFu));
                     }
-                    const bool finite = largest[0] < 0x7F80u && largest[1] < 0x7F80u;
-                    const bool seen = key0 + kWaveKeys * half + c < most;
-                    const unsigned long long which = __ballot(seen && !finite);
-                    const unsigned wrong = (unsigned)(which | which >> 32) | bads[buf][2 * half] | bads[buf][2 * half + 1] << 16;
-                    meet_lds();  // (both waves of a row have looked at it)
-                    if (!seen || (wrong >> c & 1u)) {
+                    const bool seen = key0 + own_key < most;
+                    const unsigned long long which = __ballot(seen && (largest[0] >= 0x7F80u || largest[1] >= 0x7F80u));
+                    const unsigned wrong = bads[buf][wave] |
+                                           ((unsigned)(which | which >> 16 | which >> 32 | which >> 48) & 0xFFFFu);
+                    if (!seen || (wrong >> c16 & 1u)) {
 #pragma unroll 8
-                        for (int j = 0; j < kLatentMax / 16; ++j)
-                            *(LdsPiece *)(base_lds + row_at + 16 * ((2 * j + h) ^ c % 16)) = u32x4{0, 0, 0, 0};
+                        for (int j = 0; j < kLatentMax / 32; ++j)
+                            *(LdsPiece *)(base_lds + own_at + 16 * ((4 * j + g) ^ c16)) = u32x4{0, 0, 0, 0};
                     }
+                    bads[buf][wave] = wrong;
                     meet_lds();
-                    const unsigned bits = wrong >> 4 * h;
+                    const unsigned bits = (bads[buf][2 * half] | bads[buf][2 * half + 1] << 16) >> 4 * h;
                     const int end = limit - (key0 + kWaveKeys * half + 4 * h);
 #pragma unroll
                     for (int i = 0; i < 16; ++i) {
