@@ -15,6 +15,10 @@ namespace mlh {
 constexpr int kLatentMax = 512;       // values of a latent row
 constexpr int kLatentRopeMax = 64;    // values of a rope row
 constexpr int kLatentMaxHeads = 1024;
+// A launch counts threads in 32 bits: a row of append is a workgroup, four of gather are.
+constexpr int kLatentRowThreads = 256, kLatentGatherRows = 4;
+constexpr int kLatentMaxAppend = 0xFFFFFFFFu / kLatentRowThreads;
+constexpr int kLatentMaxGather = kLatentMaxAppend * kLatentGatherRows;
 constexpr int kFp4Group = 32;         // values of a scale
 constexpr int kFp4ScaleBytes = 16;    // bytes of a row's scales
 constexpr int kFp4Bias = 127;         // of a scale byte; 255: its values are NaN
@@ -95,6 +99,7 @@ struct TokenLogprobs {
     float *top_logprobs = nullptr;
     void *workspace = nullptr;
 };
+bool token_logprobs_fits(int rows, int vocab);  // into a launch
 size_t token_logprobs_workspace(int rows, int vocab, int top);
 int token_logprobs(const TokenLogprobs &p, hipStream_t stream);
 

@@ -45,6 +45,7 @@ int mlk_latent_append(const MlkLatentBatch *batch, int type, const void *kv, lon
     const char *what = "mlk_latent_append";
     if (!type_ok(type)) return refuse(what, "type must be MLK_F32 or MLK_BF16");
     if (int e = check_batch(what, batch, rows)) return e;
+    if (rows > kLatentMaxAppend) return refuse(what, "rows must be below 2^24", kErrSize);
     if (kv_stride < batch->latent + batch->rope)
         return refuse(what, "kv_stride must be at least latent + rope");
     if (!(eps >= 0.0f) || isinf(eps)) return refuse(what, "eps must be finite and >= 0");
@@ -87,6 +88,7 @@ int mlk_latent_gather(const MlkLatentBatch *batch, int type, int rows, void *out
     const char *what = "mlk_latent_gather";
     if (!type_ok(type)) return refuse(what, "type must be MLK_F32 or MLK_BF16");
     if (int e = check_batch(what, batch, rows)) return e;
+    if (rows > kLatentMaxGather) return refuse(what, "rows must be at most 2^26 - 4", kErrSize);
     if (rows == 0 || batch->seqs == 0) return kOk;
     const Pointer list[] = {LATENT_BATCH_POINTERS(batch), {out, "out", size_of(type), false}};
     if (int e = check_pointers(what, list)) return e;
@@ -146,6 +148,8 @@ int mlk_token_logprobs(int type, const void *logits, long stride, int rows, int 
     if (top < 0 || top > kLogprobsMaxTop || top > vocab)
         return refuse(what, "top must be between 0 and 32, and at most vocab");
     if (rows == 0) return kOk;
+    if (!token_logprobs_fits(rows, vocab))
+        return refuse(what, "too many rows of so many logits for one launch", kErrSize);
     const size_t need = token_logprobs_workspace(rows, vocab, top);
     if (workspace_bytes < need)
         return refuse(what, "the workspace needs " + std::to_string(need) + " bytes");

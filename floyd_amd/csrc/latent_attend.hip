@@ -420,6 +420,8 @@ static bool wide_pays(const MlkLatentBatch &b, const LatentAttend &p) {
            pairs >= 64 * few * b.seqs && pairs >= 1024 * few && (long)b.table_width * b.page_size >= 512;
 }
 
+constexpr int kMostKeys = 0x7FFFFF80;  // (a step may begin behind the last one)
+
 size_t latent_attend_workspace() { return kSumsBytes + kStatsBytes + kRecordBytes; }
 
 int latent_attend(const MlkLatentBatch &b, const LatentAttend &p, int cu_count, hipStream_t stream) {
@@ -434,7 +436,7 @@ int latent_attend(const MlkLatentBatch &b, const LatentAttend &p, int cu_count, 
     const int most_groups = wide ? Wide::kGroups : Narrow::kGroups;
     a.groups = cu_count < most_groups ? cu_count : most_groups;
     const long room = (long)b.table_width * b.page_size;
-    a.keys = room < 0x7FFFFFFF ? (int)room : 0x7FFFFFFF;
+    a.keys = room < kMostKeys ? (int)room : kMostKeys;
     // units of more keys where there could be 2^31 of them (a tile has at least a column)
     const long tiles = (long)p.rows * p.heads / (wide ? Wide::kCols : Narrow::kCols) + b.seqs;
     const int step_shift = wide ? Wide::kStepShift : Narrow::kStepShift;

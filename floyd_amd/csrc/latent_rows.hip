@@ -19,6 +19,7 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kWaves = kThreads / kWave;
+static_assert(kThreads == kLatentRowThreads && kWaves == kLatentGatherRows, "the rows of a launch");
 
 template <bool BF16> struct Elem { using type = float; };
 template <> struct Elem<true> { using type = uint16_t; };

@@ -298,6 +298,11 @@ template <bool BF16, bool TOP> int launch(const TokenLogprobs &p, hipStream_t st
 
 }  // namespace
 
+bool token_logprobs_fits(int rows, int vocab) {
+    const long pieces = (vocab - 1) / (kThreads * values_of(rows, vocab)) + 1;
+    return pieces * rows <= 0xFFFFFFFFl / kThreads;
+}
+
 size_t token_logprobs_workspace(int rows, int vocab, int top) {
     const size_t pieces = (vocab - 1) / (kThreads * values_of(rows, vocab)) + 1;
     return pieces == 1 ? 0 : pieces * rows * (sizeof(Stats) + sizeof(Rank) * top);

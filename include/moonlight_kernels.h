@@ -212,10 +212,13 @@ int mlk_matmul_fp8_grouped(int out_type, const uint8_t *w, const float *ws,
  * Nothing out of range is read or written whatever they hold: a key whose page is
  * outside [0, pages), or behind the table's last page, is not written and makes
  * the rows that read it NaN; a sequence whose row_starts decrease or leave
- * [0, rows] has no rows.  Rows of no sequence are left as they were; what rows and
- * slots hold that several sequences or rows claim is any of theirs.
+ * [0, rows] has no rows, and rows of the others in such a batch are done or left.
+ * Rows of no sequence are left as they were; what a slot holds that several rows
+ * claim is one of theirs.
  *
- * Limits: latent a multiple of 64 up to 512, rope a multiple of 16 up to 64;
+ * Limits: latent a multiple of 64 up to 512, rope a multiple of 16 up to 64; a
+ * key from 2^31 - 128 on is behind any table for mlk_latent_attend; rows up to 2^24 - 1
+ * for mlk_latent_append (2^26 - 4 for mlk_latent_gather);
  * data 16-byte aligned, other pointers to their values.  Calls queue on the library
  * stream and return, as the fp8 entry points do, with the same rules for
  * pointers, other streams and overlap; they allocate nothing and keep nothing.
@@ -278,8 +281,8 @@ int mlk_latent_attend(const MlkLatentBatch *batch, int type, const void *q,
  * [0, vocab); entropy[r] (unless NULL) of the softmax in nats; top_ids and
  * top_logprobs [rows, top] (top 0 .. 32, at most vocab) the most likely tokens,
  * the lower index first among equal ones.  A logit of -inf has probability 0; a row
- * with a NaN, +inf or nothing above -inf has NaN for every result but the ids
- * (a NaN counts as the largest there).  Sums are 64 bits.  The workspace (device
+ * with a NaN, +inf or nothing above -inf has NaN for every result but the ids,
+ * from which NaNs are left out (-1 where no logit is left).  Sums are 64 bits.  The workspace (device
  * memory, 16-byte aligned) has at least mlk_token_logprobs_workspace() bytes; pointers,
  * streams and overlap as for the latent entry points. */
 size_t mlk_token_logprobs_workspace(int rows, int vocab, int top);

@@ -67,6 +67,9 @@ def test_batches_refused(call, bad, says):
     (append, dict(kv=P + 2), "kv is not aligned"),
     (append, dict(dtype=MLK_BF16, kv=P + 1), "kv is not aligned"),
     (append, dict(stride=575), "kv_stride"),
+    (append, dict(rows=1 << 24), "rows must be below"), (gather, dict(rows=(1 << 26) - 3), "rows must be at most"),
+    (logprobs, dict(rows=1 << 24, vocab=1, space=0), "too many rows"),
+    (logprobs, dict(rows=1 << 19, vocab=1 << 22, space=1 << 62), "too many rows"),
     (append, dict(norm_w=P + 2), "norm_w is not aligned"),
     (append, dict(inv_freq=None), "inv_freq is null"),
     (append, dict(inv_freq=P + 3), "inv_freq is not aligned"),
