@@ -3,11 +3,12 @@
 //
 //   s_j = scale * q . [latent_j | rope_j],  out = sum_j exp(s_j - m) latent_j / sum_j exp(s_j - m)
 //
-// for each (token row, head); a sequence's (row, head) pairs are taken 16 at a time
-// (a tile: the 16 columns of a matrix instruction), and a tile's keys 16 at a time (a
-// step, and a unit where those can be counted in 32 bits).  The units of all tiles, in order, are dealt out in equal runs to as many
-// workgroups as the chip holds, so ragged lengths leave none of them idle; a tile whose
-// units fell to several is joined by latent_join_kernel from their partial sums.
+// for each (token row, head); a sequence's (row, head) pairs are taken 16 at a time (a tile:
+// the 16 columns of a matrix instruction), and a tile's keys 16 at a time (a step, and a unit
+// of work where those can be counted in 32 bits).  The units of all tiles, in order, are
+// dealt out in equal runs to as many workgroups as the chip holds, so ragged lengths leave
+// none of them idle; a tile whose units fell to several is joined by latent_join_kernel from
+// their partial sums.
 //
 // The waves of a workgroup take its steps in turn, with a running maximum and sum of their
 // own, and meet at the end of a tile.  The keys are read straight into the matrix operand
@@ -18,7 +19,8 @@
 // identity, whose result registers hold 4 keys of a latent value, exact and to be packed.
 // (Through LDS, written in rows and read transposed, it is 16 KB of writes and as much of
 // reads a step: 4-bit keys took the same, bf16 ones 3 % less, and f32 queries, for which the
-// LDS then has room for four waves only, 13 % more.)
+// LDS then has room for four waves only, 13 % more.)  f32 queries and probabilities go in as
+// three bf16 parts each, which add up to them.
 //
 // The next keys are on their way from when the first product has taken the present ones, and
 // the page numbers of those after them.
@@ -26,6 +28,15 @@
 // What runs once costs its instructions' way from memory, about 4 cycles a byte: loops are
 // entered a step early rather than with a copy of their loads before them, and unrolled
 // only where registers are counted.
+//
+// Measured with 16 heads (this kernel, then the join): 16 rows over 16000 .. 16384 bf16 keys each
+// 62-65 and 6 us, 4.6-4.8 TB/s; a kernel that only reads the same rows, a key's 64 bytes by four
+// lanes, takes 54 and one that reads 1 KB runs 47-49: what bounds it is the reads, by the order
+// that the operand asks for, and the start.  64 rows over 4-bit keys, 159 MB, 48 and 6 us; reading
+// alone takes 31: two waves a SIMD whose products, codes' conversion and softmax, one after the
+// other, keep the matrix unit busy a third of the time.  One row over 4096 bf16 keys 10 and 5.5,
+// 17 rows of f32 queries over 4-bit keys 20 and 6: some seven trips to memory that depend on each
+// other, a microsecond each, with lengths and tables among them.
 #include "latent_attend.h"
 
 namespace mlh {
@@ -405,15 +416,15 @@ template <bool FP4, bool BF16, bool FULL> int launch(const Params &p, hipStream_
 
 }  // namespace
 
-// Whether the wide kernel is taken, for bf16 queries: it reads keys once for 64 columns and not for
-// 16, and takes 25 us where there is next to nothing to do, the narrow one 15.  What the host
-// knows are the pairs, the sequences and the keys that a table holds.  Measured, wide and narrow,
-// in us, 3000 .. 4096 keys a sequence: bf16 keys, 4 sequences of 128 pairs 40 and 35, of 256 46 and
-// 49, of 512 45 and 62, of 2048 92 and 181; 16 of 48 44 and 41, of 64 44 and 45; 64 of 64 94 and
-// 101; 4-bit keys, 4 of 256 45 and 38, of 512 44 and 43, of 1024 56 and 65, of 2048 88 and 126; 32 of
-// 128 59 and 58; 64 of 64 72 and 58.  One sequence of 4096 pairs over 256 keys: bf16 27 and 22, 4
-// bits 27 and 17; one of 8192 pairs over 512 bf16 keys 39 and 55.  The queries come by copies of
-// 16 bytes.
+// Whether the wide kernel is taken, for bf16 queries of full rows: it reads keys once for 64 columns
+// and not for 16, but begins and ends a tile more slowly.  The host knows the pairs, the sequences
+// and the keys that a table holds.  Calls in us, wide and narrow, 3000 .. 4096 keys a sequence:
+//   bf16 keys   4 sequences of 128 pairs 40 and 35, of 256 46 and 49, of 512 45 and 62, of 2048
+//               92 and 181; 16 of 48 44 and 41, of 64 44 and 45; 64 of 64 94 and 101
+//   4-bit keys  4 of 256 45 and 38, of 512 44 and 43, of 1024 56 and 65, of 2048 86 and 126;
+//               32 of 128 59 and 58; 64 of 64 72 and 58
+// One sequence of 4096 pairs over 256 keys: bf16 27 and 22, 4 bits 27 and 17; of 8192 pairs over
+// 512 bf16 keys 39 and 55.  Queries at 16-byte addresses, which it copies so.
 static bool wide_pays(const MlkLatentBatch &b, const LatentAttend &p) {
     const long pairs = (long)p.rows * p.heads, few = b.type == MLK_FP4 ? 2 : 1;
     return p.bf16 && b.latent == kLatentMax && b.rope == kLatentRopeMax && (reinterpret_cast<uintptr_t>(p.q) & 15) == 0 &&
