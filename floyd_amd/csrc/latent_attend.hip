@@ -34,7 +34,7 @@
 // lanes, takes 54 and one that reads 1 KB runs 47-49: what bounds it is the reads, by the order
 // that the operand asks for, and the start.  64 rows over 4-bit keys, 159 MB, 48 and 6 us; reading
 // alone takes 31: two waves a SIMD whose products, codes' conversion and softmax, one after the
-// other, keep the matrix unit busy a third of the time.  One row over 4096 bf16 keys 10 and 5.5,
+// other, keep the matrix unit busy a quarter of the time.  One row over 4096 bf16 keys 10 and 5.5,
 // 17 rows of f32 queries over 4-bit keys 20 and 6: some seven trips to memory that depend on each
 // other, a microsecond each, with lengths and tables among them.
 #include "latent_attend.h"
