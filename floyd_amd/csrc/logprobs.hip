@@ -34,9 +34,11 @@ namespace {
 constexpr int kThreads = 256;
 constexpr int kWaves = kThreads / kWave;
 constexpr int kFew = 8, kMany = 32;  // values a thread holds
-// Pieces of kMany values a thread, where that gives the chip's 256 CUs two workgroups each: 512
-// bf16 rows of 163840 take 41 us so, 60 with kFew; one f32 row 11.3 with kFew, 12.9 with kMany.
-constexpr long kManyFrom = 512;
+// Pieces of kMany values a thread, where that gives the chip's 256 CUs a workgroup each.  Calls in
+// us with kMany and kFew: 512 bf16 rows of 163840 41 and 60; 61 f32 rows of 50021 (427 pieces of
+// kMany) 10.1 and 11.5, with 20 likely tokens 17.1 and 17.4, with 32 19 and 27; 30 such rows
+// (210) with 20 16.5 and 15; one f32 row of 163840 12.9 and 11.3.
+constexpr long kManyFrom = 256;
 
 typedef u32x4 u32x4_any __attribute__((aligned(2)));
 typedef unsigned long long Rank;  // value, then the lower index first; 0: none
