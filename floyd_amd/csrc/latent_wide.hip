@@ -21,8 +21,9 @@
 // the two, the way of P through LDS with its two meetings, and bf16 rows' copies, which S waits
 // for here and there (36 products 2100 cycles, over 4-bit keys 1500); of a workgroup's 28 steps
 // the beginning takes 4 us (queries, pages and first keys), an edge 3, the 128 KB of a part 3.5.
-// Copies in the second product's time, more operands ahead and the exponentials' registers held
-// apart from the accumulators' made nothing of it faster.
+// Copies in the second product's time and more operands ahead made nothing of it faster; steps of
+// 32 keys in three places, with the softmax beside the second product's instructions and one
+// meeting a step, took 80 us: what a step waits for at its beginning then comes twice as often.
 #include "latent_attend.h"
 
 namespace mlh {
