@@ -19,8 +19,8 @@
 // the vector units do of bf16 logits in the time that the memory takes to bring them.
 //
 // Measured, pieces and join: 512 bf16 rows of 163840 logits 34 and 5 us (4.9 TB/s, what a copy
-// of memory reaches), 61 f32 rows of 50021 with 20 likely tokens 11.4 and 6.2 (5.0 and 3.2
-// without: the vector units, in what it takes to choose and order 20 of a piece), one f32 row of
+// of memory reaches), 61 f32 rows of 50021 with 20 likely tokens 12 and 5.4 (without them 10 in
+// all: the vector units, in what it takes to choose and order 20 of a piece), one f32 row of
 // 163840 with 5 likely tokens 5.6 and 5.0 (two launches and the trips to memory of each).
 #include "bf16.h"
 #include "latent.h"
