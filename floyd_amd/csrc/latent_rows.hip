@@ -49,28 +49,31 @@ template <bool BF16> __device__ __forceinline__ Pair<BF16> load_pair(const typen
     return v;
 }
 
-// The sequence of token row r (b.seqs: none), by every lane of a wave: the number of
-// sequences that end at r or before.
-__device__ __forceinline__ int seq_of_row(const MlkLatentBatch &b, int r) {
-    if (!b.row_starts) return r < b.seqs ? r : b.seqs;
-    int before = 0;
-    for (int s0 = 0; s0 < b.seqs; s0 += kWave) {
-        const int s = s0 + (int)(threadIdx.x % kWave);
-        const bool ends = s < b.seqs && b.row_starts[s + 1] <= r;
-        before += __popcll(__ballot(ends));
-    }
-    return before;
-}
-
-// Key position of token row r (below 0: padding) and its place in the pages (-1: none);
-// false: r is no row of a sequence.
+// Key position of token row r (below 0: padding) and its place in the pages (-1: none), by every
+// lane of a wave; false: r is no row of a sequence.  Its sequence is the number of those that end
+// at r or before; their starts and lengths, 64 sequences at a time, are asked for together.
 __device__ __forceinline__ bool place_of_row(const MlkLatentBatch &b, int r, int rows, int *position,
                                              long *slot) {
-    const int s = seq_of_row(b, r);
-    if (s >= b.seqs) return false;
-    const LatentSeq q = latent_seq(b, s, rows);
-    if (r < q.begin || r >= q.begin + q.count) return false;
-    const long j = (long)q.length - (q.begin + q.count - r);
+    int s = r, begin = r, end = r + 1, length = 0;
+    if (!b.row_starts) {
+        if (r >= b.seqs) return false;
+        length = b.lengths[r];
+    } else {
+        const int lane = (int)(threadIdx.x % kWave);
+        int before = kWave;
+        for (int s0 = 0; before == kWave; s0 += kWave) {
+            if (s0 >= b.seqs) return false;
+            const int mine = s0 + lane < b.seqs ? s0 + lane : b.seqs - 1;
+            const int first = b.row_starts[mine], last = b.row_starts[mine + 1], n = b.lengths[mine];
+            before = __popcll(__ballot(s0 + lane < b.seqs && last <= r));
+            s = s0 + before;
+            begin = __builtin_amdgcn_readlane(first, before % kWave);
+            end = __builtin_amdgcn_readlane(last, before % kWave);
+            length = __builtin_amdgcn_readlane(n, before % kWave);
+        }
+        if (s >= b.seqs || begin < 0 || end > rows || r < begin || r >= end) return false;
+    }
+    const long j = (long)length - (end - r);
     *position = j < 0 ? -1 : (int)j;
     *slot = j < 0 ? -1 : latent_slot(b, s, (unsigned)j);
     return true;
@@ -138,7 +141,7 @@ __device__ __forceinline__ unsigned row_max(unsigned v) {
 }
 
 // One token row a workgroup.  What it reads of the row is asked for at once, beside the way to
-// its place (starts, then length and table, a microsecond each).  Queries: 32 threads for the
+// its place (starts and length, then table, a microsecond each).  Queries: 32 threads for the
 // pairs of a head, 8 heads a pass.  4095 bf16 rows with 16 heads into 4 bits, 29 MB, take 13-14 us
 // (2.1 TB/s; the library's sine and cosine, loads in turn and codes in 64 bits 19): what bounds it
 // is 64-bit arithmetic, at a half to a quarter of 32 bits' rate, and what each workgroup waits for
@@ -238,7 +241,7 @@ __global__ __launch_bounds__(kThreads) void latent_append_kernel(MlkLatentBatch 
 typedef unsigned u32x4_any __attribute__((ext_vector_type(4), aligned(2)));
 
 // One token row a wave, 8 values a lane and step.  67 MB of ragged f32 rows 14 us (4.8 TB/s; a large
-// copy reaches 5.1), 8192 rows of 4 bits, 13 MB, 5.7 (the way to a row and from it, four trips).
+// copy reaches 5.1), 8192 rows of 4 bits, 13 MB, 5.3 (the way to a row and from it, three trips).
 template <bool BF16, bool FP4>
 __global__ __launch_bounds__(kThreads) void latent_gather_kernel(MlkLatentBatch b, int rows, void *to) {
     using T = typename Elem<BF16>::type;
