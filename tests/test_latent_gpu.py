@@ -102,6 +102,26 @@ def test_append_many_sequences_one_row_each(device, cache_type):
     run_append(rng, cache, MLK_F32, heads=1)
 
 
+@pytest.mark.parametrize("seqs", [64, 65, 128, 300])
+def test_rows_of_many_sequences(device, workspace, seqs):
+    """Appended, read back and attended to by starts of more sequences than a wave has lanes,
+    some of them without rows, the last ones among them."""
+    rng = np.random.default_rng(seqs)
+    counts = rng.integers(0, 4, seqs)
+    counts[-3:] = 0
+    pairs = [(int(n) + int(rng.integers(0, 9)), int(n)) for n in counts]
+    cache = L.Cache(rng, MLK_FP4, pairs, 64, 16, 4, rows_behind=3)
+    run_append(rng, cache, MLK_F32, heads=1)
+    cache.fill(rng)
+    out = Out(cache.rows * 80 * 4)
+    native.latent_gather(cache.upload(), MLK_F32, out.ptr, cache.rows)
+    got = out.get(F32, (cache.rows, 80))
+    for r, s, j in cache.each_row():
+        np.testing.assert_array_equal(got[r], cache.get(s, j))
+    assert np.all(got[cache.starts[-1]:].view(np.uint8) == out.fill)
+    check_attend(rng, cache, MLK_F32, 2, workspace)
+
+
 @pytest.mark.parametrize("cache_type", [MLK_BF16, MLK_FP4])
 def test_append_without_norm_or_queries(device, cache_type):
     rng = np.random.default_rng(5)
