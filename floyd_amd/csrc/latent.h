@@ -100,7 +100,8 @@ struct TokenLogprobs {
     void *workspace = nullptr;
 };
 bool token_logprobs_fits(int rows, int vocab);  // into a launch
-size_t token_logprobs_workspace(int rows, int vocab, int top);
+size_t token_logprobs_needs(int rows, int vocab, int top);      // of a call
+size_t token_logprobs_workspace(int rows, int vocab, int top);  // of it and all smaller ones
 int token_logprobs(const TokenLogprobs &p, hipStream_t stream);
 
 }  // namespace mlh

@@ -150,7 +150,7 @@ int mlk_token_logprobs(int type, const void *logits, long stride, int rows, int 
     if (rows == 0) return kOk;
     if (!token_logprobs_fits(rows, vocab))
         return refuse(what, "too many rows of so many logits for one launch", kErrSize);
-    const size_t need = token_logprobs_workspace(rows, vocab, top);
+    const size_t need = token_logprobs_needs(rows, vocab, top);
     if (workspace_bytes < need)
         return refuse(what, "the workspace needs " + std::to_string(need) + " bytes");
     const unsigned size = size_of(type);

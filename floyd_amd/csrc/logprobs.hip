@@ -336,9 +336,21 @@ bool token_logprobs_fits(int rows, int vocab) {
     return pieces * rows <= 0xFFFFFFFFl / kThreads;
 }
 
-size_t token_logprobs_workspace(int rows, int vocab, int top) {
+static size_t piece_bytes(int top) { return sizeof(Stats) + sizeof(Rank) * top; }
+
+size_t token_logprobs_needs(int rows, int vocab, int top) {
     const size_t pieces = (vocab - 1) / (kThreads * values_of(rows, vocab)) + 1;
-    return pieces == 1 ? 0 : pieces * rows * (sizeof(Stats) + sizeof(Rank) * top);
+    return pieces == 1 ? 0 : pieces * rows * piece_bytes(top);
+}
+
+// Of any call of at most `rows` rows of `vocab` logits: pieces of kFew values are taken while
+// those of kMany are fewer than kManyFrom in all, so they are at most kMany / kFew times as many.
+size_t token_logprobs_workspace(int rows, int vocab, int top) {
+    const size_t many = (vocab - 1) / (kThreads * kMany) + 1, few = (vocab - 1) / (kThreads * kFew) + 1;
+    constexpr size_t kMostFew = kMany / kFew * (kManyFrom - 1);
+    const size_t of_few = few == 1 ? 0 : few * rows < kMostFew ? few * rows : kMostFew;
+    const size_t of_many = many == 1 ? 0 : many * rows;
+    return (of_few > of_many ? of_few : of_many) * piece_bytes(top);
 }
 
 int token_logprobs(const TokenLogprobs &p, hipStream_t stream) {

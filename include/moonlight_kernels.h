@@ -283,7 +283,8 @@ int mlk_latent_attend(const MlkLatentBatch *batch, int type, const void *q,
  * the lower index first among equal ones.  A logit of -inf has probability 0; a row
  * with a NaN, +inf or nothing above -inf has NaN for every result but the ids,
  * from which NaNs are left out (-1 where no logit is left).  Sums are 64 bits.  The workspace (device
- * memory, 16-byte aligned) has at least mlk_token_logprobs_workspace() bytes; pointers,
+ * memory, 16-byte aligned) has at least mlk_token_logprobs_workspace() bytes, which never
+ * fall as rows, vocab or top grow: one of the largest call's serves the smaller ones.  Pointers,
  * streams and overlap as for the latent entry points. */
 size_t mlk_token_logprobs_workspace(int rows, int vocab, int top);
 int mlk_token_logprobs(int type, const void *logits, long stride, int rows,

@@ -146,6 +146,29 @@ def test_workspaces():
     assert 0 < native.token_logprobs_workspace(4, 163840, 20) < 1 << 20
 
 
+def test_logprobs_workspace_serves_smaller_calls():
+    """It never falls as rows, vocabulary or top grow, and no call of at most as many of each asks
+    for more."""
+    size = native.token_logprobs_workspace
+    vocabs = [1, 300, 2048, 2049, 8192, 8193, 16385, 50021, 131072, 163840, 262144, 1 << 20, 2 << 20, 1 << 22]
+    for top in (0, 20):
+        for vocab in vocabs:
+            sizes = [size(rows, vocab, top) for rows in range(1, 700)]
+            assert sizes == sorted(sizes), vocab
+        for rows in (1, 2, 3, 12, 13, 36, 37, 60, 255, 256, 600):
+            sizes = [size(rows, vocab, top) for vocab in vocabs + list(range(1900, 100000, 700))]
+            assert sizes[:len(vocabs)] == sorted(sizes[:len(vocabs)]), rows
+            assert sizes[len(vocabs):] == sorted(sizes[len(vocabs):]), rows
+    for rows, vocab, top in ((13, 163840, 20), (64, 50021, 20), (300, 8200, 32), (300, 8192, 5), (1, 1 << 22, 32)):
+        space = size(rows, vocab, top)
+        assert size(rows, vocab, top - 1) <= space
+        for fewer in {1, 2, 12, 36, 255, 256, rows - 1, rows} & set(range(1, rows + 1)):
+            for less in {vocab, vocab // 2 + 1, min(vocab, 8193), min(vocab, 2049), min(vocab, 40)}:
+                for some in (0, top):
+                    with pytest.raises(NativeError, match="no HIP device|not device memory"):
+                        logprobs(rows=fewer, vocab=less, top=some, top_ids=P, top_logprobs=P, space=space)
+
+
 @pytest.mark.gpu
 def test_host_memory_is_refused(device):
     d = native.DeviceBuffer(1 << 20)

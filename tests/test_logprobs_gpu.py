@@ -185,3 +185,25 @@ def test_greedy_sampler_takes_the_first(device):
     _, _, ids, _ = check(MLK_F32, x, [0], 5)
     xb, at = put(x.astype(F32))
     assert native.sample(at, 163840, 0.0, 1.0, 0.0) == ids[0, 0]
+
+
+@pytest.mark.parametrize("dtype", [MLK_F32, MLK_BF16])
+@pytest.mark.parametrize("most,vocab", [(40, 50021), (13, 163840), (300, 8200)])
+def test_one_workspace_for_batches_that_shrink(device, dtype, most, vocab):
+    """The largest batch's workspace serves fewer rows, by whichever pieces these are taken."""
+    rng = np.random.default_rng(10)
+    top = 20
+    space = DeviceBuffer(native.token_logprobs_workspace(most, vocab, top))
+    raw, x = L.typed(dtype, rng.standard_normal((most, vocab)))
+    tokens = rng.integers(0, vocab, most)
+    xb, xat = put(raw)
+    tb, tat = put(tokens.astype(np.int32))
+    for rows in [r for r in (most, 255, 36, 12, 3, 1) if r <= most]:
+        lp, ids, tops = Out(4 * rows), Out(4 * rows * top), Out(4 * rows * top)
+        native.token_logprobs(dtype, xat, rows, vocab, tat, lp.ptr, space, top=top, top_ids=ids.ptr,
+                              top_logprobs=tops.ptr)
+        want = exact(x[:rows], tokens[:rows], top)
+        np.testing.assert_array_equal(ids.get(np.int32, (rows, top)), want[2])
+        # as in check(): log p is off by half a last place of it and 252 * 2^-24
+        for got, ref in ((lp.get(F32, rows), want[0]), (tops.get(F32, (rows, top)), want[3])):
+            assert np.all(np.abs(got - ref) <= U.HALF_F32 * (np.abs(ref) + 252) + 1e-13)
