@@ -24,6 +24,12 @@ constexpr int kFp4ScaleBytes = 16;    // bytes of a row's scales
 constexpr int kFp4Bias = 127;         // of a scale byte; 255: its values are NaN
 constexpr int kFp4LeastExp = -100;    // (far from bf16's subnormals)
 
+// Launches of `kernel` may ask for so much LDS beside its static arrays (else 64 KB).
+template <class Kernel> inline bool allow_lds(Kernel kernel, int bytes) {
+    return hipFuncSetAttribute(reinterpret_cast<const void *>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize,
+                               bytes) == hipSuccess;
+}
+
 __host__ __device__ constexpr bool latent_widths_ok(int latent, int rope) {
     return latent > 0 && latent <= kLatentMax && latent % 64 == 0 && rope > 0 &&
            rope <= kLatentRopeMax && rope % 16 == 0;
@@ -88,6 +94,7 @@ int latent_attend(const MlkLatentBatch &b, const LatentAttend &p, int cu_count, 
 
 // Log probabilities of rows of logits (logprobs.hip).
 constexpr int kLogprobsMaxTop = 32;
+constexpr int kLogprobsMaxVocab = 1 << 22;
 struct TokenLogprobs {
     bool bf16 = false;
     const void *logits = nullptr;

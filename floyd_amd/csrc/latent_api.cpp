@@ -10,7 +10,6 @@ using namespace mlh;
 namespace {
 
 constexpr long kMaxPairs = 0x7FFFFFFF - 15;  // (row, head) pairs, counted in 32 bits
-constexpr int kMaxVocab = 1 << 22;
 
 int check_batch(const char *what, const MlkLatentBatch *b, int rows) {
     if (!b) return refuse(what, "batch is null");
@@ -132,7 +131,7 @@ int mlk_latent_attend(const MlkLatentBatch *batch, int type, const void *q, void
 }
 
 size_t mlk_token_logprobs_workspace(int rows, int vocab, int top) {
-    if (rows <= 0 || vocab <= 0 || vocab > kMaxVocab || top < 0 || top > kLogprobsMaxTop) return 0;
+    if (rows <= 0 || vocab <= 0 || vocab > kLogprobsMaxVocab || top < 0 || top > kLogprobsMaxTop) return 0;
     return token_logprobs_workspace(rows, vocab, top);
 }
 
@@ -143,7 +142,7 @@ int mlk_token_logprobs(int type, const void *logits, long stride, int rows, int 
     if (!type_ok(type)) return refuse(what, "type must be MLK_F32 or MLK_BF16");
     if (rows < 0) return refuse(what, "rows must be >= 0");
     if (vocab <= 0) return refuse(what, "vocab must be > 0");
-    if (vocab > kMaxVocab) return refuse(what, "vocab must be at most 2^22", kErrSize);
+    if (vocab > kLogprobsMaxVocab) return refuse(what, "vocab must be at most 2^22", kErrSize);
     if (stride < vocab) return refuse(what, "stride must be at least vocab");
     if (top < 0 || top > kLogprobsMaxTop || top > vocab)
         return refuse(what, "top must be between 0 and 32, and at most vocab");

@@ -387,11 +387,6 @@ template <class Til, bool BF16> int launch_join(const Params &p, hipStream_t str
     return hipGetLastError() == hipSuccess ? kOk : kErrLaunch;
 }
 
-template <class Kernel> bool allow_lds(Kernel kernel, int bytes) {
-    return hipFuncSetAttribute(reinterpret_cast<const void *>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize,
-                               bytes) == hipSuccess;
-}
-
 // The kernel for many (row, head) pairs a sequence, bf16 queries and full rows (latent_wide.hip).
 int launch_wide(bool fp4, const Params &p, hipStream_t stream);
 

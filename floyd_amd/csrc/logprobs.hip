@@ -310,17 +310,31 @@ int values_of(int rows, int vocab) {
     return pieces * rows >= kManyFrom ? kMany : kFew;
 }
 
+// Ranks that the join of so many pieces may have to put in order: of the threads that reach the
+// bound, at most `top` of a wave, all that they hold.
+constexpr size_t most_found(size_t pieces, size_t top) {
+    const size_t n = pieces * top, reach = kWaves * top * ((n + kThreads - 1) / kThreads);
+    return n < reach ? n : reach;
+}
+// A call's pieces of kFew values, which are taken while those of kMany are fewer than kManyFrom; a
+// row's of kMany.
+constexpr size_t kMostFew = kMany / kFew * (kManyFrom - 1), kMostMany = kLogprobsMaxVocab / (kThreads * kMany);
+constexpr size_t kMostFound = most_found(kMostFew > kMostMany ? kMostFew : kMostMany, kLogprobsMaxTop);
+static_assert(sizeof(Rank) * kMostFound <= 128 << 10, "LDS, of 160 KB with the join's own arrays");
+
 template <bool BF16, bool TOP, int N> int launch(const TokenLogprobs &p, hipStream_t stream) {
     const int pieces = (p.vocab - 1) / (kThreads * N) + 1;
     const size_t blocks = (size_t)pieces * p.rows;
     Stats *stats = static_cast<Stats *>(p.workspace);
     Rank *ranks = reinterpret_cast<Rank *>(stats + blocks);
+    if (TOP && pieces > 1) {
+        static const bool ok = allow_lds(logprobs_join_kernel<true>, sizeof(Rank) * kMostFound);
+        if (!ok) return kErrLaunch;
+    }
     logprobs_piece_kernel<BF16, TOP, N><<<(unsigned)blocks, kThreads, 0, stream>>>(p, pieces, stats, ranks);
     if (hipGetLastError() != hipSuccess) return kErrLaunch;
     if (pieces == 1) return kOk;
-    // ranks of the threads that reach the bound: at most `top` of a wave, and all of n
-    const size_t n = (size_t)pieces * p.top, reach = kWaves * p.top * ((n - 1) / kThreads + 1);
-    const size_t found = TOP ? sizeof(Rank) * (n < reach ? n : reach) : 0;
+    const size_t found = TOP ? sizeof(Rank) * most_found(pieces, p.top) : 0;
     logprobs_join_kernel<TOP><<<p.rows, kThreads, found, stream>>>(p, pieces, stats, ranks);
     return hipGetLastError() == hipSuccess ? kOk : kErrLaunch;
 }
@@ -343,11 +357,9 @@ size_t token_logprobs_needs(int rows, int vocab, int top) {
     return pieces == 1 ? 0 : pieces * rows * piece_bytes(top);
 }
 
-// Of any call of at most `rows` rows of `vocab` logits: pieces of kFew values are taken while
-// those of kMany are fewer than kManyFrom in all, so they are at most kMany / kFew times as many.
+// Of any call of at most `rows` rows of `vocab` logits.
 size_t token_logprobs_workspace(int rows, int vocab, int top) {
     const size_t many = (vocab - 1) / (kThreads * kMany) + 1, few = (vocab - 1) / (kThreads * kFew) + 1;
-    constexpr size_t kMostFew = kMany / kFew * (kManyFrom - 1);
     const size_t of_few = few == 1 ? 0 : few * rows < kMostFew ? few * rows : kMostFew;
     const size_t of_many = many == 1 ? 0 : many * rows;
     return (of_few > of_many ? of_few : of_many) * piece_bytes(top);

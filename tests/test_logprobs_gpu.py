@@ -207,3 +207,16 @@ def test_one_workspace_for_batches_that_shrink(device, dtype, most, vocab):
         # as in check(): log p is off by half a last place of it and 252 * 2^-24
         for got, ref in ((lp.get(F32, rows), want[0]), (tops.get(F32, (rows, top)), want[3])):
             assert np.all(np.abs(got - ref) <= U.HALF_F32 * (np.abs(ref) + 252) + 1e-13)
+
+
+@pytest.mark.parametrize("dtype", [MLK_F32, MLK_BF16])
+@pytest.mark.parametrize("rows,vocab", [(1, 2000000), (1, 2088960), (2, 1000001), (1, 1 << 22), (3, 1 << 21)])
+def test_widest_vocabularies_with_most_alternatives(device, dtype, rows, vocab):
+    """Up to 1020 small pieces, or 512 large ones, whose likely tokens are put in order together;
+    many of them are equal."""
+    rng = np.random.default_rng(11)
+    x = np.round(8 * 2.5 * rng.standard_normal((rows, vocab))) / 8
+    check(dtype, x, rng.integers(0, vocab, rows), 32)
+    x[:] = -1.0
+    x[:, ::5] = 2.0
+    check(dtype, x, rng.integers(0, vocab, rows), 32)
