@@ -264,6 +264,11 @@ __global__ __launch_bounds__((kWavesOf<FP4> * kWave), 1) void latent_attend_kern
                         hidden[i] = key0 + 4 * g + i >= limit;
                     }
                 }
+                if (__any(fmaxf(fmaxf(fabsf(sc[0]), fabsf(sc[1])), fmaxf(fabsf(sc[2]), fabsf(sc[3]))) * fabsf(p.scale) == INFINITY)) {
+                    // (a score of -inf would be a key without weight)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) sc[i] = fabsf(sc[i] * p.scale) < INFINITY ? sc[i] : NAN;
+                }
                 float high = -INFINITY;
 #pragma unroll
                 for (int i = 0; i < 4; ++i) high = fmaxf(high, hidden[i] ? -INFINITY : sc[i] * p.scale);

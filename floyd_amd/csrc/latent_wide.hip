@@ -302,6 +302,15 @@ template <bool FP4> __global__ __launch_bounds__(kThreads, 1) void latent_wide_k
                 }
 
                 float scale = p.scale;
+                float high = score[0], low = score[0];
+#pragma unroll
+                for (int i = 1; i < 16; ++i) high = fmaxf(high, score[i]), low = fminf(low, score[i]);
+                if (__any(fmaxf(fabsf(high), fabsf(low)) * fabsf(scale) == INFINITY)) {
+                    // (a score of -inf would be a key without weight)
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) score[i] = fabsf(score[i] * scale) < INFINITY ? score[i] : NAN;
+                }
+                high = scale >= 0 ? high * scale : low * scale;
                 const unsigned bad = (unsigned)uniform((int)(bad4[0] | bad4[1] | bad4[2] | bad4[3]));
                 if (bad || key0 + kStepKeys > least) {
                     // Keys that not every column sees, or that have no place: those that a column
@@ -340,16 +349,10 @@ template <bool FP4> __global__ __launch_bounds__(kThreads, 1) void latent_wide_k
                         if (k >= end) score[i] = -INFINITY;
                     }
                     scale = 1.0f;
-                }
-                float high = score[0];
-                if (scale >= 0) {
+                    high = score[0];
 #pragma unroll
                     for (int i = 1; i < 16; ++i) high = fmaxf(high, score[i]);
-                } else {
-#pragma unroll
-                    for (int i = 1; i < 16; ++i) high = fminf(high, score[i]);
                 }
-                high *= scale;
                 high = halves_max(high);
                 highs[half][col0 + c] = high;
                 flags[~step & 1] = 0;

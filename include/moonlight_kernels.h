@@ -267,8 +267,9 @@ int mlk_latent_gather(const MlkLatentBatch *batch, int type, int rows, void *out
  * [rows, heads, latent] are of `type`.  Scores, sums and results are f32; with
  * MLK_BF16 the p of a key is rounded to bf16 before it is multiplied with its
  * row (the softmax's sum is that of the rounded ones), with MLK_F32 nothing is.
- * A NaN or an infinity in a key's row makes NaN of values of the rows that see it and of no
- * others.  The workspace has at least mlk_latent_attend_workspace() bytes
+ * A NaN or an infinity in a key's row makes NaN of every result of the rows that see it, and of
+ * no others; one in a query, or a score beyond f32, makes NaN of that head's results where a key
+ * is seen.  The workspace has at least mlk_latent_attend_workspace() bytes
  * (device memory, 16-byte aligned). */
 size_t mlk_latent_attend_workspace(void);
 int mlk_latent_attend(const MlkLatentBatch *batch, int type, const void *q,

@@ -590,3 +590,51 @@ def test_calls_from_two_threads(device):
     for t in threads:
         t.join()
     assert not failed, failed
+
+
+def with_bad_key(cache, s, at, column, bad):
+    v = cache.get(s, at)
+    v[column] = bad
+    cache.put(s, at, v)
+
+
+@pytest.mark.parametrize("cache_type", [MLK_BF16, MLK_FP4])
+@pytest.mark.parametrize("dtype", [MLK_F32, MLK_BF16])
+@pytest.mark.parametrize("bad", [np.nan, np.inf, -np.inf])
+@pytest.mark.parametrize("heads,rows", [(3, 2), (16, 70)])
+def test_attend_keys_that_are_not_finite_are_told_by_every_head(device, workspace, dtype, cache_type, bad, heads, rows):
+    """Whatever the sign of a head's score: all of its results are NaN where a row sees the key, in
+    the latent row or the rope row, at a sequence's beginning, middle and end; the others are right."""
+    rng = np.random.default_rng(34)
+    pairs = [(700, rows), (1, 1), (0, 1), (90, rows)]
+    for column in (100, 512, 540, 575):
+        for s, at in ((0, 0), (0, 330), (0, 698), (0, 699), (1, 0), (3, 89)):
+            cache = L.Cache(rng, cache_type, pairs, table_extra=32).fill(rng)
+            clean = cache.get(s, at)
+            with_bad_key(cache, s, at, column, bad)
+            got, q, scale = run_attend(rng, cache, dtype, heads, workspace)
+            sees = np.array([t == s and j >= at for _, t, j in cache.each_row()])
+            assert np.isnan(got[sees]).all(), (column, s, at)
+            cache.put(s, at, clean)
+            want, mass, score = L.attend(cache, q, heads, scale)
+            room = L.attend_tolerance(cache, want, mass, score, dtype)
+            assert np.all(np.abs(got - want)[~sees] <= room[~sees]), (column, s, at)
+
+
+@pytest.mark.parametrize("cache_type", [MLK_BF16, MLK_FP4])
+@pytest.mark.parametrize("dtype", [MLK_F32, MLK_BF16])
+@pytest.mark.parametrize("bad", [np.nan, np.inf, -np.inf])
+@pytest.mark.parametrize("rows", [1, 70])
+def test_attend_queries_that_are_not_finite(device, workspace, dtype, cache_type, bad, rows):
+    """Such a query's results are NaN, over one key as over many; a row that sees none is zero."""
+    rng = np.random.default_rng(35)
+    cache = L.Cache(rng, cache_type, [(700, rows), (1, 1), (0, 1)], table_extra=32).fill(rng)
+    for column in (7, 520):
+        q = rng.standard_normal((cache.rows, 16, 576))
+        fine = np.ones((cache.rows, 16), bool)
+        for r, h in ((0, 1), (rows - 1, 15), (rows, 0), (rows, 9), (rows + 1, 4)):
+            q[r, h, column] = bad
+            fine[r, h] = r == rows + 1
+        got, _, _ = run_attend(rng, cache, dtype, 16, workspace, q=q)
+        assert np.isfinite(got[fine]).all() and np.isnan(got[~fine]).all()
+        assert np.all(got[rows + 1] == 0)
