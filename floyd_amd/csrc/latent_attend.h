@@ -287,9 +287,15 @@ template <bool BF16> __device__ __forceinline__ void store4(void *out, long at, 
 }
 
 // The reference that exponents are taken to moves up only when a score is this far above
-// it (in powers of 2): p stays below 2^24 and sums lose nothing by that (2^31 keys' are finite for
-// values below 2^72), and most steps need not scale what is summed.
+// it (in powers of 2): p stays below 2^25 and sums lose nothing by that (2^31 keys' are finite for
+// values below 2^71), and most steps need not scale what is summed.
 constexpr float kSlack = 24.0f;
+// exp2(q . k scale - top) takes the product and the difference in one rounding, `top` is a rounded
+// product: from here on they may be more than 1 apart, at 2^32 more than 2^7, which makes 0 or an
+// infinity of the largest p.
+constexpr float kLarge = 0x1p25f;
+// (a score of -inf would be a key without weight: a score that is not finite is NaN)
+__device__ __forceinline__ float large_score(float s) { return fabsf(s) < INFINITY ? s : NAN; }
 
 // Joins the tile of record blockIdx.x: its sums are in part 2 first + 1 and in parts 2w of
 // the workgroups w after the first.  128 threads take a column's values, and TEAMS such teams

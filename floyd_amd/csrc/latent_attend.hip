@@ -264,15 +264,22 @@ __global__ __launch_bounds__((kWavesOf<FP4> * kWave), 1) void latent_attend_kern
                         hidden[i] = key0 + 4 * g + i >= limit;
                     }
                 }
-                if (__any(fmaxf(fmaxf(fabsf(sc[0]), fabsf(sc[1])), fmaxf(fabsf(sc[2]), fabsf(sc[3]))) * fabsf(p.scale) == INFINITY)) {
-                    // (a score of -inf would be a key without weight)
+                float scale = p.scale, high = -INFINITY;
+                const auto set_high = [&] {
+                    high = -INFINITY;
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) sc[i] = fabsf(sc[i] * p.scale) < INFINITY ? sc[i] : NAN;
-                }
-                float high = -INFINITY;
+                    for (int i = 0; i < 4; ++i) high = fmaxf(high, hidden[i] ? -INFINITY : sc[i] * scale);
+                };
+                set_high();
+                const float largest = fabsf(scale) * fmaxf(fmaxf(fabsf(sc[0]), fabsf(sc[1])), fmaxf(fabsf(sc[2]), fabsf(sc[3])));
+                if (__any(high > top + kSlack || largest >= kLarge)) {
+                    if (__any(largest >= kLarge)) {
+                        // (the product that `top` is of is the one that is subtracted from)
 #pragma unroll
-                for (int i = 0; i < 4; ++i) high = fmaxf(high, hidden[i] ? -INFINITY : sc[i] * p.scale);
-                if (__any(high > top + kSlack)) {
+                        for (int i = 0; i < 4; ++i) sc[i] = large_score(sc[i] * scale);
+                        scale = 1.0f;
+                        set_high();
+                    }
                     const float next = fmaxf(top, groups_max(high));
                     const float by = top == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(top - next);
                     const bool begun = __any(top != -INFINITY);  // (else there is nothing yet, or NaN)
@@ -292,7 +299,7 @@ __global__ __launch_bounds__((kWavesOf<FP4> * kWave), 1) void latent_attend_kern
                 float prob[4];
 #pragma unroll
                 for (int i = 0; i < 4; ++i)
-                    prob[i] = hidden[i] ? 0.0f : __builtin_amdgcn_exp2f(fmaf(sc[i], p.scale, -to));
+                    prob[i] = hidden[i] ? 0.0f : __builtin_amdgcn_exp2f(fmaf(sc[i], scale, -to));
                 if constexpr (BF16) {
                     bf16x4 r;
 #pragma unroll

@@ -305,12 +305,15 @@ template <bool FP4> __global__ __launch_bounds__(kThreads, 1) void latent_wide_k
                 float high = score[0], low = score[0];
 #pragma unroll
                 for (int i = 1; i < 16; ++i) high = fmaxf(high, score[i]), low = fminf(low, score[i]);
-                if (__any(fmaxf(fabsf(high), fabsf(low)) * fabsf(scale) == INFINITY)) {
-                    // (a score of -inf would be a key without weight)
+                if (__any(fmaxf(fabsf(high), fabsf(low)) * fabsf(scale) >= kLarge)) {
+                    // (the product that `top` is of is the one that is subtracted from)
 #pragma unroll
-                    for (int i = 0; i < 16; ++i) score[i] = fabsf(score[i] * scale) < INFINITY ? score[i] : NAN;
+                    for (int i = 0; i < 16; ++i) score[i] = large_score(score[i] * scale);
+                    high = scale >= 0 ? high * scale : low * scale;
+                    scale = 1.0f;
+                } else {
+                    high = scale >= 0 ? high * scale : low * scale;
                 }
-                high = scale >= 0 ? high * scale : low * scale;
                 const unsigned bad = (unsigned)uniform((int)(bad4[0] | bad4[1] | bad4[2] | bad4[3]));
                 if (bad || key0 + kStepKeys > least) {
                     // Keys that not every column sees, or that have no place: those that a column

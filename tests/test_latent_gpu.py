@@ -638,3 +638,30 @@ def test_attend_queries_that_are_not_finite(device, workspace, dtype, cache_type
         got, _, _ = run_attend(rng, cache, dtype, 16, workspace, q=q)
         assert np.isfinite(got[fine]).all() and np.isnan(got[~fine]).all()
         assert np.all(got[rows + 1] == 0)
+
+
+@pytest.mark.parametrize("cache_type", [MLK_BF16, MLK_FP4])
+@pytest.mark.parametrize("dtype", [MLK_F32, MLK_BF16])
+@pytest.mark.parametrize("rows", [1, 70])
+@pytest.mark.parametrize("power", [20, 27, 34, 50, 90])
+def test_attend_scores_far_above_a_last_place(device, workspace, dtype, cache_type, rows, power):
+    """Scores of 2^power and more, whose last place is many times the slack of a softmax: the
+    largest one's key is the result, wherever it lies."""
+    rng = np.random.default_rng(36)
+    cache = L.Cache(rng, cache_type, [(300, rows), (1, 1)], table_extra=32).fill(rng)
+    for sign in (1, -1):
+        q = rng.standard_normal((cache.rows, 16, 576))
+        got, v, scale = run_attend(rng, cache, dtype, 16, workspace, q=q, scale=sign * 2.0 ** power)
+        for r, s, j in cache.each_row():
+            k = cache.keys(s, j + 1)
+            x = v[r] @ k.T * scale
+            order = np.sort(x, 1)
+            # a score is off by 2 * 1728 additions' half last places of the magnitudes added
+            off = 2 * 1728 * U.HALF_F32 * (np.abs(v[r]) @ np.abs(k).T).max(1) * abs(scale)
+            clear = order[:, -1] - order[:, -2] > 2 * off + 200 if j else np.ones(16, bool)
+            want = k[x.argmax(1), :512]
+            # p v / p: three f32 roundings, then the result's
+            half = U.HALF_BF16 if dtype == MLK_BF16 else U.HALF_F32
+            assert np.all(np.abs(got[r] - want)[clear] <= (np.abs(want) * (half + 4 * U.HALF_F32))[clear]), (r, s)
+            assert np.all(np.abs(got[r]) <= np.abs(k[:, :512]).max(0) * (1 + 2 * half + 8 * U.HALF_F32))
+            assert clear.any()
