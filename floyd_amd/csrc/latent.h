@@ -19,6 +19,9 @@ constexpr int kLatentMaxHeads = 1024;
 constexpr int kLatentRowThreads = 256, kLatentGatherRows = 4;
 constexpr int kLatentMaxAppend = 0xFFFFFFFFu / kLatentRowThreads;
 constexpr int kLatentMaxGather = kLatentMaxAppend * kLatentGatherRows;
+// Sequences are gone through in 32 bits, a workgroup's threads at a time, and counted with 2^27 tiles
+// of 16 (row, head) pairs.
+constexpr int kLatentMaxSeqs = 1 << 30;
 constexpr int kFp4Group = 32;         // values of a scale
 constexpr int kFp4ScaleBytes = 16;    // bytes of a row's scales
 constexpr int kFp4Bias = 127;         // of a scale byte; 255: its values are NaN

@@ -19,6 +19,7 @@ int check_batch(const char *what, const MlkLatentBatch *b, int rows) {
         return refuse(what, "latent must be a multiple of 64 up to 512, rope a multiple of 16 up to 64");
     if (b->pages <= 0 || b->page_size <= 0 || b->seqs < 0 || b->table_width <= 0)
         return refuse(what, "pages, page_size and table_width must be > 0, seqs >= 0");
+    if (b->seqs > kLatentMaxSeqs) return refuse(what, "seqs must be at most 2^30", kErrSize);
     if (rows < 0) return refuse(what, "rows must be >= 0");
     if (!b->row_starts && rows < b->seqs)
         return refuse(what, "without row_starts every sequence needs a row");

@@ -460,7 +460,8 @@ int latent_attend(const MlkLatentBatch &b, const LatentAttend &p, int cu_count, 
     a.groups = cu_count < most_groups ? cu_count : most_groups;
     const long room = (long)b.table_width * b.page_size;
     a.keys = room < kMostKeys ? (int)room : kMostKeys;
-    // units of more keys where there could be 2^31 of them (a tile has at least a column)
+    // units of more keys where there could be 2^31 of them (a tile has at least a column; tiles are at
+    // most 2^27 + kLatentMaxSeqs)
     const long tiles = (long)p.rows * p.heads / (wide ? Wide::kCols : Narrow::kCols) + b.seqs;
     const int step_shift = wide ? Wide::kStepShift : Narrow::kStepShift;
     a.parts.tiles = tiles <= kMaxTileRecords ? (int)tiles : 0;

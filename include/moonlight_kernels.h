@@ -216,8 +216,8 @@ int mlk_matmul_fp8_grouped(int out_type, const uint8_t *w, const float *ws,
  * Rows of no sequence are left as they were; what a slot holds that several rows
  * claim is one of theirs.
  *
- * Limits: latent a multiple of 64 up to 512, rope a multiple of 16 up to 64; a
- * key from 2^31 - 128 on is behind any table for mlk_latent_attend; rows up to 2^24 - 1
+ * Limits: latent a multiple of 64 up to 512, rope a multiple of 16 up to 64; seqs up to
+ * 2^30; a key from 2^31 - 128 on is behind any table for mlk_latent_attend; rows up to 2^24 - 1
  * for mlk_latent_append (2^26 - 4 for mlk_latent_gather);
  * data 16-byte aligned, other pointers to their values.  Calls queue on the library
  * stream and return, as the fp8 entry points do, with the same rules for

@@ -107,6 +107,15 @@ def test_refused(call, bad, says):
         call(**bad)
 
 
+@pytest.mark.parametrize("call", [append, gather, attend])
+@pytest.mark.parametrize("seqs", [(1 << 30) + 1, (1 << 31) - 1])
+def test_more_sequences_than_are_counted(call, seqs):
+    with pytest.raises(NativeError, match="seqs must be at most"):
+        call(seqs=seqs)
+    with pytest.raises(NativeError, match="no HIP device|not device memory"):
+        call(seqs=1 << 30)
+
+
 def test_null_batch():
     lib = native.load()
     assert lib.mlk_latent_gather(None, MLK_F32, 1, P) == -1 and "batch is null" in native.last_error()
