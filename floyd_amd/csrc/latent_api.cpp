@@ -108,7 +108,8 @@ int mlk_latent_attend(const MlkLatentBatch *batch, int type, const void *q, void
         return refuse(what, "heads must be > 0 and at most 1024");
     if ((long)rows * heads > kMaxPairs)
         return refuse(what, "rows * heads must be below 2^31 - 15", kErrSize);
-    if (!isfinite(scale)) return refuse(what, "scale must be finite");
+    // (times log2(e) it has to be an f32 too)
+    if (!(fabsf(scale) < 0x1p127f)) return refuse(what, "scale must be finite and below 2^127");
     if (rows == 0 || batch->seqs == 0) return kOk;
     if (workspace_bytes < latent_attend_workspace())
         return refuse(what, "the workspace needs " + std::to_string(latent_attend_workspace()) + " bytes");

@@ -263,7 +263,7 @@ int mlk_latent_gather(const MlkLatentBatch *batch, int type, int rows, void *out
 
 /* Attention in the absorbed form: for each head of each token row
  *   out = sum_j p_j latent_j,  p = softmax_j(scale * q . [latent_j | rope_j])
- * over the keys j up to the row's own.  q [rows, heads, latent + rope] and out
+ * over the keys j up to the row's own; |scale| < 2^127.  q [rows, heads, latent + rope] and out
  * [rows, heads, latent] are of `type`.  Scores, sums and results are f32; with
  * MLK_BF16 the p of a key is rounded to bf16 before it is multiplied with its
  * row (the softmax's sum is that of the rounded ones), with MLK_F32 nothing is.

@@ -116,6 +116,14 @@ def test_more_sequences_than_are_counted(call, seqs):
         call(seqs=1 << 30)
 
 
+@pytest.mark.parametrize("scale", [2.0 ** 127, -2.0 ** 127, 2.0 ** 127.8, float("-inf")])
+def test_scales_that_log2_e_takes_past_f32(scale):
+    with pytest.raises(NativeError, match="scale"):
+        attend(scale=scale)
+    with pytest.raises(NativeError, match="no HIP device|not device memory"):
+        attend(scale=np.nextafter(np.float32(2.0 ** 127), np.float32(0)))
+
+
 def test_null_batch():
     lib = native.load()
     assert lib.mlk_latent_gather(None, MLK_F32, 1, P) == -1 and "batch is null" in native.last_error()
