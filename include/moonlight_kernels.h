@@ -213,8 +213,8 @@ int mlk_matmul_fp8_grouped(int out_type, const uint8_t *w, const float *ws,
  * outside [0, pages), or behind the table's last page, is not written and makes
  * the rows that read it NaN; a sequence whose row_starts decrease or leave
  * [0, rows] has no rows, and rows of the others in such a batch are done or left.
- * Rows of no sequence are left as they were; what a slot holds that several rows
- * claim is one of theirs.
+ * Rows of no sequence are left as they were; a slot that several rows of a call claim may hold
+ * parts of each of them.
  *
  * Limits: latent a multiple of 64 up to 512, rope a multiple of 16 up to 64; seqs up to
  * 2^30; a key from 2^31 - 128 on is behind any table for mlk_latent_attend; rows up to 2^24 - 1
@@ -283,7 +283,9 @@ int mlk_latent_attend(const MlkLatentBatch *batch, int type, const void *q,
  * top_logprobs [rows, top] (top 0 .. 32, at most vocab) the most likely tokens,
  * the lower index first among equal ones.  A logit of -inf has probability 0; a row
  * with a NaN, +inf or nothing above -inf has NaN for every result but the ids,
- * from which NaNs are left out (-1 where no logit is left).  Sums are 64 bits.  The workspace (device
+ * from which NaNs are left out (-1 where no logit is left).  Exponentials are f32 and are added 4
+ * (f32 logits) or 8 (bf16) at a time in f32, those near a row's largest one by one, to sums of 64
+ * bits.  vocab is at most 2^22, rows * ceil(vocab / 8192) below 2^24.  The workspace (device
  * memory, 16-byte aligned) has at least mlk_token_logprobs_workspace() bytes, which never
  * fall as rows, vocab or top grow: one of the largest call's serves the smaller ones.  Pointers,
  * streams and overlap as for the latent entry points. */
