@@ -46,7 +46,8 @@ __host__ __device__ constexpr int latent_row_bytes(bool fp4, int latent, int rop
 }
 
 // The token rows of sequence s: rows begin .. begin + count - 1 of the batch, the last one
-// key length - 1.  What the device's memory holds is not trusted.
+// key length - 1.  What the device's memory holds is not trusted; `begin` is below 0 where starts
+// decrease, without which no row belongs to two sequences.
 struct LatentSeq {
     int begin, count;
     int length;
@@ -55,7 +56,7 @@ __device__ __forceinline__ LatentSeq latent_seq(const MlkLatentBatch &b, int s, 
     const int length = b.lengths[s];
     if (!b.row_starts) return {s, s < rows ? 1 : 0, length};
     const int begin = b.row_starts[s], end = b.row_starts[s + 1];
-    return {begin, begin >= 0 && begin < end && end <= rows ? end - begin : 0, length};
+    return {end < begin ? -1 : begin, begin >= 0 && begin < end && end <= rows ? end - begin : 0, length};
 }
 
 // The place of key j >= 0 of sequence s among the rows of all pages; -1: it has none.

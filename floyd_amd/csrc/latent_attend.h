@@ -116,6 +116,7 @@ __device__ __forceinline__ int wave_sum_int(int v) {
 struct Run {
     int seq, offset, begin, length;
     int share, rest;  // workgroups have `share` units each, the first `rest` of them one more
+    bool malformed;   // starts decrease: rows of several sequences could make more units than are counted
     // Of `total` units, dealt to no more workgroups than leaves each 2^least of them: then no run
     // between those of one tile is empty, and a tile has no more parts than pay.
     __device__ __forceinline__ void deal(int total, int groups, int group, int least) {
@@ -148,31 +149,45 @@ template <class Til, int WAVES> __device__ __forceinline__ Run find_run(const Pa
     Run r;
     const LatentSeq mine = seq_of(t);
     int units = units_of(mine), all = units, total = 0;
-    if (t == 0) at[0] = p.b.seqs;  // (no sequence: starts that overlap could make more units than are counted)
+    if (t == 0) at[0] = p.b.seqs;  // (no sequence, until one is found)
+    bool decrease = mine.begin < 0;
+    r.malformed = false;
     if (p.b.seqs <= kThreads) {
         held[t] = mine;
     } else {
-        for (int s = t + kThreads; s < p.b.seqs; s += kThreads) all += units_of(seq_of(s));
-        all = wave_sum_int(all);
+        for (int s = t + kThreads; s < p.b.seqs; s += kThreads) {
+            const LatentSeq seq = seq_of(s);
+            all += units_of(seq);
+            decrease |= seq.begin < 0;
+        }
+        all = __any(decrease) ? -1 : wave_sum_int(all);
         if (lane == 0) sums[wave] = all;
         __syncthreads();
-        for (int w = 0; w < kWaves; ++w) total += uniform(sums[w]);
-        r.deal(total, p.groups, group, kLeast);
+        for (int w = 0; w < kWaves; ++w) {
+            const int units = uniform(sums[w]);
+            r.malformed |= units < 0;
+            total += units;
+        }
+        r.deal(r.malformed ? 0 : total, p.groups, group, kLeast);
+        decrease = false;
     }
     int before = 0;
     for (int s0 = 0;; s0 += kThreads) {
         if (s0) units = units_of(seq_of(s0 + t));
+        const bool none = __any(decrease);
         const int upto = wave_scan(units);
         __syncthreads();
-        if (lane == kWave - 1) sums[wave] = upto;
+        if (lane == kWave - 1) sums[wave] = none ? -1 : upto;
         __syncthreads();
         int first = before + upto - units;
 #pragma unroll
         for (int w = 0; w < kWaves; ++w) {
-            if (w < wave) first += sums[w];
-            before += uniform(sums[w]);
+            const int all = uniform(sums[w]);
+            r.malformed |= all < 0;
+            if (w < wave) first += all;
+            before += all;
         }
-        if (p.b.seqs <= kThreads) r.deal(before, p.groups, group, kLeast);
+        if (p.b.seqs <= kThreads) r.deal(r.malformed ? 0 : before, p.groups, group, kLeast);
         if (r.begin >= first && r.begin < first + units) {
             at[0] = s0 + t;
             at[1] = r.begin - first;
@@ -186,6 +201,16 @@ template <class Til, int WAVES> __device__ __forceinline__ Run find_run(const Pa
     }
     return r;
 }
+
+// Records of workgroups begin without a tile; those of tiles that no workgroup is to do are told, or an
+// earlier call's would be joined.
+__device__ __forceinline__ void begin_records(const Params &p, const Run &run, int group) {
+    if (threadIdx.x) return;
+    if (!p.parts.tiles) p.parts.records[group].first = -1;
+    else if (run.malformed)
+        for (int i = group; i < p.parts.tiles; i += p.groups) p.parts.records[i].first = -1;
+}
+
 // Product step st, lane group g: the first of the 8 values that a lane holds.  Codes are
 // taken 32 at a time, one scale, so four steps go over 128 values.
 template <bool FP4> __device__ __forceinline__ int dim_of(int st, int g) {

@@ -124,7 +124,7 @@ __global__ __launch_bounds__((kWavesOf<FP4> * kWave), 1) void latent_attend_kern
 
     const int group = blockIdx.x;
     const Run run = find_run<Narrow, kWaves>(p, group, held);
-    if (t == 0 && !p.parts.tiles) p.parts.records[group].first = -1;
+    begin_records(p, run, group);
     int left = run.length, offset = run.offset;
     for (int s = run.seq; left > 0 && s < p.b.seqs; ++s, offset = 0) {
         const LatentSeq seq = p.b.seqs <= kThreads ? held[s] : latent_seq(p.b, s, p.rows);

@@ -113,7 +113,7 @@ template <bool FP4> __global__ __launch_bounds__(kThreads, 1) void latent_wide_k
     const int xcd = blockIdx.x % 8, longer = p.groups % 8;
     const int group = xcd * (p.groups / 8) + (xcd < longer ? xcd : longer) + blockIdx.x / 8;
     const Run run = find_run<Wide, kWaves>(p, group, held);
-    if (t == 0 && !p.parts.tiles) p.parts.records[group].first = -1;
+    begin_records(p, run, group);
 
     // Where a lane reads: of keys (queries) their row c, and of 4 keys' 64 bytes its 8; a place in a
     // row is reached by changing bits of these.

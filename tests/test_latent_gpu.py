@@ -665,3 +665,27 @@ def test_attend_scores_far_above_a_last_place(device, workspace, dtype, cache_ty
             assert np.all(np.abs(got[r] - want)[clear] <= (np.abs(want) * (half + 4 * U.HALF_F32))[clear]), (r, s)
             assert np.all(np.abs(got[r]) <= np.abs(k[:, :512]).max(0) * (1 + 2 * half + 8 * U.HALF_F32))
             assert clear.any()
+
+
+@pytest.mark.parametrize("dtype,length", [(MLK_F32, 1 << 20), (MLK_BF16, 1 << 24)])
+def test_attend_leaves_rows_that_sequences_share(device, workspace, dtype, length):
+    """Starts that go back and forth give the same rows to a hundred long sequences, more work than
+    is counted in 32 bits: nothing is done, and nothing that an earlier call left in the workspace
+    becomes a result."""
+    rows, heads, seqs, page = 1024, 16, 200, 1 << 14
+    size = L.item_size(dtype)
+    row = native.latent_row_bytes(MLK_BF16, 512, 64)
+    data = DeviceBuffer.from_array(np.zeros(page * row, np.uint8))
+    tables = DeviceBuffer.from_array(np.zeros((seqs, length // page), np.int32))
+    rng = np.random.default_rng(37)
+    qb, qat = put(L.typed(dtype, rng.standard_normal((rows, heads, 576)))[0])
+    lengths, starts = DeviceBuffer(4 * seqs), DeviceBuffer(4 * (seqs + 1))
+    batch = native.LatentBatch(MLK_BF16, data, 512, 64, 1, page, seqs, tables, length // page, lengths, starts)
+    for far, begins in ((3000, [0] + [rows - 24] * seqs), (length, [0, rows] * (seqs // 2) + [0])):
+        lengths.upload(np.full(seqs, far, np.int32))
+        starts.upload(np.array(begins, np.int32))
+        out = Out(rows * heads * 512 * size)
+        native.latent_attend(batch, dtype, qat, out.ptr, rows, heads, 0.1, workspace)
+        got = out.get(np.uint8, (rows, heads * 512 * size))
+        done = rows - 24 if far == 3000 else 0
+        assert np.all(got[:done] == 0) and np.all(got[done:] == out.fill)
