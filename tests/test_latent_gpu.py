@@ -689,3 +689,39 @@ def test_attend_leaves_rows_that_sequences_share(device, workspace, dtype, lengt
         got = out.get(np.uint8, (rows, heads * 512 * size))
         done = rows - 24 if far == 3000 else 0
         assert np.all(got[:done] == 0) and np.all(got[done:] == out.fill)
+
+
+@pytest.mark.parametrize("cache_type", [MLK_BF16, MLK_FP4])
+def test_many_pairs_past_32_bits(device, workspace, cache_type):
+    """A prompt's chunk over pages more than 2^32 bytes into the cache."""
+    rng = np.random.default_rng(38)
+    rows, heads, length, page = 140, 16, 2600, 1024
+    row = native.latent_row_bytes(cache_type, 512, 64)
+    pages = (1 << 32) // (page * row) + 40
+    cache = L.Cache(rng, cache_type, [(length, rows)], page_size=page, table_extra=0).fill(rng)
+    data = DeviceBuffer(pages * page * row)
+    places = np.array([[pages - 1, 3, pages - 20]], np.int32)
+    for at, held in zip(places[0], cache.tables[0]):
+        data.upload(cache.pool[held].reshape(-1), int(at) * page * row)
+    tables = DeviceBuffer.from_array(places)
+    lengths, starts = DeviceBuffer.from_array(cache.lengths), DeviceBuffer.from_array(cache.starts)
+    batch = native.LatentBatch(cache_type, data, 512, 64, pages, page, 1, tables, 3, lengths, starts)
+    raw, q = L.typed(MLK_BF16, rng.standard_normal((rows, heads, 576)))
+    qb, qat = put(raw)
+    out = Out(rows * heads * 512 * 2)
+    native.latent_attend(batch, MLK_BF16, qat, out.ptr, rows, heads, 0.07, workspace)
+    got = L.values(MLK_BF16, out.get(np.uint8, rows * heads * 512 * 2)).reshape(rows, heads, 512)
+    want, mass, score = L.attend(cache, q, heads, F64(F32(0.07)))
+    assert np.all(np.abs(got - want) <= L.attend_tolerance(cache, want, mass, score, MLK_BF16))
+
+
+@pytest.mark.parametrize("cache_type", [MLK_BF16, MLK_FP4])
+@pytest.mark.parametrize("starts", [True, False])
+def test_many_pairs_of_more_sequences_than_threads(device, workspace, cache_type, starts):
+    """Many heads of a few rows each, some sequences without rows or keys."""
+    rng = np.random.default_rng(39)
+    counts = rng.integers(0, 4, 300) if starts else np.ones(300, int)
+    pairs = [(int(rng.integers(0, 40)), int(n)) for n in counts]
+    pairs[7] = (1500, pairs[7][1])
+    cache = L.Cache(rng, cache_type, pairs, starts=starts, table_extra=8).fill(rng)
+    check_attend(rng, cache, MLK_BF16, 128, workspace)
