@@ -328,8 +328,8 @@ __device__ __forceinline__ float large_score(float s) { return fabsf(s) < INFINI
 // microsecond, so as many as can are under way at once: four teams where all workgroups are
 // resident that way, and 16 loads a thread for the few tiles of small batches, whose parts are
 // many; else 4 loads, for what a thread asks for beyond the last part is read again for nothing
-// (17 tiles of about 15 parts 9.6 us with 16 loads, 6.1 with 4; 128 tiles of 64 columns and of two
-// or three parts 16.3 and 11.6).
+// (17 tiles of about 15 parts 9.6 us with 16 loads, 6.1 with 4; 80 tiles of 64 columns and of about
+// four parts 16.3 and 11.6).
 constexpr int kTeam = kLatentMax / 4;
 constexpr int kMaxTeams = 4;
 template <class Til, bool BF16, int TEAMS, int LOADS> __global__ __launch_bounds__((kTeam * TEAMS)) void latent_join_kernel(Params p) {

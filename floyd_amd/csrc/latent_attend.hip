@@ -29,14 +29,24 @@
 // entered a step early rather than with a copy of their loads before them, and unrolled
 // only where registers are counted.
 //
-// Measured with 16 heads (this kernel, then the join): 16 rows over 16000 .. 16384 bf16 keys each
-// 62-65 and 6 us, 4.6-4.8 TB/s; a kernel that only reads the same rows, a key's 64 bytes by four
-// lanes, takes 54 and one that reads 1 KB runs 47-49: what bounds it is the reads, by the order
-// that the operand asks for, and the start.  64 rows over 4-bit keys, 159 MB, 48 and 6 us; reading
-// alone takes 31: two waves a SIMD whose products, codes' conversion and softmax, one after the
-// other, keep the matrix unit busy a quarter of the time.  One row over 4096 bf16 keys 10 and 5.5,
-// 17 rows of f32 queries over 4-bit keys 20 and 6: some seven trips to memory that depend on each
-// other, a microsecond each, with lengths and tables among them.
+// With bf16 queries a key's p is rounded to bf16, as one operand of the second product: in two bf16
+// parts, which add up to 16 bits of it, 64 rows over 4-bit keys take 58 us instead of 53 and 16 long
+// rows over bf16 keys 72 instead of 71, and the results come as near to those in 64 bits as their own
+// rounding lets them, 0.00159 and 0.00166 of their norm; with the one part it is 0.00172 and 0.00176.
+//
+// Measured with 16 heads (calls without the join, and what it adds): 16 rows over 16000 .. 16384
+// bf16 keys each, 299 MB, 66 and 5 us, 4.5 TB/s; a kernel that only reads the same rows, a key's 64
+// bytes by four lanes, takes 54, one that reads 1 KB runs 47-49 and a plain read 43: what bounds it is
+// the reads, by the order that the operand asks for, and the start.  64 rows over 4-bit keys, 159 MB,
+// 48 and 5; reading alone takes 31, a plain read 23: two waves a SIMD whose products, codes'
+// conversion (twice a step, once for each product) and softmax follow each other keep the matrix
+// unit busy 26 % of the time and the vector units 34 %.  The scores of a step beside the softmax of
+// the one before are not tried: the kernel has 243 of 256 registers, 128 of them sums.  One row over
+// 4096 bf16 keys 10 and 6, 17 rows of f32 queries over 4-bit keys 21 and 6: some seven trips to
+// memory that depend on each other, a microsecond each, with lengths and tables among them.
+// f32 queries and probabilities take 182 products of 16 columns by 16 keys: chunks of 32, 64, 96 and
+// 128 rows over 3000 .. 4096 keys 190 us over 4-bit keys and 290 over bf16 ones, whose registers leave
+// one wave a SIMD instead of two: the matrix unit is busy 54 and 33 % of the time.
 #include "latent_attend.h"
 
 namespace mlh {
@@ -430,13 +440,19 @@ template <bool FP4, bool BF16, bool FULL> int launch(const Params &p, hipStream_
 
 // Whether the wide kernel is taken, for bf16 queries of full rows: it reads keys once for 64 columns
 // and not for 16, but begins and ends a tile more slowly.  The host knows the pairs, the sequences
-// and the keys that a table holds.  Calls in us, wide and narrow, 3000 .. 4096 keys a sequence:
-//   bf16 keys   4 sequences of 128 pairs 40 and 35, of 256 46 and 49, of 512 45 and 62, of 2048
-//               92 and 181; 16 of 48 44 and 41, of 64 44 and 45; 64 of 64 94 and 101
-//   4-bit keys  4 of 256 45 and 38, of 512 44 and 43, of 1024 56 and 65, of 2048 86 and 126;
-//               32 of 128 59 and 58; 64 of 64 72 and 58
-// One sequence of 4096 pairs over 256 keys: bf16 27 and 22, 4 bits 27 and 17; of 8192 pairs over
-// 512 bf16 keys 39 and 55.  Queries at 16-byte addresses, which it copies so.
+// and the keys that a table holds.  Calls in us, wide and narrow, by the pairs of each sequence (16 to
+// a row), 3000 .. 4096 keys:
+//   bf16 keys   4 sequences of 128 41 and 39, of 256 42 and 53, of 512 49 and 82, of 2048 103 and
+//               284; 16 of 48 46 and 50, of 64 49 and 56; 32 of 32 63 and 61, of 64 65 and 98; 64 of
+//               64 97 and 177
+//   4-bit keys  4 of 128 39 and 29, of 256 40 and 37, of 512 48 and 54, of 2048 99 and 152; 16 of 64
+//               44 and 38; 32 of 32 49 and 38, of 64 53 and 54, of 128 69 and 93; 64 of 64 75 and 95
+// One sequence of 4096 pairs over 256 keys: bf16 27 and 21, 4 bits 27 and 16; of 8192 pairs over
+// 512 keys 37 and 53, 37 and 36.  One of 2048 pairs over 4096 keys beside 63 of 16: bf16 110 and 122,
+// 4 bits 88 and 77; one of 8192 beside them 184 and 325, 150 and 189.  So the rule errs by a tenth to a
+// fifth near its borders, where one sequence's pairs are far from the average, and by more for prompts
+// of few keys whose table is wide: the host does not know lengths.  Queries at 16-byte addresses,
+// which it copies so.
 static bool wide_pays(const MlkLatentBatch &b, const LatentAttend &p) {
     const long pairs = (long)p.rows * p.heads, few = b.type == MLK_FP4 ? 2 : 1;
     return p.bf16 && b.latent == kLatentMax && b.rope == kLatentRopeMax && (reinterpret_cast<uintptr_t>(p.q) & 15) == 0 &&

@@ -142,10 +142,12 @@ __device__ __forceinline__ unsigned row_max(unsigned v) {
 
 // One token row a workgroup.  What it reads of the row is asked for at once, beside the way to
 // its place (starts and length, then table, a microsecond each).  Queries: 32 threads for the
-// pairs of a head, 8 heads a pass.  4095 bf16 rows with 16 heads into 4 bits, 29 MB, take 13-14 us
-// (2.1 TB/s; the library's sine and cosine, loads in turn and codes in 64 bits 19): what bounds it
-// is 64-bit arithmetic, at a half to a quarter of 32 bits' rate, and what each workgroup waits for
-// one after the other.  One row 3.1 us: a launch and those trips.
+// pairs of a head, 8 heads a pass.  4095 bf16 rows with 16 heads into 4 bits, 23.1 MB, take 13-14 us
+// (1.7 TB/s; the library's sine and cosine, loads in turn and codes in 64 bits 19), into bf16 rows, 26
+// MB, 12: 8 workgroups a CU, in two rounds, whose waves wait 45 % of their time, for those trips one
+// after the other and for the wave that makes sine and cosine.  The vector units are busy 33 % of the
+// time; a fifth of their instructions are 64-bit arithmetic.  One row 3.0-3.2 us: a launch and those
+// trips.
 constexpr int kPairLanes = kLatentRopeMax / 2, kPassHeads = kThreads / kPairLanes;
 constexpr int kTurns = 2;  // passes on their way at once
 template <bool BF16, bool FP4>
@@ -240,8 +242,8 @@ __global__ __launch_bounds__(kThreads) void latent_append_kernel(MlkLatentBatch 
 
 typedef unsigned u32x4_any __attribute__((ext_vector_type(4), aligned(2)));
 
-// One token row a wave, 8 values a lane and step.  67 MB of ragged f32 rows 14 us (4.8 TB/s; a large
-// copy reaches 5.1), 8192 rows of 4 bits, 13 MB, 5.3 (the way to a row and from it, three trips).
+// One token row a wave, 8 values a lane and step.  67 MB of ragged f32 rows 13.5-14 us (4.8-5.0 TB/s; a
+// large copy reaches 5.2), 8192 rows of 4 bits, 13 MB, 5.3 (the way to a row and from it, three trips).
 template <bool BF16, bool FP4>
 __global__ __launch_bounds__(kThreads) void latent_gather_kernel(MlkLatentBatch b, int rows, void *to) {
     using T = typename Elem<BF16>::type;

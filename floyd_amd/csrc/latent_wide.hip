@@ -12,18 +12,25 @@
 //     every 8, of a column, and so the operands of this product have them.
 // (With sums split by columns and keys, as the scores are, every wave holds all 512 of 32 columns,
 // 256 registers, reads V^T twice as often and moves all of it where the reference moves: 99 us
-// where this takes 74.)
+// where this split took 84.)  P is rounded to bf16, as one operand of the second product: a second
+// part would double its matrix instructions and P's way through LDS; the results are 0.00177 of their
+// norm off those in 64 bits, of which their own rounding is 0.00166.
 //
-// Measured: 4 sequences of 128 rows and 16 heads over 3000 .. 4096 keys, 41 GFLOP, bf16 keys 74 and
-// the join 11 us, 4-bit ones 70 and 11; 256 rows over 8192 keys 95 and 11 (a large library product
-// reaches 1190 TFLOP/s, and products on random values in registers alone 1675 once they run long:
-// the clock falls).  Of a step's 5000 cycles 2200 are products.  The rest is the softmax between
-// the two, the way of P through LDS with its two meetings, and bf16 rows' copies, which S waits
-// for here and there (36 products 2100 cycles, over 4-bit keys 1500); of a workgroup's 28 steps
-// the beginning takes 4 us (queries, pages and first keys), an edge 3, the 128 KB of a part 3.5.
+// Measured, calls over 3000 .. 4096 keys with the join, which is 11 us of the first: four sequences of
+// 32, 64, 96 and 128 rows of 16 heads (41 GFLOP, 18.5 steps a workgroup) bf16 keys 79 us, 4-bit ones
+// 75; four of 128 rows (62 GFLOP, 28 steps) 103 and 99; one of 256 rows over 8192 keys (72 GFLOP, 32
+// steps) 107 and 101.  (A large library product reaches 1150-1190 TFLOP/s, and products on random
+// values in registers alone 1675 once they run long: the clock falls.)  The matrix unit is busy 22 %
+// of the first one's time.  By cycle stamps, with which the call takes a tenth more, a wave of it lives
+// 129 000 cycles at 2.2 GHz, the longest 17 % more.  Its steps are 99 000, 5400 each, of which 2200 are
+// products: S 2400 with the bf16 rows' copies among them (4-bit keys 2000), edges and the search for
+// the largest 290, exponentials 570, the moved reference 370 on average, two meetings 410, O 1350
+// (2000 with the 4-bit keys' conversion).  What is not steps: the run and tiles found 6000, queries and
+// first keys 13 000, results 10 500.
 // Copies in the second product's time and more operands ahead made nothing of it faster; steps of
 // 32 keys in three places, with the softmax beside the second product's instructions and one
-// meeting a step, took 80 us: what a step waits for at its beginning then comes twice as often.
+// meeting a step, took 80 us where this took 74: what a step waits for at its beginning then comes
+// twice as often.
 #include "latent_attend.h"
 
 namespace mlh {

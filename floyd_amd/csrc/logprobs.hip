@@ -15,13 +15,13 @@
 // compared as one whole number, all different.
 //
 // exp(d) is the hardware's 2^(d log2 e): d and the product are rounded to f32, which puts a
-// term off by 2.1 |d| 2^-24 of itself.  That and the rest is 12 operations a value, what
-// the vector units do of bf16 logits in the time that the memory takes to bring them.
+// term off by 2.1 |d| 2^-24 of itself.
 //
-// Measured, pieces and join: 512 bf16 rows of 163840 logits 34 and 5 us (4.9 TB/s, what a copy
-// of memory reaches), 61 f32 rows of 50021 with 20 likely tokens 12 and 5.4 (without them 10 in
-// all: the vector units, in what it takes to choose and order 20 of a piece), one f32 row of
-// 163840 with 5 likely tokens 5.6 and 5.0 (two launches and the trips to memory of each).
+// Measured, calls without the join and what it adds: 512 bf16 rows of 163840 logits, 168 MB, 36-40 and 2
+// us, where a plain read takes 24: 14 vector instructions a logit, which keep the vector units busy
+// 82 % of the time.  61 f32 rows of 50021 with 20 likely tokens 11.5 and 5.8 (without them 10 in all:
+// what it takes to choose and order 20 of a piece, waves waiting 57 % of their time), one f32 row of
+// 163840 with 5 likely tokens 6.8 and 4.2 (two launches and the trips to memory of each).
 #include "bf16.h"
 #include "latent.h"
 #include "mlh_device.h"
